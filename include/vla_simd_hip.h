@@ -399,6 +399,108 @@ VLA_API int32_t vla_dense_linear_dev(float* out, int32_t ldo, const float* x, in
                                      int32_t N, int32_t K, int32_t act, int32_t accumulate,
                                      float alpha, void* stream);
 
+/* ------------------------------------- decoders with several sequences -- */
+/* What a decoder needs to serve several prompts at once (no counterpart in the
+ * reference, which runs one sequence in fp32): norms and rotation of queries
+ * and keys, attention over packed prompts, and a cache of 4-bit keys and values
+ * with the attention that reads it. Device forms only. Rows are [tokens,
+ * heads * head_dim] of one type (vla_dtype) with a stride in values, 16-byte
+ * aligned; sums, statistics and angles are held in 32 bits or more and a result is
+ * rounded to its type once.
+ *
+ * Sequences are packed: rows start[s] .. start[s + 1] - 1 belong to sequence s, with
+ * start [n_seqs + 1] int32 on the device, ascending from 0. Rows behind
+ * start[n_seqs] are neither read nor written. The host does not see the offsets,
+ * lengths and page tables; kernels clamp them to the sizes given here, so that wrong
+ * ones give wrong values but never an access outside the buffers. */
+typedef enum { VLA_F32 = 0, VLA_BF16 = 1, VLA_F16 = 2 } vla_dtype;
+
+/* Per token and head, x / sqrt(mean(x^2) + eps) * weight (weight [head_dim] fp32,
+ * NULL: x itself), then the NeoX rotation of the pairs (i, i + head_dim / 2) by the
+ * angle pos[axis of i][token] * base^(-2 i / head_dim). sections (host, [n_axes]) gives
+ * how many of the head_dim / 2 pairs each axis has, in their order: one axis is
+ * vla_rope_neox_dev's rotation, three (time, height, width) serve images and video.
+ * pos: n_axes rows of seq int32 at stride ld_pos (device). q_out and k_out may be q
+ * and k themselves, else they overlap nothing that is read. n_q or n_kv may be 0.
+ * head_dim a multiple of 8 up to 256, n_axes up to 8. */
+VLA_API int32_t vla_qk_norm_rope_dev(void* q_out, int64_t ldqo, void* k_out, int64_t ldko,
+                                     const void* q, int64_t ldq, const void* k, int64_t ldk,
+                                     const float* q_weight, const float* k_weight, float eps,
+                                     const int32_t* pos, int64_t ld_pos, const int32_t* sections,
+                                     int32_t n_axes, float base, int32_t seq, int32_t n_q,
+                                     int32_t n_kv, int32_t head_dim, int32_t dtype, void* stream);
+
+/* Attention of packed sequences: query i of a sequence with len_q queries and len_k
+ * keys sees its keys j <= i + len_k - len_q (causal != 0), or all of them; kv head =
+ * h / (n_q / n_kv). A query that sees no key gets zeros (vla_attention_dev gives the mean
+ * of V there: it masks keys of one sequence, here there may be none); a key
+ * that a query does not see adds nothing to it, infinities and NaN included.
+ * k_start NULL: the keys are packed as the queries. total_q and total_k are the
+ * buffers' rows. head_dim a multiple of 8 up to 256. In 16-bit types the softmax
+ * weights are rounded to that type for the product with V. */
+VLA_API int32_t vla_packed_attention_dev(void* out, int64_t ldo, const void* Q, int64_t ldq,
+                                         const void* K, int64_t ldk, const void* V, int64_t ldv,
+                                         const int32_t* q_start, const int32_t* k_start,
+                                         int32_t n_seqs, int32_t total_q, int32_t total_k,
+                                         int32_t n_q, int32_t n_kv, int32_t head_dim, float scale,
+                                         int32_t causal, int32_t dtype, void* stream);
+
+/* A paged cache of keys and values in 4 bits. cache: n_pages pages of
+ * vla_kv4_page_bytes bytes (16-byte aligned), each page_size tokens (a multiple of
+ * 32 up to 2048) of all kv heads:
+ *   K codes  [n_kv][page_size][head_dim / 2] bytes, value 2 i in the low half of byte i
+ *   V codes  the same
+ *   K scales [n_kv][head_dim / 32][page_size] bytes
+ *   V scales the same
+ * 32 neighbouring values share the scale 2^(byte - 127), with the smallest exponent
+ * >= -100 for which the largest magnitude is <= 7 * 2^e; a code is a sign and one of
+ * 0, 0.5, 1, 1.5, 2, 3, 4, 6, the nearest, ties to the even code. A block with an
+ * infinity or a NaN has byte 255 and reads as NaN. head_dim 32, 64, 96, 128, 192 or 256.
+ * table (device): a row of ld_table page numbers per sequence, tokens in order. A
+ * number outside [0, n_pages) or a token behind the table's row names no page: append
+ * drops its rows, gather and attention read NaN. Sequences may share pages that
+ * neither appends to. -1 for shapes outside these limits. */
+VLA_API int64_t vla_kv4_page_bytes(int32_t n_kv, int32_t head_dim, int32_t page_size);
+/* Byte offset in the cache of the 16 code bytes (part 0 K, 1 V) or of the scale byte
+ * (part 2 K, 3 V) of a token's head and block of 32 values, for a table row in
+ * host memory; -1 where there is none. */
+VLA_API int64_t vla_kv4_offset(int32_t n_kv, int32_t head_dim, int32_t page_size, int32_t n_pages,
+                               const int32_t* table_row, int32_t ld_table, int64_t token,
+                               int32_t part, int32_t head, int32_t block);
+/* Writes packed rows K, V [total, n_kv * head_dim] as the newest tokens of their
+ * sequences: lens [n_seqs] (device) counts a sequence's tokens with them, so row i of n
+ * becomes token lens[s] - n + i. */
+VLA_API int32_t vla_kv4_append_dev(void* cache, int32_t n_pages, int32_t page_size, const void* K,
+                                   int64_t ldk, const void* V, int64_t ldv, const int32_t* table,
+                                   int32_t ld_table, const int32_t* lens, const int32_t* start,
+                                   int32_t n_seqs, int32_t total, int32_t n_kv, int32_t head_dim,
+                                   int32_t dtype, void* stream);
+/* Reads cached tokens back as packed rows: row i of sequence s is its token first[s] + i
+ * (first [n_seqs] on the device, NULL: 0). A prompt whose beginning is cached runs
+ * through vla_packed_attention_dev this way. */
+VLA_API int32_t vla_kv4_gather_dev(void* K, int64_t ldk, void* V, int64_t ldv, const void* cache,
+                                   int32_t n_pages, int32_t page_size, const int32_t* table,
+                                   int32_t ld_table, const int32_t* start, const int32_t* first,
+                                   int32_t n_seqs, int32_t total, int32_t n_kv, int32_t head_dim,
+                                   int32_t dtype, void* stream);
+/* Attention of the newest tokens over the cache: of the n query rows of sequence s
+ * (q_start; NULL: one each, row s), row i sees the keys j < lens[s] - n + i + 1. Rows that
+ * see no key get zeros. max_new and max_len are upper bounds of n and lens that choose
+ * the launch: too small ones cost time, not values. The key axis is split over blocks
+ * when there are few rows, with the partial results in work
+ * (vla_kv4_attention_work_bytes of the same numbers, 16-byte aligned; a smaller or
+ * null one runs unsplit). Calls that may overlap need a workspace each. */
+VLA_API int64_t vla_kv4_attention_work_bytes(int32_t total_q, int32_t n_seqs, int32_t max_new,
+                                             int32_t max_len, int32_t n_q, int32_t n_kv,
+                                             int32_t head_dim);
+VLA_API int32_t vla_kv4_attention_dev(void* out, int64_t ldo, const void* Q, int64_t ldq,
+                                      const void* cache, int32_t n_pages, int32_t page_size,
+                                      const int32_t* table, int32_t ld_table, const int32_t* lens,
+                                      const int32_t* q_start, int32_t n_seqs, int32_t total_q,
+                                      int32_t max_new, int32_t max_len, int32_t n_q, int32_t n_kv,
+                                      int32_t head_dim, float scale, int32_t dtype, void* work,
+                                      int64_t work_bytes, void* stream);
+
 /* ------------------------------------------------------------ convolution -- */
 /* W8A8 2-D convolution, tcpu::conv2d_i8 (src/ops/conv_ops.h:31-35,
  * src/hal/common/conv.cpp:424-526): x [H, Wd, Cin] fp32 NHWC -> out

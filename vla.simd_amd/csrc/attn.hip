@@ -58,29 +58,6 @@ __device__ __forceinline__ v4f mfma_f32(float a, float b, v4f c) {
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// max / sum of x over the lanes l, l^16, l^32, l^48 (the four 16-lane rows of
-// a wave) with gfx950's row-swap permutes, VALU ops instead of LDS round trips.
-// permlane16_swap(x, x) returns, in every lane, the values of the lane pair
-// {l, l^16} (one from the even row, one from the odd row); permlane32_swap the
-// pair {l, l^32}. The sum adds each pair in either order, which is the same
-// float: the results equal those of x op shfl_xor(x, 16), then 32.
-__device__ __forceinline__ float rows_max(float x) {
-    const unsigned u = __float_as_uint(x);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const unsigned v = __float_as_uint(y);
-    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float rows_sum(float x) {
-    const unsigned u = __float_as_uint(x);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const unsigned v = __float_as_uint(y);
-    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // Orders this wave's LDS accesses (its writes before other lanes' reads) with
 // no block barrier.
 __device__ __forceinline__ void wave_lds_sync() {

@@ -1,0 +1,580 @@
+// packed_attn.hip - attention over packed sequences of different lengths:
+//   out[i] = sum_j softmax_j(scale * q[i] . k[j]) v[j]
+// over the keys j of the query's own sequence that it sees: all of them, or with
+// `causal` those with j <= i + (len_k - len_q), so that the last query sees the last
+// key. A query that sees no key gets zeros; a key that it does not see
+// counts for nothing, whatever it holds (infinities and NaN included).
+//
+// One pass over the keys with the running maximum m and sum l of the softmax; the
+// weights stay in registers. Both products run on the matrix cores with fp32 sums:
+//   S^T = K Q^T  (A: 32 keys, B: 32 queries) leaves in lane n + 32 h, for query n, the
+//                scores of keys 8 (i / 4) + 4 h + i % 4, i = 0..15;
+//   O^T = V^T P^T takes of that lane 8 weights per 16 keys: with the product's
+//                inner index 8 h + j read as key 4 h + j (j < 4) and 8 + 4 h + j - 4, those
+//                are the ones it holds, so no weight moves between lanes.
+//                V^T's operand, 4 keys of one dim per half, is what a
+//                transposed LDS read (ds_read_b64_tr_b16) of row-major V gives.
+//
+// 16-bit types: the weights are rounded to the operands' type for the second product
+// (2^-9 of a weight for bf16, 2^-12 for fp16, each on its own, as large as the
+// rounding of the result); the sum l is of the unrounded ones.
+// fp32: both products on the fp32 matrix cores, nothing rounded.
+
+#include "serving.h"
+#include "wave.h"
+
+#include <cmath>
+
+namespace vla {
+namespace hip {
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef bf16_t v8bf __attribute__((ext_vector_type(8)));
+typedef f16_t v8h __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+template <class T>
+struct Vec8;
+template <>
+struct Vec8<bf16_t> { typedef v8bf type; };
+template <>
+struct Vec8<f16_t> { typedef v8h type; };
+
+__device__ __forceinline__ v16f mfma32(v8bf a, v8bf b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v16f mfma32(v8h a, v8h b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// max / sum of x over the lanes l and l ^ 32
+__device__ __forceinline__ float halves_max(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// What a block works on: query rows [q0, q0 + nq) of the packed buffers, at
+// offset `at` in their sequence, and its keys [k0, k0 + nk).
+struct Job {
+    int q0, nq, at, len_q, k0, nk;
+};
+
+__device__ __forceinline__ int clamp_row(int x, int total) { return x < 0 ? 0 : (x < total ? x : total); }
+
+// The block's tile number -> its job; false when there are fewer tiles. Starts
+// are read clamped to the buffers' rows, a sequence that would end before it
+// begins as empty, so that no offsets can lead out of the buffers. Every wave does the same
+// search, 64 sequences at a time; tiles are counted from the last one of the
+// last sequence, whose queries see the most keys under a causal mask.
+template <int QT>
+__device__ bool find_job(const PackedAttnArgs& a, int tile, Job& job) {
+    const int lane = threadIdx.x & 63;
+    int total = 0;
+    for (int pass = 0; pass < 2; pass++) {
+        int run = 0;
+        const int want = total - 1 - tile;
+        if (pass && want < 0) return false;
+        for (int base = 0; base < a.n_seqs; base += 64) {
+            const int s = base + lane;
+            int q0 = 0, n = 0;
+            if (s < a.n_seqs) {
+                q0 = clamp_row(a.q_start[s], a.total_q);
+                n = clamp_row(a.q_start[s + 1], a.total_q) - q0;
+                if (n < 0) n = 0;
+            }
+            const int tiles = (n + QT - 1) / QT;
+            int incl = tiles;
+            for (int d = 1; d < 64; d <<= 1) {
+                const int o = __shfl_up(incl, d);
+                if (lane >= d) incl += o;
+            }
+            const int sum = __shfl(incl, 63);
+            if (pass && want < run + sum) {
+                const unsigned long long hit = __ballot(run + incl > want);
+                const int l = __ffsll(hit) - 1;
+                const int t = want - run - (__shfl(incl, l) - __shfl(tiles, l));
+                const int sq = base + l;
+                const int start = __shfl(q0, l), len = __shfl(n, l);
+                job.at = t * QT;
+                job.q0 = start + job.at;
+                job.len_q = len;
+                job.nq = len - job.at < QT ? len - job.at : QT;
+                job.k0 = clamp_row(a.k_start[sq], a.total_k);
+                job.nk = clamp_row(a.k_start[sq + 1], a.total_k) - job.k0;
+                if (job.nk < 0) job.nk = 0;
+                return true;
+            }
+            run += sum;
+        }
+        total = run;
+    }
+    return false;
+}
+
+// Blocks of one kv head share its rows, so where the heads divide over the 8
+// XCDs (the hardware deals block i to XCD i % 8) each XCD's L2 gets heads of its own.
+__device__ __forceinline__ void tile_and_head(const PackedAttnArgs& a, int& tile, int& h) {
+    const int b = blockIdx.x;
+    tile = b / a.n_q;
+    const int r = b - tile * a.n_q;
+    h = a.n_q % 8 == 0 ? (r & 7) * (a.n_q >> 3) + (r >> 3) : r;
+}
+
+// ---------------------------------------------------- 16-bit types ----
+
+// LDS rows of HDP values in 16-byte chunks; chunk c of row r lies at c ^ swz(r).
+// 16 rows' reads of one chunk (K) then fall on all 64 banks, and so do the 64-byte
+// pieces of 4 neighbouring rows that a transposed read takes (V).
+template <int HDP>
+__device__ __forceinline__ int swz(int row) {
+    return (HDP == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2) | (row >> 2 & 3);
+}
+
+template <class T, int HDP, int KT>
+__global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(PackedAttnArgs a) {
+    typedef typename Vec8<T>::type v8;
+    constexpr int QT = 128, NK = KT / 32;
+    constexpr int CH = HDP / 8;             // chunks of a row
+    constexpr int LOADS = KT * CH / 256;    // chunks per thread of a K or V tile
+    constexpr int DT = HDP / 32, KS = HDP / 16;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    T* Ks = reinterpret_cast<T*>(smem);     // [2][KT][HDP]
+    T* Vs = Ks + 2 * KT * HDP;
+
+    int tile, head;
+    tile_and_head(a, tile, head);
+    Job job;
+    if (!find_job<QT>(a, tile, job)) return;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int n = lane & 31, hf = lane >> 5;
+    const int hd = a.head_dim;
+    const int kvh = head / (a.n_q / a.n_kv);
+    const T* Kg = static_cast<const T*>(a.K) + (size_t)job.k0 * a.ldk + kvh * hd;
+    const T* Vg = static_cast<const T*>(a.V) + (size_t)job.k0 * a.ldv + kvh * hd;
+
+    const int qi = wave * 32 + n;  // in the tile
+    const bool qok = qi < job.nq;
+    v8 qv[KS];
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const int d = 16 * s + 8 * hf;
+        v8 z = {};
+        if (qok && d < hd) z = *reinterpret_cast<const v8*>(static_cast<const T*>(a.Q) + (size_t)(job.q0 + qi) * a.ldq + head * hd + d);
+        qv[s] = z;
+    }
+    // keys [0, lim) are seen by the lane's query; wave_min/max over the wave's queries
+    const int off = job.nk - job.len_q + job.at + 1;
+    auto limit = [&](int q) {
+        const int e = a.causal ? q + off : job.nk;
+        return e < 0 ? 0 : (e < job.nk ? e : job.nk);
+    };
+    const int lim = qok ? limit(qi) : 0;
+    const int wq_last = wave * 32 + 31 < job.nq ? wave * 32 + 31 : job.nq - 1;
+    const int wave_end = wave * 32 < job.nq ? limit(wq_last) : 0;
+    const int wave_all = wave * 32 < job.nq ? limit(wave * 32) : 0;  // every query of the wave sees keys below
+    const int end = limit(job.nq - 1);
+    const int tiles = (end + KT - 1) / KT;
+
+    uint4 kr[LOADS], vr[LOADS];
+    auto gload = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int e = tid + 256 * i, row = e / CH, d = (e % CH) * 8;
+            int j = t * KT + row;
+            if (j >= end) j = end - 1;  // masked below; keeps the address among the sequence's rows
+            kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+            if (d < hd) {
+                kr[i] = *reinterpret_cast<const uint4*>(Kg + (size_t)j * a.ldk + d);
+                vr[i] = *reinterpret_cast<const uint4*>(Vg + (size_t)j * a.ldv + d);
+            }
+        }
+    };
+    auto lstore = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int e = tid + 256 * i, row = e / CH, c = (e % CH) ^ swz<HDP>(row);
+            *reinterpret_cast<uint4*>(Ks + (buf * KT + row) * HDP + c * 8) = kr[i];
+            *reinterpret_cast<uint4*>(Vs + (buf * KT + row) * HDP + c * 8) = vr[i];
+        }
+    };
+
+    v16f o[DT] = {};
+    float m = -INFINITY, l = 0.0f;
+    const float c2 = a.scale * kLog2e;
+
+    if (tiles) {
+        gload(0);
+        lstore(0);
+    }
+    __syncthreads();
+    for (int t = 0; t < tiles; t++) {
+        const int buf = t & 1, k0 = t * KT;
+        if (t + 1 < tiles) gload(t + 1);
+        const T* Kt = Ks + buf * KT * HDP;
+        const T* Vt = Vs + buf * KT * HDP;
+        const bool masked_block = k0 + KT > limit(0);  // some query of the block does not see all of the tile
+        bool rare = false;
+        if (masked_block) {
+            // a value that is not finite must not meet a zero weight in the product
+            int bad = 0;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const uint4 w = *reinterpret_cast<const uint4*>(Vt + (tid + 256 * i) * 8);
+                constexpr unsigned E = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
+                const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int x = 0; x < 4; x++) bad |= (u[x] & E) == E || (u[x] >> 16 & E) == E;
+            }
+            rare = __syncthreads_or(bad);
+        }
+        if (k0 < wave_end) {
+            v16f s[NK] = {};
+#pragma unroll
+            for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+                for (int x = 0; x < KS; x++) {
+                    const int row = 32 * kt + n;
+                    const v8 k = *reinterpret_cast<const v8*>(Kt + row * HDP + ((2 * x + hf) ^ swz<HDP>(row)) * 8);
+                    s[kt] = mfma32(k, qv[x], s[kt]);
+                }
+            const bool full = k0 + KT <= wave_all;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float x = s[kt][i] * c2;
+                    const int j = k0 + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3);
+                    if (!full && j >= lim) x = -INFINITY;
+                    s[kt][i] = x;
+                    mx = fmaxf(mx, x);
+                }
+            const float mn = fmaxf(m, halves_max(mx));
+            const float mu = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m - mu);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] *= alpha;
+            v8 p[NK][2];
+#pragma unroll
+            for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float x = __builtin_amdgcn_exp2f(s[kt][i] - mu);
+                    l += x;
+                    p[kt][i >> 3][i & 7] = (T)x;
+                }
+            // 8 keys of dim 32 d + n, rows 4 hf + 0..3 and 8 + 4 hf + 0..3 of the 16 at kb
+            auto vfrag = [&](int d, int kb) {
+                typedef __attribute__((address_space(3))) v4s* lptr;
+                const int r = kb + 4 * hf + (lane >> 2 & 3);
+                const int col = 32 * d + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+                const int c = col >> 3, in = col & 7;
+                const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(Vt + r * HDP + (c ^ swz<HDP>(r)) * 8 + in));
+                const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(Vt + (r + 8) * HDP + (c ^ swz<HDP>(r + 8)) * 8 + in));
+                return __builtin_bit_cast(v8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            if (!rare) {
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+                        for (int x = 0; x < 2; x++) o[d] = mfma32(vfrag(d, 32 * kt + 16 * x), p[kt][x], o[d]);
+            } else {
+                // the product once per query of the wave, over the keys that it sees
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    v16f keep = o[d];
+#pragma unroll 1
+                    for (int r = 0; r < 32; r++) {
+                        const int rl = __shfl(lim, r);
+                        v16f acc = o[d];
+#pragma unroll
+                        for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+                            for (int x = 0; x < 2; x++) {
+                                v8 v = vfrag(d, 32 * kt + 16 * x);
+#pragma unroll
+                                for (int e = 0; e < 8; e++) {
+                                    const int j = k0 + 32 * kt + 16 * x + 8 * (e >> 2) + 4 * hf + (e & 3);
+                                    if (j >= rl) v[e] = (T)0.0f;
+                                }
+                                acc = mfma32(v, p[kt][x], acc);
+                            }
+#pragma unroll
+                        for (int i = 0; i < 16; i++) keep[i] = n == r ? acc[i] : keep[i];
+                    }
+                    o[d] = keep;
+                }
+            }
+        }
+        if (t + 1 < tiles) lstore(buf ^ 1);
+        __syncthreads();
+    }
+
+    l = halves_sum(l);
+    const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+    if (!qok) return;
+    T* dst = static_cast<T*>(a.out) + (size_t)(job.q0 + qi) * a.ldo + head * hd;
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int col = 32 * d + 8 * i + 4 * hf;
+            Pack<T, 4> z;
+#pragma unroll
+            for (int r = 0; r < 4; r++) z.v[r] = (T)(m == -INFINITY ? 0.0f : o[d][4 * i + r] * inv);
+            if (col < hd) *reinterpret_cast<Pack<T, 4>*>(dst + col) = z;
+        }
+}
+
+// ------------------------------------------------------------- fp32 ----
+// A wave owns 16 queries: v_mfma_f32_16x16x4_f32 leaves in lane n + 16 g, for query
+// n, the scores of keys 4 g + r of 16, and takes weight r of the lane as key 4 g
+// + r of its step r. The head dimension is walked as d = g * (HDP / 4) + s, so
+// that a lane's K row comes in 16-byte reads.
+
+__device__ __forceinline__ v4f mfma_f32(float a, float b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+template <int HDP>
+__global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
+    constexpr int KT = 32, QT = 64, SK = HDP + 4, QS = HDP / 4, DT = HDP / 16;
+    constexpr int LOADS = KT * HDP / 4 / 256;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float* Ks = reinterpret_cast<float*>(smem);  // [KT][SK]
+    float* Vs = Ks + KT * SK;
+
+    int tile, head;
+    tile_and_head(a, tile, head);
+    Job job;
+    if (!find_job<QT>(a, tile, job)) return;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int n = lane & 15, g = lane >> 4;
+    const int hd = a.head_dim;
+    const int kvh = head / (a.n_q / a.n_kv);
+    const float* Kg = static_cast<const float*>(a.K) + (size_t)job.k0 * a.ldk + kvh * hd;
+    const float* Vg = static_cast<const float*>(a.V) + (size_t)job.k0 * a.ldv + kvh * hd;
+
+    const int qi = wave * 16 + n;
+    const bool qok = qi < job.nq;
+    float qv[QS];
+#pragma unroll
+    for (int s = 0; s < QS; s += 4) {
+        const int d = g * QS + s;
+        float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (qok && d < hd) z = *reinterpret_cast<const float4*>(static_cast<const float*>(a.Q) + (size_t)(job.q0 + qi) * a.ldq + head * hd + d);
+        qv[s] = z.x;
+        qv[s + 1] = z.y;
+        qv[s + 2] = z.z;
+        qv[s + 3] = z.w;
+    }
+    const int off = job.nk - job.len_q + job.at + 1;
+    auto limit = [&](int q) {
+        const int e = a.causal ? q + off : job.nk;
+        return e < 0 ? 0 : (e < job.nk ? e : job.nk);
+    };
+    const int lim = qok ? limit(qi) : 0;
+    const int wq_last = wave * 16 + 15 < job.nq ? wave * 16 + 15 : job.nq - 1;
+    const int wave_end = wave * 16 < job.nq ? limit(wq_last) : 0;
+    const int wave_all = wave * 16 < job.nq ? limit(wave * 16) : 0;
+    const int end = limit(job.nq - 1);
+    const int tiles = (end + KT - 1) / KT;
+
+    float4 kr[LOADS], vr[LOADS];
+    auto gload = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int e = tid + 256 * i, row = e / (HDP / 4), d = 4 * (e % (HDP / 4));
+            int j = t * KT + row;
+            if (j >= end) j = end - 1;
+            kr[i] = vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (d < hd) {
+                kr[i] = *reinterpret_cast<const float4*>(Kg + (size_t)j * a.ldk + d);
+                vr[i] = *reinterpret_cast<const float4*>(Vg + (size_t)j * a.ldv + d);
+            }
+        }
+    };
+    auto lstore = [&]() {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int e = tid + 256 * i, row = e / (HDP / 4), d = 4 * (e % (HDP / 4));
+            *reinterpret_cast<float4*>(Ks + row * SK + d) = kr[i];
+            *reinterpret_cast<float4*>(Vs + row * SK + d) = vr[i];
+        }
+    };
+
+    v4f o[DT] = {};
+    float m = -INFINITY, l = 0.0f;
+    const float c2 = a.scale * kLog2e;
+    if (tiles) gload(0);
+    for (int t = 0; t < tiles; t++) {
+        const int k0 = t * KT;
+        __syncthreads();
+        lstore();
+        __syncthreads();
+        if (t + 1 < tiles) gload(t + 1);
+        bool rare = false;
+        if (k0 + KT > limit(0)) {
+            int bad = 0;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const int e = tid + 256 * i, row = e / (HDP / 4), d = 4 * (e % (HDP / 4));
+                const uint4 w = *reinterpret_cast<const uint4*>(Vs + row * SK + d);
+                const unsigned E = 0x7f800000u;
+                bad |= (w.x & E) == E || (w.y & E) == E || (w.z & E) == E || (w.w & E) == E;
+            }
+            rare = __syncthreads_or(bad);
+        }
+        if (k0 < wave_end) {
+            v4f s[KT / 16] = {};
+#pragma unroll
+            for (int kt = 0; kt < KT / 16; kt++)
+#pragma unroll
+                for (int x = 0; x < QS; x += 4) {
+                    const float4 k = *reinterpret_cast<const float4*>(Ks + (16 * kt + n) * SK + g * QS + x);
+                    s[kt] = mfma_f32(k.x, qv[x], s[kt]);
+                    s[kt] = mfma_f32(k.y, qv[x + 1], s[kt]);
+                    s[kt] = mfma_f32(k.z, qv[x + 2], s[kt]);
+                    s[kt] = mfma_f32(k.w, qv[x + 3], s[kt]);
+                }
+            const bool full = k0 + KT <= wave_all;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < KT / 16; kt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float x = s[kt][r] * c2;
+                    if (!full && k0 + 16 * kt + 4 * g + r >= lim) x = -INFINITY;
+                    s[kt][r] = x;
+                    mx = fmaxf(mx, x);
+                }
+            const float mn = fmaxf(m, rows_max(mx));
+            const float mu = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = __builtin_amdgcn_exp2f(m - mu);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) o[d][r] *= alpha;
+#pragma unroll
+            for (int kt = 0; kt < KT / 16; kt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    s[kt][r] = __builtin_amdgcn_exp2f(s[kt][r] - mu);
+                    l += s[kt][r];
+                }
+            if (!rare) {
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int kt = 0; kt < KT / 16; kt++)
+#pragma unroll
+                        for (int r = 0; r < 4; r++)
+                            o[d] = mfma_f32(Vs[(16 * kt + 4 * g + r) * SK + 16 * d + n], s[kt][r], o[d]);
+            } else {
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    v4f keep = o[d];
+#pragma unroll 1
+                    for (int q = 0; q < 16; q++) {
+                        const int rl = __shfl(lim, q);
+                        v4f acc = o[d];
+#pragma unroll
+                        for (int kt = 0; kt < KT / 16; kt++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                const int j = 16 * kt + 4 * g + r;
+                                const float v = k0 + j < rl ? Vs[j * SK + 16 * d + n] : 0.0f;
+                                acc = mfma_f32(v, s[kt][r], acc);
+                            }
+#pragma unroll
+                        for (int r = 0; r < 4; r++) keep[r] = n == q ? acc[r] : keep[r];
+                    }
+                    o[d] = keep;
+                }
+            }
+        }
+    }
+
+    l = rows_sum(l);
+    const float inv = 1.0f / l;
+    if (!qok) return;
+    float* dst = static_cast<float*>(a.out) + (size_t)(job.q0 + qi) * a.ldo + head * hd;
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+        const int col = 16 * d + 4 * g;
+        float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (m != -INFINITY) z = make_float4(o[d][0] * inv, o[d][1] * inv, o[d][2] * inv, o[d][3] * inv);
+        if (col < hd) *reinterpret_cast<float4*>(dst + col) = z;
+    }
+}
+
+template <class F>
+void launch_lds(F* kernel, const PackedAttnArgs& a, int qt, int lds, hipStream_t st) {
+    if (lds > 65536)
+        VLA_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    // the most tiles that n_seqs sequences of total_q rows can have
+    const int64_t tiles = a.total_q / qt + (a.n_seqs < a.total_q ? a.n_seqs : a.total_q);
+    const int64_t blocks = tiles * a.n_q;
+    VLA_REQUIRE(blocks < (int64_t)1 << 31, "packed_attention: too many rows times heads for one call");
+    kernel<<<(unsigned)blocks, 256, lds, st>>>(a);
+    VLA_LAUNCH_CHECK();
+}
+
+template <class T, int HDP, int KT>
+void run_16(const PackedAttnArgs& a, hipStream_t st) {
+    launch_lds(&packed_attn_16<T, HDP, KT>, a, 128, 4 * KT * HDP * 2, st);
+}
+template <class T>
+void run_16(const PackedAttnArgs& a, hipStream_t st) {
+    if (a.head_dim <= 64) run_16<T, 64, 64>(a, st);
+    else if (a.head_dim <= 128) run_16<T, 128, 64>(a, st);
+    else run_16<T, 256, 32>(a, st);
+}
+template <int HDP>
+void run_f32(const PackedAttnArgs& a, hipStream_t st) {
+    launch_lds(&packed_attn_f32<HDP>, a, 64, 2 * 32 * (HDP + 4) * 4, st);
+}
+
+}  // namespace
+
+void launch_packed_attention(const PackedAttnArgs& a, hipStream_t st) {
+    VLA_REQUIRE(dtype_ok(a.dtype), "packed_attention: dtype must be VLA_F32, VLA_BF16 or VLA_F16");
+    VLA_REQUIRE(a.n_seqs >= 0 && a.total_q >= 0 && a.total_k >= 0 && a.n_q > 0 && a.n_kv > 0,
+                "packed_attention: need n_seqs, total_q, total_k >= 0, n_q > 0, n_kv > 0");
+    VLA_REQUIRE(a.n_q % a.n_kv == 0, "packed_attention: n_q must be a multiple of n_kv");
+    VLA_REQUIRE(a.head_dim > 0 && a.head_dim <= 256 && a.head_dim % 8 == 0,
+                "packed_attention: head_dim must be a multiple of 8 in [8, 256]");
+    VLA_REQUIRE(std::isfinite(a.scale), "packed_attention: scale must be finite");
+    if (a.n_seqs == 0 || a.total_q == 0) return;
+    VLA_REQUIRE(a.out && a.Q && a.q_start && a.k_start, "packed_attention: null buffer");
+    VLA_REQUIRE(a.total_k == 0 || (a.K && a.V), "packed_attention: null keys or values");
+    const int sz = dtype_size(a.dtype);
+    VLA_REQUIRE(aligned(a.Q, 16) && aligned(a.K, 16) && aligned(a.V, 16) && aligned(a.out, 16) && a.ldq * sz % 16 == 0 &&
+                    a.ldk * sz % 16 == 0 && a.ldv * sz % 16 == 0 && a.ldo * sz % 16 == 0,
+                "packed_attention: rows must be 16-byte aligned");
+    VLA_REQUIRE(a.ldq >= a.n_q * a.head_dim && a.ldo >= a.n_q * a.head_dim && a.ldk >= a.n_kv * a.head_dim &&
+                    a.ldv >= a.n_kv * a.head_dim,
+                "packed_attention: row stride shorter than heads * head_dim");
+    if (a.dtype == kBf16) run_16<bf16_t>(a, st);
+    else if (a.dtype == kF16) run_16<f16_t>(a, st);
+    else if (a.head_dim <= 64) run_f32<64>(a, st);
+    else if (a.head_dim <= 128) run_f32<128>(a, st);
+    else run_f32<256>(a, st);
+}
+
+}  // namespace hip
+}  // namespace vla

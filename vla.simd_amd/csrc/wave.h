@@ -57,5 +57,28 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
     return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
 }
 
+// max / sum of x over the lanes l, l^16, l^32, l^48 (the four 16-lane rows of
+// a wave) with gfx950's row-swap permutes, VALU ops instead of LDS round trips.
+// permlane16_swap(x, x) returns, in every lane, the values of the lane pair
+// {l, l^16} (one from the even row, one from the odd row); permlane32_swap the
+// pair {l, l^32}. The sum adds each pair in either order, which is the same
+// float: the results equal those of x op shfl_xor(x, 16), then 32.
+__device__ __forceinline__ float rows_max(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const unsigned v = __float_as_uint(y);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float rows_sum(float x) {
+    const unsigned u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const unsigned v = __float_as_uint(y);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 }  // namespace hip
 }  // namespace vla
