@@ -101,13 +101,15 @@ __device__ bool find_job(const PackedAttnArgs& a, int tile, Job& job) {
                 const int t = want - run - (__shfl(incl, l) - __shfl(tiles, l));
                 const int sq = base + l;
                 const int start = __shfl(q0, l), len = __shfl(n, l);
-                job.at = t * QT;
-                job.q0 = start + job.at;
-                job.len_q = len;
-                job.nq = len - job.at < QT ? len - job.at : QT;
-                job.k0 = clamp_row(a.k_start[sq], a.total_k);
-                job.nk = clamp_row(a.k_start[sq + 1], a.total_k) - job.k0;
-                if (job.nk < 0) job.nk = 0;
+                int nk = clamp_row(a.k_start[sq + 1], a.total_k) - clamp_row(a.k_start[sq], a.total_k);
+                if (nk < 0) nk = 0;
+                // the same in every lane: kept in scalar registers
+                job.at = __builtin_amdgcn_readfirstlane(t * QT);
+                job.q0 = __builtin_amdgcn_readfirstlane(start) + job.at;
+                job.len_q = __builtin_amdgcn_readfirstlane(len);
+                job.nq = job.len_q - job.at < QT ? job.len_q - job.at : QT;
+                job.k0 = __builtin_amdgcn_readfirstlane(clamp_row(a.k_start[sq], a.total_k));
+                job.nk = __builtin_amdgcn_readfirstlane(nk);
                 return true;
             }
             run += sum;
@@ -128,6 +130,9 @@ __device__ __forceinline__ void tile_and_head(const PackedAttnArgs& a, int& tile
 
 // ---------------------------------------------------- 16-bit types ----
 
+// waits for this wave's loads, those into LDS among them (vmcnt 0 alone)
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // LDS rows of HDP values in 16-byte chunks; chunk c of row r lies at c ^ swz(r).
 // 16 rows' reads of one chunk (K) then fall on all 64 banks, and so do the 64-byte
 // pieces of 4 neighbouring rows that a transposed read takes (V).
@@ -136,40 +141,56 @@ __device__ __forceinline__ int swz(int row) {
     return (HDP == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2) | (row >> 2 & 3);
 }
 
-template <class T, int HDP, int KT>
+// Rows in global memory from `first` on, `bytes` of them, read 16 bytes a lane straight into
+// LDS at lds + 16 * lane. Reads from `bytes` on (checked by the hardware) give zeros.
+struct Rows {
+    __amdgpu_buffer_rsrc_t rs;
+    __device__ __forceinline__ Rows(const void* first, int64_t bytes)
+        : rs(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(first), 0, bytes < 0x7fffffff ? (int)bytes : 0x7fffffff, 0x27000)) {}
+    __device__ __forceinline__ void to_lds(void* lds, unsigned offset) const {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16, offset, 0, 0, 0);
+    }
+};
+
+// FULL: head_dim is HDP; else a tile's columns behind head_dim are zeros.
+template <class T, int HDP, int KT, bool FULL>
 __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(PackedAttnArgs a) {
     typedef typename Vec8<T>::type v8;
     constexpr int QT = 128, NK = KT / 32;
     constexpr int CH = HDP / 8;             // chunks of a row
     constexpr int LOADS = KT * CH / 256;    // chunks per thread of a K or V tile
     constexpr int DT = HDP / 32, KS = HDP / 16;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    T* Ks = reinterpret_cast<T*>(smem);     // [2][KT][HDP]
-    T* Vs = Ks + 2 * KT * HDP;
+    constexpr unsigned kExp = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;  // exponent bits: all set where not finite
+    __shared__ __attribute__((aligned(16))) T K0[KT * HDP], K1[KT * HDP], V0[KT * HDP], V1[KT * HDP];
 
     int tile, head;
     tile_and_head(a, tile, head);
     Job job;
     if (!find_job<QT>(a, tile, job)) return;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, hf = lane >> 5;
-    const int hd = a.head_dim;
-    const int kvh = head / (a.n_q / a.n_kv);
+    const int hd = FULL ? HDP : a.head_dim;
+    const int kvh = __builtin_amdgcn_readfirstlane(head / (a.n_q / a.n_kv));
     const T* Kg = static_cast<const T*>(a.K) + (size_t)job.k0 * a.ldk + kvh * hd;
     const T* Vg = static_cast<const T*>(a.V) + (size_t)job.k0 * a.ldv + kvh * hd;
 
     const int qi = wave * 32 + n;  // in the tile
     const bool qok = qi < job.nq;
+    // the sign goes to the queries, so that larger products are larger scores; 0 becomes the
+    // smallest factor, which leaves scores at 0 and masked ones at -inf
+    const float c2 = a.scale == 0.0f ? 1.17549435e-38f : fabsf(a.scale) * kLog2e;
     v8 qv[KS];
 #pragma unroll
     for (int s = 0; s < KS; s++) {
         const int d = 16 * s + 8 * hf;
         v8 z = {};
         if (qok && d < hd) z = *reinterpret_cast<const v8*>(static_cast<const T*>(a.Q) + (size_t)(job.q0 + qi) * a.ldq + head * hd + d);
+        if (a.scale < 0.0f) z = -z;
         qv[s] = z;
     }
-    // keys [0, lim) are seen by the lane's query; wave_min/max over the wave's queries
+    // keys [0, lim) are seen by the lane's query, [0, wave_all) by all of the wave's,
+    // [wave_end, ..) by none of them
     const int off = job.nk - job.len_q + job.at + 1;
     auto limit = [&](int q) {
         const int e = a.causal ? q + off : job.nk;
@@ -178,153 +199,167 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(Packed
     const int lim = qok ? limit(qi) : 0;
     const int wq_last = wave * 32 + 31 < job.nq ? wave * 32 + 31 : job.nq - 1;
     const int wave_end = wave * 32 < job.nq ? limit(wq_last) : 0;
-    const int wave_all = wave * 32 < job.nq ? limit(wave * 32) : 0;  // every query of the wave sees keys below
+    const int wave_all = wave * 32 < job.nq ? limit(wave * 32) : 0;
     const int end = limit(job.nq - 1);
-    const int tiles = (end + KT - 1) / KT;
+    const int tiles = (end + KT - 1) / KT, plain = limit(0) / KT;  // tiles [0, plain) are seen whole by every query
 
-    uint4 kr[LOADS], vr[LOADS];
-    auto gload = [&](int t) {
+    typedef __attribute__((address_space(3))) v4s* trptr;
+    // 16-byte piece e of a tile is chunk e % CH of row e / CH, which holds the row's chunk
+    // (e % CH) ^ swz; its offset from the tile's first row is the same in every tile
+    unsigned ko[LOADS], vo[LOADS];
 #pragma unroll
-        for (int i = 0; i < LOADS; i++) {
-            const int e = tid + 256 * i, row = e / CH, d = (e % CH) * 8;
-            int j = t * KT + row;
-            if (j >= end) j = end - 1;  // masked below; keeps the address among the sequence's rows
-            kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-            if (d < hd) {
-                kr[i] = *reinterpret_cast<const uint4*>(Kg + (size_t)j * a.ldk + d);
-                vr[i] = *reinterpret_cast<const uint4*>(Vg + (size_t)j * a.ldv + d);
-            }
-        }
-    };
-    auto lstore = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < LOADS; i++) {
-            const int e = tid + 256 * i, row = e / CH, c = (e % CH) ^ swz<HDP>(row);
-            *reinterpret_cast<uint4*>(Ks + (buf * KT + row) * HDP + c * 8) = kr[i];
-            *reinterpret_cast<uint4*>(Vs + (buf * KT + row) * HDP + c * 8) = vr[i];
-        }
-    };
-
-    v16f o[DT] = {};
-    float m = -INFINITY, l = 0.0f;
-    const float c2 = a.scale * kLog2e;
-
-    if (tiles) {
-        gload(0);
-        lstore(0);
+    for (int i = 0; i < LOADS; i++) {
+        const int e = tid + 256 * i, row = e / CH, d = ((e % CH) ^ swz<HDP>(row)) * 8;
+        const bool in = FULL || d < hd;  // behind head_dim: behind every row, zeros
+        ko[i] = in ? (unsigned)(row * (int)a.ldk + d) * sizeof(T) : 0x80000000u;
+        vo[i] = in ? (unsigned)(row * (int)a.ldv + d) * sizeof(T) : 0x80000000u;
     }
-    __syncthreads();
-    for (int t = 0; t < tiles; t++) {
-        const int buf = t & 1, k0 = t * KT;
-        if (t + 1 < tiles) gload(t + 1);
-        const T* Kt = Ks + buf * KT * HDP;
-        const T* Vt = Vs + buf * KT * HDP;
-        const bool masked_block = k0 + KT > limit(0);  // some query of the block does not see all of the tile
-        bool rare = false;
-        if (masked_block) {
-            // a value that is not finite must not meet a zero weight in the product
+    auto issue = [&](int t, T* kd, T* vd) {
+        // the rows from the tile's first to the last key: reads behind them give zeros
+        const int64_t rows = end - t * KT;
+        const int64_t kb = rows * a.ldk * (int)sizeof(T), vb = rows * a.ldv * (int)sizeof(T);
+        const Rows kt(Kg + (size_t)t * KT * a.ldk, kb), vt(Vg + (size_t)t * KT * a.ldv, vb);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            kt.to_lds(kd + (256 * i + wave * 64) * 8, ko[i]);
+            vt.to_lds(vd + (256 * i + wave * 64) * 8, vo[i]);
+        }
+    };
+    v16f o[DT] = {};
+    float m = -INFINITY, l = 0.0f;  // the reference of the weights, in log2, and their sum
+    int cleaned = 0x7fffffff;       // first key of the first tile with values taken out
+
+    // one tile of keys; MASKED: some query of the block does not see all of it
+    auto step = [&]<bool MASKED>(int k0, const T* Kt, T* Vt) {
+        if constexpr (MASKED) {
+            // A value that is not finite must not meet a zero weight in the product.
+            // Such values are taken out here and added at the end to the queries that see them.
             int bad = 0;
 #pragma unroll
             for (int i = 0; i < LOADS; i++) {
                 const uint4 w = *reinterpret_cast<const uint4*>(Vt + (tid + 256 * i) * 8);
-                constexpr unsigned E = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;
                 const unsigned u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int x = 0; x < 4; x++) bad |= (u[x] & E) == E || (u[x] >> 16 & E) == E;
+                for (int x = 0; x < 4; x++) bad |= (u[x] & kExp) == kExp || (u[x] >> 16 & kExp) == kExp;
             }
-            rare = __syncthreads_or(bad);
+            if (__syncthreads_or(bad)) {
+                cleaned = cleaned < k0 ? cleaned : k0;
+                unsigned short* w = reinterpret_cast<unsigned short*>(Vt);
+                for (int e = tid; e < KT * HDP; e += 256)
+                    if ((w[e] & kExp) == kExp) w[e] = 0;
+                __syncthreads();
+            }
+            if (k0 >= wave_end) return;
         }
-        if (k0 < wave_end) {
-            v16f s[NK] = {};
+        v16f s[NK] = {};
+#pragma unroll
+        for (int x = 0; x < KS; x++)
+#pragma unroll
+            for (int kt = 0; kt < NK; kt++) {
+                const int row = 32 * kt + n;
+                const v8 k = *reinterpret_cast<const v8*>(Kt + row * HDP + ((2 * x + hf) ^ swz<HDP>(row)) * 8);
+                s[kt] = mfma32(k, qv[x], s[kt]);
+            }
+        // two rows' reads stay ahead of the products that take them
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * NK, 0);
+#pragma unroll
+        for (int x = 0; x < KS - 2; x++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, NK, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, NK, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 2 * NK, 0);
+        if (MASKED && k0 + KT > wave_all) {
 #pragma unroll
             for (int kt = 0; kt < NK; kt++)
 #pragma unroll
-                for (int x = 0; x < KS; x++) {
-                    const int row = 32 * kt + n;
-                    const v8 k = *reinterpret_cast<const v8*>(Kt + row * HDP + ((2 * x + hf) ^ swz<HDP>(row)) * 8);
-                    s[kt] = mfma32(k, qv[x], s[kt]);
-                }
-            const bool full = k0 + KT <= wave_all;
-            float mx = -INFINITY;
+                for (int i = 0; i < 16; i++)
+                    if (k0 + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3) >= lim) s[kt][i] = -INFINITY;
+        }
+        float mx = s[0][0];
 #pragma unroll
-            for (int kt = 0; kt < NK; kt++)
+        for (int kt = 0; kt < NK; kt++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float x = s[kt][i] * c2;
-                    const int j = k0 + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3);
-                    if (!full && j >= lim) x = -INFINITY;
-                    s[kt][i] = x;
-                    mx = fmaxf(mx, x);
-                }
-            const float mn = fmaxf(m, halves_max(mx));
-            const float mu = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = __builtin_amdgcn_exp2f(m - mu);
+            for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[kt][i]);
+        mx = halves_max(mx) * c2;
+        // The reference only has to keep the weights in range: it follows the
+        // maximum when a query's has grown by 2^6, so most tiles rescale nothing.
+        if (__any(mx > m + 6.0f)) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
             m = mn;
             l *= alpha;
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] *= alpha;
-            v8 p[NK][2];
-#pragma unroll
-            for (int kt = 0; kt < NK; kt++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float x = __builtin_amdgcn_exp2f(s[kt][i] - mu);
-                    l += x;
-                    p[kt][i >> 3][i & 7] = (T)x;
-                }
-            // 8 keys of dim 32 d + n, rows 4 hf + 0..3 and 8 + 4 hf + 0..3 of the 16 at kb
-            auto vfrag = [&](int d, int kb) {
-                typedef __attribute__((address_space(3))) v4s* lptr;
-                const int r = kb + 4 * hf + (lane >> 2 & 3);
-                const int col = 32 * d + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
-                const int c = col >> 3, in = col & 7;
-                const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(Vt + r * HDP + (c ^ swz<HDP>(r)) * 8 + in));
-                const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr)(Vt + (r + 8) * HDP + (c ^ swz<HDP>(r + 8)) * 8 + in));
-                return __builtin_bit_cast(v8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-            };
-            if (!rare) {
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int kt = 0; kt < NK; kt++)
-#pragma unroll
-                        for (int x = 0; x < 2; x++) o[d] = mfma32(vfrag(d, 32 * kt + 16 * x), p[kt][x], o[d]);
-            } else {
-                // the product once per query of the wave, over the keys that it sees
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    v16f keep = o[d];
-#pragma unroll 1
-                    for (int r = 0; r < 32; r++) {
-                        const int rl = __shfl(lim, r);
-                        v16f acc = o[d];
-#pragma unroll
-                        for (int kt = 0; kt < NK; kt++)
-#pragma unroll
-                            for (int x = 0; x < 2; x++) {
-                                v8 v = vfrag(d, 32 * kt + 16 * x);
-#pragma unroll
-                                for (int e = 0; e < 8; e++) {
-                                    const int j = k0 + 32 * kt + 16 * x + 8 * (e >> 2) + 4 * hf + (e & 3);
-                                    if (j >= rl) v[e] = (T)0.0f;
-                                }
-                                acc = mfma32(v, p[kt][x], acc);
-                            }
-#pragma unroll
-                        for (int i = 0; i < 16; i++) keep[i] = n == r ? acc[i] : keep[i];
-                    }
-                    o[d] = keep;
-                }
-            }
         }
-        if (t + 1 < tiles) lstore(buf ^ 1);
+        const float mu = m == -INFINITY ? 0.0f : m;
+        v8 p[NK][2];
+#pragma unroll
+        for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], c2, -mu));
+                l += x;
+                p[kt][i >> 3][i & 7] = (T)x;
+            }
+        // 8 keys of dim 32 d + n: rows 4 hf + 0..3 and 8 + 4 hf + 0..3 of the 16 at kb
+        auto vfrag = [&](int d, int kb) {
+            const int r = kb + 4 * hf + (lane >> 2 & 3);
+            const int col = 32 * d + (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+            const int c = col >> 3, in = col & 7;
+            const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((trptr)(Vt + r * HDP + (c ^ swz<HDP>(r)) * 8 + in));
+            const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((trptr)(Vt + (r + 8) * HDP + (c ^ swz<HDP>(r + 8)) * 8 + in));
+            return __builtin_bit_cast(v8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+#pragma unroll
+        for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] = mfma32(vfrag(d, 32 * kt + 16 * x), p[kt][x], o[d]);
+        __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+#pragma unroll
+        for (int x = 0; x < 2 * NK * DT - 4; x++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 4, 1);
+    };
+    // tiles alternate between the two buffers; the next one is loaded while this one is worked on
+    auto turn = [&]<bool MASKED>(int t, T* kc, T* vc, T* kn, T* vn) {
+        if (t + 1 < tiles) issue(t + 1, kn, vn);
+        step.template operator()<MASKED>(t * KT, kc, vc);
+        wait_loads();
         __syncthreads();
+    };
+
+    if (tiles) issue(0, K0, V0);
+    wait_loads();
+    __syncthreads();
+    int t = 0;
+    for (; t + 2 <= plain; t += 2) {
+        turn.template operator()<false>(t, K0, V0, K1, V1);
+        turn.template operator()<false>(t + 1, K1, V1, K0, V0);
+    }
+    for (; t < tiles; t += 2) {
+        turn.template operator()<true>(t, K0, V0, K1, V1);
+        if (t + 1 < tiles) turn.template operator()<true>(t + 1, K1, V1, K0, V0);
+    }
+
+    for (int j = cleaned; j < end; j++) {
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int col = 32 * d + 8 * (i >> 2) + 4 * hf + (i & 3);
+                const float x = col < hd ? to_f32(Vg[(size_t)j * a.ldv + col]) : 0.0f;
+                if (!(fabsf(x) < INFINITY) && j < lim) o[d][i] += x;
+            }
     }
 
     l = halves_sum(l);
-    const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+    const float inv = 1.0f / l;
     if (!qok) return;
     T* dst = static_cast<T*>(a.out) + (size_t)(job.q0 + qi) * a.ldo + head * hd;
 #pragma unroll
@@ -334,7 +369,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(Packed
             const int col = 32 * d + 8 * i + 4 * hf;
             Pack<T, 4> z;
 #pragma unroll
-            for (int r = 0; r < 4; r++) z.v[r] = (T)(m == -INFINITY ? 0.0f : o[d][4 * i + r] * inv);
+            for (int r = 0; r < 4; r++) z.v[r] = (T)(l == 0.0f ? 0.0f : o[d][4 * i + r] * inv);
             if (col < hd) *reinterpret_cast<Pack<T, 4>*>(dst + col) = z;
         }
 }
@@ -517,7 +552,7 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
     for (int d = 0; d < DT; d++) {
         const int col = 16 * d + 4 * g;
         float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (m != -INFINITY) z = make_float4(o[d][0] * inv, o[d][1] * inv, o[d][2] * inv, o[d][3] * inv);
+        if (l != 0.0f) z = make_float4(o[d][0] * inv, o[d][1] * inv, o[d][2] * inv, o[d][3] * inv);
         if (col < hd) *reinterpret_cast<float4*>(dst + col) = z;
     }
 }
@@ -536,7 +571,8 @@ void launch_lds(F* kernel, const PackedAttnArgs& a, int qt, int lds, hipStream_t
 
 template <class T, int HDP, int KT>
 void run_16(const PackedAttnArgs& a, hipStream_t st) {
-    launch_lds(&packed_attn_16<T, HDP, KT>, a, 128, 4 * KT * HDP * 2, st);
+    if (a.head_dim == HDP) launch_lds(&packed_attn_16<T, HDP, KT, true>, a, 128, 0, st);
+    else launch_lds(&packed_attn_16<T, HDP, KT, false>, a, 128, 0, st);
 }
 template <class T>
 void run_16(const PackedAttnArgs& a, hipStream_t st) {
@@ -566,6 +602,7 @@ void launch_packed_attention(const PackedAttnArgs& a, hipStream_t st) {
     VLA_REQUIRE(aligned(a.Q, 16) && aligned(a.K, 16) && aligned(a.V, 16) && aligned(a.out, 16) && a.ldq * sz % 16 == 0 &&
                     a.ldk * sz % 16 == 0 && a.ldv * sz % 16 == 0 && a.ldo * sz % 16 == 0,
                 "packed_attention: rows must be 16-byte aligned");
+    VLA_REQUIRE(a.ldk < 1 << 22 && a.ldv < 1 << 22, "packed_attention: row stride of K or V past 2^22 values");
     VLA_REQUIRE(a.ldq >= a.n_q * a.head_dim && a.ldo >= a.n_q * a.head_dim && a.ldk >= a.n_kv * a.head_dim &&
                     a.ldv >= a.n_kv * a.head_dim,
                 "packed_attention: row stride shorter than heads * head_dim");
