@@ -731,58 +731,61 @@ def attention_dev(out, Q, K, V, n_q, n_kv, head_dim, scale, mask: VlaMask | None
 
 
 # ------------------- decoders with several sequences (torch tensors) --
+# Their checks read each attribute of a tensor once: a call on one token takes some 10 us on the
+# host, most of it these reads.
 
-_DTYPES = None
+_torch = _TYPE_IDS = _INT32 = None
 
 
-def _dtype_of(t):
+def _import_torch():
+    global _torch, _TYPE_IDS, _INT32
+    import torch
+    _TYPE_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # vla_dtype
+    _INT32 = torch.int32
+    _torch = torch
+
+
+def _type_id(t):
     """The vla_dtype of a tensor's rows."""
-    global _DTYPES
-    if _DTYPES is None:
-        import torch
-        _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    d = _DTYPES.get(t.dtype)
+    if _torch is None:
+        _import_torch()
+    d = _TYPE_IDS.get(t.dtype)
     if d is None:
         raise ValueError(f"rows must be float32, bfloat16 or float16, not {t.dtype}")
     return d
 
 
-def _rows_of(name, t, rows, width, dtype):
-    """The row stride of a [rows, width] tensor whose rows are contiguous."""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width or t.dtype != dtype:
+def _row_ld(name, t, rows, width, dtype):
+    """The row stride of a [rows, width] tensor whose rows are contiguous and do not overlap."""
+    if t.dtype is not dtype or t.shape != (rows, width):
         raise ValueError(f"{name}: need [{rows}, {width}] of {dtype}, got {list(t.shape)} of {t.dtype}")
+    ld, step = t.stride()
     if rows <= 1:
-        return width if width == 1 or t.stride(1) == 1 else _strided(name)
-    ld = t.stride(0)
-    if (t.stride(1) != 1 and width > 1) or ld < width:
-        _strided(name)
+        ld = width
+    if ld < width or (step != 1 and width > 1):
+        raise ValueError(f"{name}: rows must be contiguous and must not overlap")
     return ld
 
 
-def _strided(name):
-    raise ValueError(f"{name}: rows must be contiguous and must not overlap")
-
-
-def _ints(name, t, n):
-    import torch
-    if t.dim() != 1 or t.dtype != torch.int32 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+def _check_ints(name, t, n):
+    if t.dtype is not _INT32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name}: need {n} contiguous int32, got {list(t.shape)} of {t.dtype}")
 
 
-def _starts_of(name, t):
+def _seqs_of(name, t):
     """The number of sequences of an offsets tensor [n_seqs + 1]."""
     n = t.shape[0] if t.dim() == 1 else 0
     if n < 1:
         raise ValueError(f"{name}: need [n_seqs + 1] offsets, got {list(t.shape)}")
-    _ints(name, t, n)
+    _check_ints(name, t, n)
     return n - 1
 
 
-def _same_device(*ts):
+def _check_devices(*ts):
     """All tensors on torch's current device, whose stream the kernels run on."""
-    import torch
+    dev = _torch.cuda.current_device() if ts[0].is_cuda else None
     for t in ts:
-        if t is not None and not (t.is_cuda and t.get_device() == torch.cuda.current_device()):
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"a tensor is on {t.device}, not on the current GPU")
 
 
@@ -792,45 +795,44 @@ def qk_norm_rope_dev(q_out, k_out, q, k, n_q, n_kv, head_dim, pos, sections, bas
     float32 weight [head_dim] is given) and their rotation by positions pos [n_axes, T] int32;
     sections[a] of the head_dim / 2 pairs turn with axis a. The outputs may be the inputs.
     q and q_out, or k and k_out, may be None where n_q, or n_kv, is 0."""
-    import torch
     x = q if n_q else k
-    T, dt = x.shape[0], _dtype_of(x)
-    lds = []
-    for name, t, h in (("q_out", q_out, n_q), ("k_out", k_out, n_kv), ("q", q, n_q), ("k", k, n_kv)):
-        lds.append(_rows_of(name, t, T, h * head_dim, x.dtype) if h else 0)
-    sections = [int(s) for s in sections]
-    if pos.dim() != 2 or pos.dtype != torch.int32 or pos.shape[0] != len(sections) or pos.shape[1] != T or \
-            (T > 1 and pos.stride(1) != 1):
-        raise ValueError(f"pos: need [{len(sections)}, {T}] int32 with contiguous rows, got {list(pos.shape)} of {pos.dtype}")
+    dt, dtype, T, axes = _type_id(x), x.dtype, x.shape[0], len(sections)
+    qp = kp = qop = kop = None
+    ldq = ldk = ldqo = ldko = 0
+    if n_q:
+        ldqo, ldq = _row_ld("q_out", q_out, T, n_q * head_dim, dtype), _row_ld("q", q, T, n_q * head_dim, dtype)
+        qp, qop = q.data_ptr(), q_out.data_ptr()
+    if n_kv:
+        ldko, ldk = _row_ld("k_out", k_out, T, n_kv * head_dim, dtype), _row_ld("k", k, T, n_kv * head_dim, dtype)
+        kp, kop = k.data_ptr(), k_out.data_ptr()
+    if pos.dtype is not _INT32 or pos.shape != (axes, T) or (T > 1 and pos.stride(1) != 1):
+        raise ValueError(f"pos: need [{axes}, {T}] int32 with contiguous rows, got {list(pos.shape)} of {pos.dtype}")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.dtype != torch.float32 or w.dim() != 1 or w.shape[0] != head_dim or not w.is_contiguous()):
+        if w is not None and (w.dtype is not _torch.float32 or w.shape != (head_dim,) or not w.is_contiguous()):
             raise ValueError(f"{name}: need {head_dim} contiguous float32")
-    _same_device(pos, q_weight, k_weight, *(t for t, h in ((q_out, n_q), (q, n_q), (k_out, n_kv), (k, n_kv)) if h))
-    _call("vla_qk_norm_rope_dev", _dp(q_out) if n_q else None, lds[0], _dp(k_out) if n_kv else None, lds[1],
-          _dp(q) if n_q else None, lds[2], _dp(k) if n_kv else None, lds[3], _dp(q_weight), _dp(k_weight), float(eps),
-          _dp(pos), pos.stride(0) if len(sections) > 1 else T, (c_int32 * len(sections))(*sections), len(sections),
-          float(base), T, n_q, n_kv, head_dim, dt, _stream(stream))
+    _check_devices(pos, q_weight, k_weight, *((q_out, q) if n_q else ()), *((k_out, k) if n_kv else ()))
+    _call("vla_qk_norm_rope_dev", qop, ldqo, kop, ldko, qp, ldq, kp, ldk, _dp(q_weight), _dp(k_weight), eps, pos.data_ptr(),
+          pos.stride(0) if axes > 1 else T, (c_int32 * axes)(*sections), axes, base, T, n_q, n_kv, head_dim, dt,
+          _stream(stream))
 
 
 def packed_attention_dev(out, Q, K, V, n_q, n_kv, head_dim, scale, q_start, k_start=None, causal=True, stream=None):
     """Attention of packed sequences: rows q_start[s] .. q_start[s + 1] - 1 of Q and out and
     k_start's of K and V (None: the same) are sequence s. Causal: the last query sees the last key."""
-    dt = _dtype_of(Q)
-    n = _starts_of("q_start", q_start)
-    ldq = _rows_of("Q", Q, Q.shape[0], n_q * head_dim, Q.dtype)
-    ldo = _rows_of("out", out, Q.shape[0], n_q * head_dim, Q.dtype)
-    ldk = _rows_of("K", K, K.shape[0], n_kv * head_dim, Q.dtype)
-    ldv = _rows_of("V", V, K.shape[0], n_kv * head_dim, Q.dtype)
+    dt, dtype, n, tq, tk = _type_id(Q), Q.dtype, _seqs_of("q_start", q_start), Q.shape[0], K.shape[0]
+    ldo, ldq = _row_ld("out", out, tq, n_q * head_dim, dtype), _row_ld("Q", Q, tq, n_q * head_dim, dtype)
+    ldk, ldv = _row_ld("K", K, tk, n_kv * head_dim, dtype), _row_ld("V", V, tk, n_kv * head_dim, dtype)
     if k_start is not None:
-        _ints("k_start", k_start, n + 1)
-    _same_device(out, Q, K, V, q_start, k_start)
-    _call("vla_packed_attention_dev", _dp(out), ldo, _dp(Q), ldq, _dp(K), ldk, _dp(V), ldv, _dp(q_start), _dp(k_start), n,
-          Q.shape[0], K.shape[0], n_q, n_kv, head_dim, float(scale), int(bool(causal)), dt, _stream(stream))
+        _check_ints("k_start", k_start, n + 1)
+    _check_devices(out, Q, K, V, q_start, k_start)
+    _call("vla_packed_attention_dev", out.data_ptr(), ldo, Q.data_ptr(), ldq, K.data_ptr(), ldk, V.data_ptr(), ldv,
+          q_start.data_ptr(), _dp(k_start), n, tq, tk, n_q, n_kv, head_dim, scale, 1 if causal else 0, dt,
+          _stream(stream))
 
 
 def kv4_page_bytes(n_kv, head_dim, page_size) -> int:
     """Bytes of a page of the 4-bit cache."""
-    n = int(lib().vla_kv4_page_bytes(n_kv, head_dim, page_size))
+    n = (_lib or lib()).vla_kv4_page_bytes(n_kv, head_dim, page_size)
     if n < 0:
         raise ValueError("kv4: head_dim a multiple of 32 up to 256, page_size a multiple of 32 up to 2048")
     return n
@@ -843,43 +845,43 @@ def kv4_offset(table_row, n_kv, head_dim, page_size, n_pages, token, part, head,
     return int(lib().vla_kv4_offset(n_kv, head_dim, page_size, n_pages, _ptr(row), row.size, token, part, head, block))
 
 
-def _cache_of(cache, n_kv, head_dim, page_size, table):
+def _cache_shape(cache, n_kv, head_dim, page_size, table):
     """(n_pages, n_seqs, ld_table) of a cache [n_pages, page bytes] and a table [n_seqs, pages]."""
-    import torch
     nb = kv4_page_bytes(n_kv, head_dim, page_size)
-    if cache.dtype != torch.uint8 or cache.dim() != 2 or cache.shape[1] != nb or not cache.is_contiguous():
-        raise ValueError(f"cache: need contiguous [n_pages, {nb}] uint8, got {list(cache.shape)} of {cache.dtype}")
-    if table.dim() != 2 or table.dtype != torch.int32 or not table.is_contiguous():
-        raise ValueError(f"table: need contiguous [n_seqs, pages] int32, got {list(table.shape)} of {table.dtype}")
-    return cache.shape[0], table.shape[0], table.shape[1]
+    if _torch is None:
+        _import_torch()
+    cs, ts = cache.shape, table.shape
+    if cache.dtype is not _torch.uint8 or len(cs) != 2 or cs[1] != nb or not cache.is_contiguous():
+        raise ValueError(f"cache: need contiguous [n_pages, {nb}] uint8, got {list(cs)} of {cache.dtype}")
+    if table.dtype is not _INT32 or len(ts) != 2 or not table.is_contiguous():
+        raise ValueError(f"table: need contiguous [n_seqs, pages] int32, got {list(ts)} of {table.dtype}")
+    return cs[0], ts[0], ts[1]
 
 
 def kv4_append_dev(cache, K, V, n_kv, head_dim, page_size, table, lens, start, stream=None):
     """Writes packed rows K, V [total, n_kv * head_dim] as the newest tokens of their sequences;
     lens [n_seqs] counts each sequence's tokens with them."""
-    pages, n, ld = _cache_of(cache, n_kv, head_dim, page_size, table)
-    dt = _dtype_of(K)
-    ldk = _rows_of("K", K, K.shape[0], n_kv * head_dim, K.dtype)
-    ldv = _rows_of("V", V, K.shape[0], n_kv * head_dim, K.dtype)
-    _ints("lens", lens, n)
-    _ints("start", start, n + 1)
-    _same_device(cache, K, V, table, lens, start)
-    _call("vla_kv4_append_dev", _dp(cache), pages, page_size, _dp(K), ldk, _dp(V), ldv, _dp(table), ld, _dp(lens),
-          _dp(start), n, K.shape[0], n_kv, head_dim, dt, _stream(stream))
+    pages, n, ld = _cache_shape(cache, n_kv, head_dim, page_size, table)
+    dt, dtype, total = _type_id(K), K.dtype, K.shape[0]
+    ldk, ldv = _row_ld("K", K, total, n_kv * head_dim, dtype), _row_ld("V", V, total, n_kv * head_dim, dtype)
+    _check_ints("lens", lens, n)
+    _check_ints("start", start, n + 1)
+    _check_devices(cache, K, V, table, lens, start)
+    _call("vla_kv4_append_dev", cache.data_ptr(), pages, page_size, K.data_ptr(), ldk, V.data_ptr(), ldv, table.data_ptr(), ld,
+          lens.data_ptr(), start.data_ptr(), n, total, n_kv, head_dim, dt, _stream(stream))
 
 
 def kv4_gather_dev(K, V, cache, n_kv, head_dim, page_size, table, start, first=None, stream=None):
     """Reads cached tokens into packed rows K, V: row i of sequence s is its token first[s] + i."""
-    pages, n, ld = _cache_of(cache, n_kv, head_dim, page_size, table)
-    dt = _dtype_of(K)
-    ldk = _rows_of("K", K, K.shape[0], n_kv * head_dim, K.dtype)
-    ldv = _rows_of("V", V, K.shape[0], n_kv * head_dim, K.dtype)
-    _ints("start", start, n + 1)
+    pages, n, ld = _cache_shape(cache, n_kv, head_dim, page_size, table)
+    dt, dtype, total = _type_id(K), K.dtype, K.shape[0]
+    ldk, ldv = _row_ld("K", K, total, n_kv * head_dim, dtype), _row_ld("V", V, total, n_kv * head_dim, dtype)
+    _check_ints("start", start, n + 1)
     if first is not None:
-        _ints("first", first, n)
-    _same_device(cache, K, V, table, start, first)
-    _call("vla_kv4_gather_dev", _dp(K), ldk, _dp(V), ldv, _dp(cache), pages, page_size, _dp(table), ld, _dp(start),
-          _dp(first), n, K.shape[0], n_kv, head_dim, dt, _stream(stream))
+        _check_ints("first", first, n)
+    _check_devices(cache, K, V, table, start, first)
+    _call("vla_kv4_gather_dev", K.data_ptr(), ldk, V.data_ptr(), ldv, cache.data_ptr(), pages, page_size, table.data_ptr(), ld,
+          start.data_ptr(), _dp(first), n, total, n_kv, head_dim, dt, _stream(stream))
 
 
 def kv4_attention_work_bytes(total_q, n_seqs, max_new, max_len, n_q, n_kv, head_dim) -> int:
@@ -893,20 +895,21 @@ def kv4_attention_dev(out, Q, cache, n_q, n_kv, head_dim, page_size, scale, tabl
     sequence s (q_start; None: one each) row i sees the keys j < lens[s] - n + i + 1. max_new and
     max_len bound n and lens (max_len None: what the table can hold); work: a uint8
     tensor of kv4_attention_work_bytes, or None to run without splitting the keys."""
-    import torch
-    pages, n, ld = _cache_of(cache, n_kv, head_dim, page_size, table)
-    dt = _dtype_of(Q)
-    ldq = _rows_of("Q", Q, Q.shape[0], n_q * head_dim, Q.dtype)
-    ldo = _rows_of("out", out, Q.shape[0], n_q * head_dim, Q.dtype)
-    _ints("lens", lens, n)
+    pages, n, ld = _cache_shape(cache, n_kv, head_dim, page_size, table)
+    dt, dtype, total = _type_id(Q), Q.dtype, Q.shape[0]
+    ldo, ldq = _row_ld("out", out, total, n_q * head_dim, dtype), _row_ld("Q", Q, total, n_q * head_dim, dtype)
+    _check_ints("lens", lens, n)
     if q_start is not None:
-        _ints("q_start", q_start, n + 1)
-    if work is not None and (work.dtype != torch.uint8 or not work.is_contiguous()):
-        raise ValueError("work: need contiguous uint8")
-    _same_device(out, Q, cache, table, lens, q_start, work)
-    _call("vla_kv4_attention_dev", _dp(out), ldo, _dp(Q), ldq, _dp(cache), pages, page_size, _dp(table), ld, _dp(lens),
-          _dp(q_start), n, Q.shape[0], max_new, ld * page_size if max_len is None else max_len, n_q, n_kv, head_dim,
-          float(scale), dt, _dp(work), 0 if work is None else work.numel(), _stream(stream))
+        _check_ints("q_start", q_start, n + 1)
+    wp, wb = None, 0
+    if work is not None:
+        if work.dtype is not _torch.uint8 or not work.is_contiguous():
+            raise ValueError("work: need contiguous uint8")
+        wp, wb = work.data_ptr(), work.numel()
+    _check_devices(out, Q, cache, table, lens, q_start, work)
+    _call("vla_kv4_attention_dev", out.data_ptr(), ldo, Q.data_ptr(), ldq, cache.data_ptr(), pages, page_size, table.data_ptr(),
+          ld, lens.data_ptr(), _dp(q_start), n, total, max_new, ld * page_size if max_len is None else max_len, n_q, n_kv,
+          head_dim, scale, dt, wp, wb, _stream(stream))
 
 
 class LinearI8:

@@ -71,52 +71,51 @@ __device__ __forceinline__ int clamp_row(int x, int total) { return x < 0 ? 0 : 
 // are read clamped to the buffers' rows, a sequence that would end before it
 // begins as empty, so that no offsets can lead out of the buffers. Every wave does the same
 // search, 64 sequences at a time; tiles are counted from the last one of the
-// last sequence, whose queries see the most keys under a causal mask.
+// last sequence, as queries late in a sequence see the most keys under a causal mask.
 template <int QT>
-__device__ bool find_job(const PackedAttnArgs& a, int tile, Job& job) {
+__device__ __forceinline__ bool find_job(const PackedAttnArgs& a, int tile, Job& job) {
     const int lane = threadIdx.x & 63;
-    int total = 0;
-    for (int pass = 0; pass < 2; pass++) {
-        int run = 0;
-        const int want = total - 1 - tile;
-        if (pass && want < 0) return false;
-        for (int base = 0; base < a.n_seqs; base += 64) {
-            const int s = base + lane;
-            int q0 = 0, n = 0;
-            if (s < a.n_seqs) {
-                q0 = clamp_row(a.q_start[s], a.total_q);
-                n = clamp_row(a.q_start[s + 1], a.total_q) - q0;
-                if (n < 0) n = 0;
-            }
-            const int tiles = (n + QT - 1) / QT;
-            int incl = tiles;
-            for (int d = 1; d < 64; d <<= 1) {
-                const int o = __shfl_up(incl, d);
-                if (lane >= d) incl += o;
-            }
-            const int sum = __shfl(incl, 63);
-            if (pass && want < run + sum) {
-                const unsigned long long hit = __ballot(run + incl > want);
-                const int l = __ffsll(hit) - 1;
-                const int t = want - run - (__shfl(incl, l) - __shfl(tiles, l));
-                const int sq = base + l;
-                const int start = __shfl(q0, l), len = __shfl(n, l);
-                int nk = clamp_row(a.k_start[sq + 1], a.total_k) - clamp_row(a.k_start[sq], a.total_k);
-                if (nk < 0) nk = 0;
-                // the same in every lane: kept in scalar registers
-                job.at = __builtin_amdgcn_readfirstlane(t * QT);
-                job.q0 = __builtin_amdgcn_readfirstlane(start) + job.at;
-                job.len_q = __builtin_amdgcn_readfirstlane(len);
-                job.nq = job.len_q - job.at < QT ? job.len_q - job.at : QT;
-                job.k0 = __builtin_amdgcn_readfirstlane(clamp_row(a.k_start[sq], a.total_k));
-                job.nk = __builtin_amdgcn_readfirstlane(nk);
-                return true;
-            }
-            run += sum;
+    int q0 = 0, n = 0, k0 = 0, nk = 0, tiles = 0, incl = 0;  // of the lane's sequence; tiles up to it
+    auto load = [&](int base) {
+        const int s = base + lane;
+        q0 = n = k0 = nk = 0;
+        if (s < a.n_seqs) {
+            q0 = clamp_row(a.q_start[s], a.total_q);
+            n = clamp_row(a.q_start[s + 1], a.total_q) - q0;
+            k0 = clamp_row(a.k_start[s], a.total_k);
+            nk = clamp_row(a.k_start[s + 1], a.total_k) - k0;
+            n = n < 0 ? 0 : n;
+            nk = nk < 0 ? 0 : nk;
         }
-        total = run;
+        incl = tiles = (n + QT - 1) / QT;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(incl, d);
+            if (lane >= d) incl += o;
+        }
+        return __builtin_amdgcn_readlane(incl, 63);
+    };
+    int total = load(0);
+    if (a.n_seqs > 64)
+        for (int base = 64; base < a.n_seqs; base += 64) total += load(base);
+    int want = total - 1 - tile;
+    if (want < 0) return false;
+    if (a.n_seqs > 64) {
+        for (int base = 0;; base += 64) {
+            const int sum = load(base);
+            if (want < sum) break;
+            want -= sum;
+        }
     }
-    return false;
+    // the same in every lane: kept in scalar registers
+    const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(incl > want)) - 1);
+    job.at = (want - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(tiles, l))) * QT;
+    job.q0 = __builtin_amdgcn_readlane(q0, l) + job.at;
+    job.len_q = __builtin_amdgcn_readlane(n, l);
+    job.nq = job.len_q - job.at < QT ? job.len_q - job.at : QT;
+    job.k0 = __builtin_amdgcn_readlane(k0, l);
+    job.nk = __builtin_amdgcn_readlane(nk, l);
+    return true;
 }
 
 // Blocks of one kv head share its rows, so where the heads divide over the 8
@@ -142,7 +141,8 @@ __device__ __forceinline__ int swz(int row) {
 }
 
 // Rows in global memory from `first` on, `bytes` of them, read 16 bytes a lane straight into
-// LDS at lds + 16 * lane. Reads from `bytes` on (checked by the hardware) give zeros.
+// LDS at lds + 16 * lane, or into registers. Reads from `bytes` on (checked by the hardware)
+// give zeros, writes there do nothing.
 struct Rows {
     __amdgpu_buffer_rsrc_t rs;
     __device__ __forceinline__ Rows(const void* first, int64_t bytes)
@@ -150,27 +150,41 @@ struct Rows {
     __device__ __forceinline__ void to_lds(void* lds, unsigned offset) const {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16, offset, 0, 0, 0);
     }
+    template <class V>
+    __device__ __forceinline__ V load16(unsigned offset) const {
+        return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(rs, offset, 0, 0));
+    }
+    template <class V>
+    __device__ __forceinline__ void store8(V v, unsigned offset) const {
+        typedef unsigned v2u __attribute__((ext_vector_type(2)));
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, v), rs, offset, 0, 0);
+    }
 };
+constexpr unsigned kNoRow = 0x80000000u;  // an offset behind every row
 
-// FULL: head_dim is HDP; else a tile's columns behind head_dim are zeros.
-template <class T, int HDP, int KT, bool FULL>
-__global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(PackedAttnArgs a) {
+// HC: columns worked on, head_dim rounded up (zeros behind it); HDP: those of an LDS row, a
+// power of two. SPLIT 2: waves 4 to 7 take every other tile of keys for the same
+// queries, joined at the end.
+template <class T, int HDP, int HC, int KT, int SPLIT>
+__global__ __launch_bounds__(256 * SPLIT, HDP <= 128 ? 2 : 1) void packed_attn_16(PackedAttnArgs a) {
     typedef typename Vec8<T>::type v8;
     constexpr int QT = 128, NK = KT / 32;
     constexpr int CH = HDP / 8;             // chunks of a row
     constexpr int LOADS = KT * CH / 256;    // chunks per thread of a K or V tile
-    constexpr int DT = HDP / 32, KS = HDP / 16;
+    constexpr int DT = HC / 32, KS = HC / 16;
+    constexpr int TILE = KT * HDP;
     constexpr unsigned kExp = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;  // exponent bits: all set where not finite
-    __shared__ __attribute__((aligned(16))) T K0[KT * HDP], K1[KT * HDP], V0[KT * HDP], V1[KT * HDP];
+    __shared__ __attribute__((aligned(16))) T K0[SPLIT * TILE], K1[SPLIT * TILE], V0[SPLIT * TILE], V1[SPLIT * TILE];
 
     int tile, head;
     tile_and_head(a, tile, head);
     Job job;
     if (!find_job<QT>(a, tile, job)) return;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int part = SPLIT == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int n = lane & 31, hf = lane >> 5;
-    const int hd = FULL ? HDP : a.head_dim;
+    const int hd = a.head_dim;
     const int kvh = __builtin_amdgcn_readfirstlane(head / (a.n_q / a.n_kv));
     const T* Kg = static_cast<const T*>(a.K) + (size_t)job.k0 * a.ldk + kvh * hd;
     const T* Vg = static_cast<const T*>(a.V) + (size_t)job.k0 * a.ldv + kvh * hd;
@@ -180,14 +194,13 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(Packed
     // the sign goes to the queries, so that larger products are larger scores; 0 becomes the
     // smallest factor, which leaves scores at 0 and masked ones at -inf
     const float c2 = a.scale == 0.0f ? 1.17549435e-38f : fabsf(a.scale) * kLog2e;
+    const Rows qrows(static_cast<const T*>(a.Q) + (size_t)job.q0 * a.ldq + head * hd, (int64_t)job.nq * a.ldq * (int)sizeof(T));
     v8 qv[KS];
 #pragma unroll
     for (int s = 0; s < KS; s++) {
         const int d = 16 * s + 8 * hf;
-        v8 z = {};
-        if (qok && d < hd) z = *reinterpret_cast<const v8*>(static_cast<const T*>(a.Q) + (size_t)(job.q0 + qi) * a.ldq + head * hd + d);
-        if (a.scale < 0.0f) z = -z;
-        qv[s] = z;
+        qv[s] = qrows.load16<v8>(qok && d < hd ? (unsigned)(qi * (int)a.ldq + d) * (int)sizeof(T) : kNoRow);
+        if (a.scale < 0.0f) qv[s] = -qv[s];
     }
     // keys [0, lim) are seen by the lane's query, [0, wave_all) by all of the wave's,
     // [wave_end, ..) by none of them
@@ -201,7 +214,8 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(Packed
     const int wave_end = wave * 32 < job.nq ? limit(wq_last) : 0;
     const int wave_all = wave * 32 < job.nq ? limit(wave * 32) : 0;
     const int end = limit(job.nq - 1);
-    const int tiles = (end + KT - 1) / KT, plain = limit(0) / KT;  // tiles [0, plain) are seen whole by every query
+    // a turn is SPLIT tiles; turns [0, plain) are seen whole by every query
+    const int turns = (end + SPLIT * KT - 1) / (SPLIT * KT), plain = limit(0) / (SPLIT * KT);
 
     typedef __attribute__((address_space(3))) v4s* trptr;
     // 16-byte piece e of a tile is chunk e % CH of row e / CH, which holds the row's chunk
@@ -210,32 +224,35 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(Packed
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
         const int e = tid + 256 * i, row = e / CH, d = ((e % CH) ^ swz<HDP>(row)) * 8;
-        const bool in = FULL || d < hd;  // behind head_dim: behind every row, zeros
-        ko[i] = in ? (unsigned)(row * (int)a.ldk + d) * sizeof(T) : 0x80000000u;
-        vo[i] = in ? (unsigned)(row * (int)a.ldv + d) * sizeof(T) : 0x80000000u;
+        const bool in = d < hd;  // behind head_dim: behind every row, zeros
+        ko[i] = in ? (unsigned)(row * (int)a.ldk + d) * (int)sizeof(T) : kNoRow;
+        vo[i] = in ? (unsigned)(row * (int)a.ldv + d) * (int)sizeof(T) : kNoRow;
     }
-    auto issue = [&](int t, T* kd, T* vd) {
+    auto issue = [&](int turn, T* kd, T* vd) {
+        const int t = turn * SPLIT + part;
         // the rows from the tile's first to the last key: reads behind them give zeros
-        const int64_t rows = end - t * KT;
+        const int64_t rows = end - t * KT > 0 ? end - t * KT : 0;
         const int64_t kb = rows * a.ldk * (int)sizeof(T), vb = rows * a.ldv * (int)sizeof(T);
-        const Rows kt(Kg + (size_t)t * KT * a.ldk, kb), vt(Vg + (size_t)t * KT * a.ldv, vb);
+        const Rows kt(Kg + (size_t)t * KT * a.ldk, kb), vt(Vg + (size_t)t * KT * a.ldv, vb);  // (no rows: nothing is read)
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
-            kt.to_lds(kd + (256 * i + wave * 64) * 8, ko[i]);
-            vt.to_lds(vd + (256 * i + wave * 64) * 8, vo[i]);
+            kt.to_lds(kd + part * TILE + (256 * i + wave * 64) * 8, ko[i]);
+            vt.to_lds(vd + part * TILE + (256 * i + wave * 64) * 8, vo[i]);
         }
     };
     v16f o[DT] = {};
     float m = -INFINITY, l = 0.0f;  // the reference of the weights, in log2, and their sum
     int cleaned = 0x7fffffff;       // first key of the first tile with values taken out
 
-    // one tile of keys; MASKED: some query of the block does not see all of it
-    auto step = [&]<bool MASKED>(int k0, const T* Kt, T* Vt) {
-        if constexpr (MASKED) {
+    // one tile of keys; masked: some query of the block does not see all of the turn's. One
+    // code for both, twice over for the two buffers: a block of a short prompt runs through it
+    // once, and fetching it costs more than the branches (a first turn of 2.2 us against 1.4).
+    auto step = [&](bool masked, int k0, const T* Kt, T* Vt) {
+        if (masked) {
             // A value that is not finite must not meet a zero weight in the product.
             // Such values are taken out here and added at the end to the queries that see them.
             int bad = 0;
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < LOADS; i++) {
                 const uint4 w = *reinterpret_cast<const uint4*>(Vt + (tid + 256 * i) * 8);
                 const unsigned u[4] = {w.x, w.y, w.z, w.w};
@@ -243,14 +260,15 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(Packed
                 for (int x = 0; x < 4; x++) bad |= (u[x] & kExp) == kExp || (u[x] >> 16 & kExp) == kExp;
             }
             if (__syncthreads_or(bad)) {
-                cleaned = cleaned < k0 ? cleaned : k0;
+                cleaned = cleaned < k0 - part * KT ? cleaned : k0 - part * KT;
                 unsigned short* w = reinterpret_cast<unsigned short*>(Vt);
-                for (int e = tid; e < KT * HDP; e += 256)
+#pragma unroll 1
+                for (int e = tid; e < TILE; e += 256)
                     if ((w[e] & kExp) == kExp) w[e] = 0;
                 __syncthreads();
             }
-            if (k0 >= wave_end) return;
         }
+        if (k0 >= wave_end) return;
         v16f s[NK] = {};
 #pragma unroll
         for (int x = 0; x < KS; x++)
@@ -268,12 +286,13 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(Packed
             __builtin_amdgcn_sched_group_barrier(0x100, NK, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x8, 2 * NK, 0);
-        if (MASKED && k0 + KT > wave_all) {
+        if (k0 + KT > wave_all) {
+            const int seen = lim - k0 - 4 * hf;
 #pragma unroll
             for (int kt = 0; kt < NK; kt++)
 #pragma unroll
                 for (int i = 0; i < 16; i++)
-                    if (k0 + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3) >= lim) s[kt][i] = -INFINITY;
+                    if (32 * kt + 8 * (i >> 2) + (i & 3) >= seen) s[kt][i] = -INFINITY;
         }
         float mx = s[0][0];
 #pragma unroll
@@ -326,27 +345,49 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(Packed
         }
         __builtin_amdgcn_sched_group_barrier(0x8, 4, 1);
     };
-    // tiles alternate between the two buffers; the next one is loaded while this one is worked on
-    auto turn = [&]<bool MASKED>(int t, T* kc, T* vc, T* kn, T* vn) {
-        if (t + 1 < tiles) issue(t + 1, kn, vn);
-        step.template operator()<MASKED>(t * KT, kc, vc);
+    // turns alternate between the two buffers; the next one is loaded while this one is worked on
+    auto turn = [&](int t, T* kc, T* vc, T* kn, T* vn) {
+        if (t + 1 < turns) issue(t + 1, kn, vn);
+        step(t >= plain, (t * SPLIT + part) * KT, kc + part * TILE, vc + part * TILE);
         wait_loads();
         __syncthreads();
     };
 
-    if (tiles) issue(0, K0, V0);
+    if (turns) issue(0, K0, V0);
     wait_loads();
     __syncthreads();
-    int t = 0;
-    for (; t + 2 <= plain; t += 2) {
-        turn.template operator()<false>(t, K0, V0, K1, V1);
-        turn.template operator()<false>(t + 1, K1, V1, K0, V0);
-    }
-    for (; t < tiles; t += 2) {
-        turn.template operator()<true>(t, K0, V0, K1, V1);
-        if (t + 1 < tiles) turn.template operator()<true>(t + 1, K1, V1, K0, V0);
+    for (int t = 0; t < turns; t += 2) {
+        turn(t, K0, V0, K1, V1);
+        if (t + 1 < turns) turn(t + 1, K1, V1, K0, V0);
     }
 
+    if constexpr (SPLIT == 2) {
+        // Every wave of the second half leaves its state to the one with its queries, lane by
+        // lane: 32 x HC floats, half of what K0 or K1 holds.
+        static_assert(HDP <= 128);
+        float* x = reinterpret_cast<float*>(wave < 2 ? K0 : K1) + (wave & 1) * 32 * HC + lane;
+        __shared__ float ml[4][2][64];
+        if (part == 1) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[(d * 16 + i) * 64] = o[d][i];
+            ml[wave][0][lane] = m;
+            ml[wave][1][lane] = l;
+        }
+        __syncthreads();
+        if (part == 1) return;
+        const float m1 = ml[wave][0][lane], l1 = ml[wave][1][lane];
+        const float mn = fmaxf(m, m1), mu = mn == -INFINITY ? 0.0f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(m1 - mu);
+        l = l * f0 + l1 * f1;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] = o[d][i] * f0 + x[(d * 16 + i) * 64] * f1;
+    }
+
+#pragma unroll 1
     for (int j = cleaned; j < end; j++) {
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -360,8 +401,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(Packed
 
     l = halves_sum(l);
     const float inv = 1.0f / l;
-    if (!qok) return;
-    T* dst = static_cast<T*>(a.out) + (size_t)(job.q0 + qi) * a.ldo + head * hd;
+    const Rows orows(static_cast<const T*>(a.out) + (size_t)job.q0 * a.ldo + head * hd, (int64_t)job.nq * a.ldo * (int)sizeof(T));
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -370,7 +410,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void packed_attn_16(Packed
             Pack<T, 4> z;
 #pragma unroll
             for (int r = 0; r < 4; r++) z.v[r] = (T)(l == 0.0f ? 0.0f : o[d][4 * i + r] * inv);
-            if (col < hd) *reinterpret_cast<Pack<T, 4>*>(dst + col) = z;
+            orows.store8(z, qok && col < hd ? (unsigned)(qi * (int)a.ldo + col) * (int)sizeof(T) : kNoRow);
         }
 }
 
@@ -557,32 +597,45 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
     }
 }
 
+// the most tiles of qt queries that n_seqs sequences of total_q rows can have
+int64_t max_tiles(const PackedAttnArgs& a, int qt) { return a.total_q / qt + (a.n_seqs < a.total_q ? a.n_seqs : a.total_q); }
+
 template <class F>
-void launch_lds(F* kernel, const PackedAttnArgs& a, int qt, int lds, hipStream_t st) {
+void launch_tiles(F* kernel, const PackedAttnArgs& a, int qt, int threads, int lds, hipStream_t st) {
     if (lds > 65536)
         VLA_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    // the most tiles that n_seqs sequences of total_q rows can have
-    const int64_t tiles = a.total_q / qt + (a.n_seqs < a.total_q ? a.n_seqs : a.total_q);
-    const int64_t blocks = tiles * a.n_q;
+    const int64_t blocks = max_tiles(a, qt) * a.n_q;
     VLA_REQUIRE(blocks < (int64_t)1 << 31, "packed_attention: too many rows times heads for one call");
-    kernel<<<(unsigned)blocks, 256, lds, st>>>(a);
+    kernel<<<(unsigned)blocks, threads, lds, st>>>(a);
     VLA_LAUNCH_CHECK();
 }
 
-template <class T, int HDP, int KT>
-void run_16(const PackedAttnArgs& a, hipStream_t st) {
-    if (a.head_dim == HDP) launch_lds(&packed_attn_16<T, HDP, KT, true>, a, 128, 0, st);
-    else launch_lds(&packed_attn_16<T, HDP, KT, false>, a, 128, 0, st);
+template <class T, int HDP, int HC, int KT, int SPLIT>
+void run_16_split(const PackedAttnArgs& a, hipStream_t st) {
+    launch_tiles(&packed_attn_16<T, HDP, HC, KT, SPLIT>, a, 128, 256 * SPLIT, 0, st);
+}
+// Two halves of the keys per block where the blocks would leave CUs idle or alone and the
+// sequences have some length. Measured, us, one half | two: 128 blocks of 512 keys 17.8 | 16.4,
+// 108 of 1024 (no mask, heads of 64) 17.1 | 15.0, 288 of 1024 27.6 | 24.2; the same where a
+// block has but one tile, 32 of 64 keys 8.0 | 10.2, and with more blocks, 324 of 1024 26.9 |
+// 29.4, 1024 of 512 46 | 57, one prompt of 8192 528 | 560.
+template <class T, int HDP, int HC>
+void run_16_hc(const PackedAttnArgs& a, hipStream_t st) {
+    if (max_tiles(a, 128) * a.n_q <= 304 && a.total_k >= (int64_t)256 * a.n_seqs) run_16_split<T, HDP, HC, 64, 2>(a, st);
+    else run_16_split<T, HDP, HC, 64, 1>(a, st);
 }
 template <class T>
 void run_16(const PackedAttnArgs& a, hipStream_t st) {
-    if (a.head_dim <= 64) run_16<T, 64, 64>(a, st);
-    else if (a.head_dim <= 128) run_16<T, 128, 64>(a, st);
-    else run_16<T, 256, 32>(a, st);
+    if (a.head_dim <= 32) run_16_hc<T, 64, 32>(a, st);
+    else if (a.head_dim <= 64) run_16_hc<T, 64, 64>(a, st);
+    else if (a.head_dim <= 96) run_16_hc<T, 128, 96>(a, st);
+    else if (a.head_dim <= 128) run_16_hc<T, 128, 128>(a, st);
+    else if (a.head_dim <= 192) run_16_split<T, 256, 192, 32, 1>(a, st);
+    else run_16_split<T, 256, 256, 32, 1>(a, st);
 }
 template <int HDP>
 void run_f32(const PackedAttnArgs& a, hipStream_t st) {
-    launch_lds(&packed_attn_f32<HDP>, a, 64, 2 * 32 * (HDP + 4) * 4, st);
+    launch_tiles(&packed_attn_f32<HDP>, a, 64, 256, 2 * 32 * (HDP + 4) * 4, st);
 }
 
 }  // namespace
@@ -602,7 +655,8 @@ void launch_packed_attention(const PackedAttnArgs& a, hipStream_t st) {
     VLA_REQUIRE(aligned(a.Q, 16) && aligned(a.K, 16) && aligned(a.V, 16) && aligned(a.out, 16) && a.ldq * sz % 16 == 0 &&
                     a.ldk * sz % 16 == 0 && a.ldv * sz % 16 == 0 && a.ldo * sz % 16 == 0,
                 "packed_attention: rows must be 16-byte aligned");
-    VLA_REQUIRE(a.ldk < 1 << 22 && a.ldv < 1 << 22, "packed_attention: row stride of K or V past 2^22 values");
+    VLA_REQUIRE(a.ldq < 1 << 22 && a.ldk < 1 << 22 && a.ldv < 1 << 22 && a.ldo < 1 << 22,
+                "packed_attention: row stride past 2^22 values");
     VLA_REQUIRE(a.ldq >= a.n_q * a.head_dim && a.ldo >= a.n_q * a.head_dim && a.ldk >= a.n_kv * a.head_dim &&
                     a.ldv >= a.n_kv * a.head_dim,
                 "packed_attention: row stride shorter than heads * head_dim");
