@@ -390,8 +390,12 @@ def test_decode_single_tokens(vla, dtype, n_q, n_kv, hd, page):
     ref.within(got, want, bound)
     # without offsets: row s is sequence s's
     out = torch.empty_like(q, device=DEV)
-    vla.kv4_attention_dev(out, q.to(DEV), cache, n_q, n_kv, hd, page, hd ** -0.5, table, _i32(lens))
+    work = torch.empty(max(16, vla.kv4_attention_work_bytes(8, 8, 1, 200, n_q, n_kv, hd)), dtype=torch.uint8, device=DEV)
+    vla.kv4_attention_dev(out, q.to(DEV), cache, n_q, n_kv, hd, page, hd ** -0.5, table, _i32(lens), max_len=200, work=work)
     assert torch.equal(out, got)
+    out.fill_(5.0)
+    vla.kv4_attention_dev(out, q.to(DEV), cache, n_q, n_kv, hd, page, hd ** -0.5, table, _i32(lens))
+    ref.within(out, want, bound, "a block per sequence")
 
 
 @pytest.mark.parametrize("dtype", TYPES)
