@@ -18,7 +18,8 @@
 // 16-bit types: the weights are rounded to the operands' type for the second product
 // (2^-9 of a weight for bf16, 2^-12 for fp16, each on its own, as large as the
 // rounding of the result); the sum l is of the unrounded ones.
-// fp32: both products on the fp32 matrix cores, nothing rounded.
+// fp32 up to 128 columns: both products from three bf16 parts of each operand, as exact as
+// fp32 products; past that on the fp32 matrix cores.
 
 #include "serving.h"
 #include "wave.h"
@@ -71,7 +72,9 @@ __device__ __forceinline__ int clamp_row(int x, int total) { return x < 0 ? 0 : 
 // are read clamped to the buffers' rows, a sequence that would end before it
 // begins as empty, so that no offsets can lead out of the buffers. Every wave does the same
 // search, 64 sequences at a time; tiles are counted from the last one of the
-// last sequence, as queries late in a sequence see the most keys under a causal mask.
+// last sequence, as queries late in a sequence see the most keys under a causal mask. (Counted by
+// their depth over all sequences, the deepest first, 12 mixed prompts took 224 us for 212: the
+// search is longer, and neighbours no longer share keys.)
 template <int QT>
 __device__ __forceinline__ bool find_job(const PackedAttnArgs& a, int tile, Job& job) {
     const int lane = threadIdx.x & 63;
@@ -158,6 +161,11 @@ struct Rows {
     __device__ __forceinline__ void store8(V v, unsigned offset) const {
         typedef unsigned v2u __attribute__((ext_vector_type(2)));
         __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, v), rs, offset, 0, 0);
+    }
+    template <class V>
+    __device__ __forceinline__ void store16(V v, unsigned offset) const {
+        typedef unsigned v4u __attribute__((ext_vector_type(4)));
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u, v), rs, offset, 0, 0);
     }
 };
 constexpr unsigned kNoRow = 0x80000000u;  // an offset behind every row
@@ -414,7 +422,330 @@ __global__ __launch_bounds__(256 * SPLIT, HDP <= 128 ? 2 : 1) void packed_attn_1
         }
 }
 
-// ------------------------------------------------------------- fp32 ----
+// ---------------------------------------------- fp32 up to 128 columns ----
+// Each operand as three bf16 parts, h + m + l = x to 2^-25 of it: h its upper 16 bits, m and l the
+// rounded rests. Of the nine products six are formed, h h, h m, m h, m m, h l and l h; m l, l m
+// and l l stay below 2^-22 of |x y|, a few roundings of an fp32 sum. Six bf16 products
+// run at 2.6 times the rate of one on the fp32 matrix cores, and bf16 has fp32's range.
+// Parts of what is not finite would not add up again: such rows of K are marked and
+// their scores formed with fp32 products, such values of V are taken out and added at the
+// end to the queries that see them.
+// K and V rows go through registers, which split them, into LDS planes [3][KT][HDP] with the
+// layout of the 16-bit kernel; the next tile's are loaded while this one is worked on.
+
+struct Parts {
+    v8bf h, m, l;
+};
+__device__ __forceinline__ Parts split8(const float* x) {
+    Parts p;
+    typedef unsigned v4u __attribute__((ext_vector_type(4)));
+    v4u h;
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const unsigned a = __float_as_uint(x[2 * i]), b = __float_as_uint(x[2 * i + 1]);
+        h[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        r[2 * i] = x[2 * i] - __uint_as_float(a & 0xffff0000u);
+        r[2 * i + 1] = x[2 * i + 1] - __uint_as_float(b & 0xffff0000u);
+    }
+    p.h = __builtin_bit_cast(v8bf, h);
+#pragma unroll
+    for (int i = 0; i < 8; i++) p.m[i] = (bf16_t)r[i];
+#pragma unroll
+    for (int i = 0; i < 8; i++) p.l[i] = (bf16_t)(r[i] - (float)p.m[i]);
+    return p;
+}
+
+// c + x y, the smaller products first
+__device__ __forceinline__ v16f mfma_parts(const Parts& x, const Parts& y, v16f c) {
+    c = mfma32(x.l, y.h, c);
+    c = mfma32(x.h, y.l, c);
+    c = mfma32(x.m, y.m, c);
+    c = mfma32(x.m, y.h, c);
+    c = mfma32(x.h, y.m, c);
+    return mfma32(x.h, y.h, c);
+}
+
+// KP 2 and 4: so many waves share 32 queries and a tile's keys, joined at the end; the block has
+// 64 queries then.
+constexpr int parts_threads(int kp) { return kp == 4 ? 512 : 256; }
+
+template <int HDP, int HC, int KT, int KP>
+__global__ __launch_bounds__(parts_threads(KP), KP == 4 || KT * HC <= 4096 && HC <= 96 ? 2 : 1) void packed_attn_parts(PackedAttnArgs a) {
+    constexpr int NTH = parts_threads(KP), QT = KP == 1 ? 128 : 64, NK = KT / 32 / KP;  // 32-key steps of a wave
+    constexpr int CH = HDP / 8;             // 8-value pieces of a row
+    constexpr int LOADS = KT * CH / NTH;    // pieces per thread of a K or V tile
+    constexpr int DT = HC / 32, KS = HC / 16;
+    constexpr int PLANE = KT * HDP;
+    __shared__ __attribute__((aligned(16))) bf16_t Ks[3 * PLANE], Vs[3 * PLANE];
+    __shared__ unsigned long long kbad[2][KT <= 64 ? 1 : 2];  // rows of the tile with values that are not finite
+    __shared__ int vbad;                    // first key of the first tile with such values of V
+
+    int tile, head;
+    tile_and_head(a, tile, head);
+    Job job;
+    if (!find_job<QT>(a, tile, job)) return;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, hf = lane >> 5;
+    const int hd = a.head_dim;
+    const int kvh = __builtin_amdgcn_readfirstlane(head / (a.n_q / a.n_kv));
+    const float* Kg = static_cast<const float*>(a.K) + (size_t)job.k0 * a.ldk + kvh * hd;
+    const float* Vg = static_cast<const float*>(a.V) + (size_t)job.k0 * a.ldv + kvh * hd;
+
+    const int off = job.nk - job.len_q + job.at + 1;
+    auto limit = [&](int q) {
+        const int e = a.causal ? q + off : job.nk;
+        return e < 0 ? 0 : (e < job.nk ? e : job.nk);
+    };
+    const int qw = KP == 1 ? wave : wave & 1, kp = KP == 1 ? 0 : wave >> 1;
+    const int kw = kp * 32 * NK;  // the wave's first key of a tile
+    const int qi = qw * 32 + n;
+    const bool qok = qi < job.nq;
+    const int lim = qok ? limit(qi) : 0;
+    const int wq_last = qw * 32 + 31 < job.nq ? qw * 32 + 31 : job.nq - 1;
+    const int wave_end = qw * 32 < job.nq ? limit(wq_last) : 0;
+    const int wave_all = qw * 32 < job.nq ? limit(qw * 32) : 0;
+    const int end = limit(job.nq - 1);
+    const int tiles = (end + KT - 1) / KT;
+
+    unsigned ko[LOADS], vo[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+        const int e = tid + NTH * i, row = e / CH, d = (e % CH) * 8;
+        ko[i] = d < hd ? (unsigned)(row * (int)a.ldk + d) * 4u : kNoRow;
+        vo[i] = d < hd ? (unsigned)(row * (int)a.ldv + d) * 4u : kNoRow;
+    }
+    float kr[LOADS][8], vr[LOADS][8];
+    auto fetch = [&](int t) {
+        const int64_t rows = end - t * KT;
+        const Rows kt(Kg + (size_t)t * KT * a.ldk, rows * a.ldk * 4), vt(Vg + (size_t)t * KT * a.ldv, rows * a.ldv * 4);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const float4 k = kt.load16<float4>(ko[i] + 16 * h), v = vt.load16<float4>(vo[i] + 16 * h);
+                kr[i][4 * h] = k.x, kr[i][4 * h + 1] = k.y, kr[i][4 * h + 2] = k.z, kr[i][4 * h + 3] = k.w;
+                vr[i][4 * h] = v.x, vr[i][4 * h + 1] = v.y, vr[i][4 * h + 2] = v.z, vr[i][4 * h + 3] = v.w;
+            }
+    };
+    auto finite8 = [](const float* x) {
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const unsigned u = __float_as_uint(x[i]) & 0x7fffffffu;
+            top = u > top ? u : top;
+        }
+        return top < 0x7f800000u;
+    };
+    auto put = [&](bf16_t* planes, int e, const float* x) {
+        const Parts p = split8(x);
+        const int row = e / CH, at = row * HDP + ((e % CH) ^ swz<HDP>(row)) * 8;
+        *reinterpret_cast<v8bf*>(planes + at) = p.h;
+        *reinterpret_cast<v8bf*>(planes + PLANE + at) = p.m;
+        *reinterpret_cast<v8bf*>(planes + 2 * PLANE + at) = p.l;
+    };
+    auto land = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int e = tid + NTH * i;
+            if (!finite8(kr[i])) {
+                atomicOr(&kbad[t & 1][e / CH >> 6], 1ull << (e / CH & 63));
+#pragma unroll
+                for (int x = 0; x < 8; x++) kr[i][x] = 0.0f;
+            }
+            if (!finite8(vr[i])) {
+                atomicMin(&vbad, t * KT);
+#pragma unroll
+                for (int x = 0; x < 8; x++)
+                    if (!(fabsf(vr[i][x]) < INFINITY)) vr[i][x] = 0.0f;
+            }
+            put(Ks, e, kr[i]);
+            put(Vs, e, vr[i]);
+        }
+    };
+
+    if (tiles) fetch(0);
+    const float c2 = a.scale == 0.0f ? 1.17549435e-38f : fabsf(a.scale) * kLog2e;  // as in the 16-bit kernel
+    const Rows qrows(static_cast<const float*>(a.Q) + (size_t)job.q0 * a.ldq + head * hd, (int64_t)job.nq * a.ldq * 4);
+    Parts qv[KS];
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const int d = 16 * s + 8 * hf;
+        const unsigned o = qok && d < hd ? (unsigned)(qi * (int)a.ldq + d) * 4u : kNoRow;
+        const float4 x = qrows.load16<float4>(o), y = qrows.load16<float4>(o + 16);
+        float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        if (a.scale < 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i] = -f[i];
+        }
+        qv[s] = split8(f);
+    }
+    if (tid == 0) {
+        for (auto& w : kbad)
+            for (auto& x : w) x = 0;
+        vbad = 0x7fffffff;
+    }
+
+    v16f o[DT] = {};
+    float m = -INFINITY, l = 0.0f;
+    typedef __attribute__((address_space(3))) v4s* trptr;
+    for (int t = 0; t < tiles; t++) {
+        const int k0 = t * KT;
+        __syncthreads();  // the previous tile is read
+        land(t);
+        __syncthreads();
+        if (t + 1 < tiles) fetch(t + 1);
+        const unsigned long long marked = kbad[t & 1][kw >> 6] >> (kw & 63);  // of the wave's keys on
+        if (tid == 0)
+            for (auto& x : kbad[(t + 1) & 1]) x = 0;
+        if (k0 + kw >= wave_end) continue;
+        v16f s[NK] = {};
+#pragma unroll
+        for (int x = 0; x < KS; x++)
+#pragma unroll
+            for (int kt = 0; kt < NK; kt++) {
+                const int row = kw + 32 * kt + n, at = row * HDP + ((2 * x + hf) ^ swz<HDP>(row)) * 8;
+                const Parts k{*reinterpret_cast<const v8bf*>(Ks + at), *reinterpret_cast<const v8bf*>(Ks + PLANE + at),
+                              *reinterpret_cast<const v8bf*>(Ks + 2 * PLANE + at)};
+                s[kt] = mfma_parts(k, qv[x], s[kt]);
+            }
+        if (marked) {
+#pragma unroll 1
+            for (int j = 0; j < 32 * NK; j++) {
+                if (!(marked >> j & 1) || k0 + kw + j >= end) continue;
+                unsigned at = 0;
+                asm volatile("" : "+v"(at));  // (keeps all of this inside the branch)
+                const Rows krow(Kg + (size_t)(k0 + kw + j) * a.ldk, (int64_t)hd * 4);
+                float dot = 0.0f;
+#pragma unroll 1
+                for (int d = 8 * hf; d < hd; d += 16)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) {
+                        const float4 q = qrows.load16<float4>(qok ? (unsigned)(qi * (int)a.ldq + d + e) * 4u + at : kNoRow);
+                        const float4 k = krow.load16<float4>((d + e) * 4u + at);
+                        dot += q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
+                    }
+                dot = halves_sum(a.scale < 0.0f ? -dot : dot);
+#pragma unroll
+                for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3) == j) s[kt][i] = dot;
+            }
+        }
+        if (k0 + KT > wave_all) {
+            const int seen = lim - k0 - kw - 4 * hf;
+#pragma unroll
+            for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (32 * kt + 8 * (i >> 2) + (i & 3) >= seen) s[kt][i] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[kt][i]);
+        mx = halves_max(mx) * c2;
+        if (__any(mx > m + 6.0f)) {  // as in the 16-bit kernel
+            const float mn = fmaxf(m, mx);
+            const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] *= alpha;
+        }
+        const float mu = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                float w[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][8 * x + i], c2, -mu));
+                    l += w[i];
+                }
+                const Parts p = split8(w);
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    const int r = kw + 32 * kt + 16 * x + 4 * hf + (lane >> 2 & 3);
+                    const int col = 32 * d + (lane >> 4 & 1) * 16 + (lane & 3) * 4, c = col >> 3, in = col & 7;
+                    const int a0 = r * HDP + (c ^ swz<HDP>(r)) * 8 + in, a1 = (r + 8) * HDP + (c ^ swz<HDP>(r + 8)) * 8 + in;
+                    auto frag = [&](const bf16_t* plane) {
+                        const v4s y0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((trptr)(plane + a0));
+                        const v4s y1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((trptr)(plane + a1));
+                        return __builtin_bit_cast(v8bf, __builtin_shufflevector(y0, y1, 0, 1, 2, 3, 4, 5, 6, 7));
+                    };
+                    o[d] = mfma_parts(Parts{frag(Vs), frag(Vs + PLANE), frag(Vs + 2 * PLANE)}, p, o[d]);
+                }
+            }
+    }
+    __syncthreads();
+    if constexpr (KP > 1) {  // lane by lane, as the two halves of the 16-bit kernel
+        static_assert((KP - 1) * 2 * 32 * HC * 4 <= (int)sizeof(Ks));
+        float* x = reinterpret_cast<float*>(Ks) + qw * 32 * HC + lane;
+        __shared__ float ml[KP][2][2][64];
+        if (kp) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[(kp - 1) * 64 * HC + (d * 16 + i) * 64] = o[d][i];
+        }
+        ml[kp][qw][0][lane] = m;
+        ml[kp][qw][1][lane] = l;
+        __syncthreads();
+        if (kp) return;
+        float mn = m;
+#pragma unroll
+        for (int p = 1; p < KP; p++) mn = fmaxf(mn, ml[p][qw][0][lane]);
+        const float mu = mn == -INFINITY ? 0.0f : mn, f0 = __builtin_amdgcn_exp2f(m - mu);
+        l *= f0;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] *= f0;
+#pragma unroll
+        for (int p = 1; p < KP; p++) {
+            const float f = __builtin_amdgcn_exp2f(ml[p][qw][0][lane] - mu);
+            l += f * ml[p][qw][1][lane];
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] += f * x[(p - 1) * 64 * HC + (d * 16 + i) * 64];
+        }
+    }
+    const int cleaned = vbad;
+#pragma unroll 1
+    for (int j = cleaned; j < end; j++) {
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int col = 32 * d + 8 * (i >> 2) + 4 * hf + (i & 3);
+                const float x = col < hd ? Vg[(size_t)j * a.ldv + col] : 0.0f;
+                if (!(fabsf(x) < INFINITY) && j < lim) o[d][i] += x;
+            }
+    }
+
+    l = halves_sum(l);
+    const float inv = 1.0f / l;
+    const Rows orows(static_cast<const float*>(a.out) + (size_t)job.q0 * a.ldo + head * hd, (int64_t)job.nq * a.ldo * 4);
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int col = 32 * d + 8 * i + 4 * hf;
+            float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (l != 0.0f) z = make_float4(o[d][4 * i] * inv, o[d][4 * i + 1] * inv, o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv);
+            orows.store16(z, qok && col < hd ? (unsigned)(qi * (int)a.ldo + col) * 4u : kNoRow);
+        }
+}
+
+// ---------------------------------------------- fp32 past 128 columns ----
 // A wave owns 16 queries: v_mfma_f32_16x16x4_f32 leaves in lane n + 16 g, for query
 // n, the scores of keys 4 g + r of 16, and takes weight r of the lane as key 4 g
 // + r of its step r. The head dimension is walked as d = g * (HDP / 4) + s, so
@@ -633,9 +964,28 @@ void run_16(const PackedAttnArgs& a, hipStream_t st) {
     else if (a.head_dim <= 192) run_16_split<T, 256, 192, 32, 1>(a, st);
     else run_16_split<T, 256, 256, 32, 1>(a, st);
 }
-template <int HDP>
+// Two waves to 32 queries where the blocks of four times 32 would leave CUs idle, four where
+// sequences have some length. Measured, us, one wave | two | four: 75 blocks of 512 keys (heads
+// of 64) 33 | 26 | 21.5, 108 of 1024 (no mask) - | 45 | 36, 288 of 1024 61 | 60 | 49; 165 of mixed lengths up to
+// 177 15.5 | 13.5 | 13.7, 285 of 177 17.0 | 17.6 | 24, 15 of 64 - | 8.6 | 10.4; heads of 128: 160 of 512 67 | 45,
+// 544 of 2048 253 | 320. The fp32 matrix cores took 30, -, 88, 14.4, 21.8, 7.9 | 52, 361.
+template <int HDP, int HC>
+void run_parts(const PackedAttnArgs& a, hipStream_t st) {
+    if constexpr (HDP == 64) {
+        if (max_tiles(a, 64) * a.n_q <= 768 && a.total_k >= (int64_t)384 * a.n_seqs) {
+            launch_tiles(&packed_attn_parts<64, HC, 128, 4>, a, 64, 512, 0, st);
+            return;
+        }
+    }
+    if (max_tiles(a, 128) * a.n_q <= 256) launch_tiles(&packed_attn_parts<HDP, HC, 64, 2>, a, 64, 256, 0, st);
+    else launch_tiles(&packed_attn_parts<HDP, HC, HDP == 64 ? 64 : 32, 1>, a, 128, 256, 0, st);
+}
 void run_f32(const PackedAttnArgs& a, hipStream_t st) {
-    launch_tiles(&packed_attn_f32<HDP>, a, 64, 256, 2 * 32 * (HDP + 4) * 4, st);
+    if (a.head_dim <= 32) run_parts<64, 32>(a, st);
+    else if (a.head_dim <= 64) run_parts<64, 64>(a, st);
+    else if (a.head_dim <= 96) run_parts<128, 96>(a, st);
+    else if (a.head_dim <= 128) run_parts<128, 128>(a, st);
+    else launch_tiles(&packed_attn_f32<256>, a, 64, 256, 2 * 32 * (256 + 4) * 4, st);
 }
 
 }  // namespace
@@ -662,9 +1012,7 @@ void launch_packed_attention(const PackedAttnArgs& a, hipStream_t st) {
                 "packed_attention: row stride shorter than heads * head_dim");
     if (a.dtype == kBf16) run_16<bf16_t>(a, st);
     else if (a.dtype == kF16) run_16<f16_t>(a, st);
-    else if (a.head_dim <= 64) run_f32<64>(a, st);
-    else if (a.head_dim <= 128) run_f32<128>(a, st);
-    else run_f32<256>(a, st);
+    else run_f32(a, st);
 }
 
 }  // namespace hip
