@@ -87,6 +87,19 @@ def test_rope_far_positions(vla):
     ref.within(o, want, bound + 2.0 ** -20 * (x.double().abs().max() * 2), "far")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [1e25, 1e-25])
+def test_norm_beyond_the_range_of_squares(vla, dtype, size):
+    """Values whose squares overflow or vanish in 32 bits are normed all the same."""
+    x = (_rows(_gen(6), 5, 2 * 64, F32) * size).to(dtype)
+    pos = torch.arange(5, dtype=torch.int32)[None]
+    w = torch.ones(64)
+    o = torch.empty(5, 128, dtype=dtype, device=DEV)
+    vla.qk_norm_rope_dev(o, None, x.to(DEV), None, 2, 0, 64, pos.to(DEV), [32], 1e4, w.to(DEV), None, 0.0)
+    want, bound = ref.rope(x, 2, 64, pos, [32], 1e4, w, 0.0)
+    ref.within(o, want, bound)
+
+
 def test_rope_agrees_with_rope_neox(vla, orc):
     x = _rows(_gen(4), 50, 15 * 64, F32)
     pos = np.arange(50, dtype=np.int32) + 3
@@ -155,13 +168,22 @@ def test_packed_heads_and_strides(vla, dtype, n_q, n_kv, hd, pad):
 @pytest.mark.parametrize("dtype", TYPES)
 def test_packed_many_sequences(vla, dtype):
     """More sequences than lanes in the tile search, and single queries over long keys."""
-    lens = [(i * 7) % 5 for i in range(150)]
-    g = _gen(9)
-    q, k, v = _packed_case(g, lens, lens, 2, 1, 64, dtype)
-    got = _run_packed(vla, q, k, v, lens, lens, 2, 1, 64, 0.125, True, same=True)
-    s = _starts(lens)
-    want, bound = ref.packed(q, k, v, s, s, 2, 1, 64, 0.125, True, base=torch.full_like(q, 5.0))
-    ref.within(got, want, bound)
+    for n, long in ((150, 0), (65, 130), (4200, 0)):
+        lens = [(i * 7) % 5 if i % 40 else long for i in range(n)]
+        g = _gen(9)
+        q, k, v = _packed_case(g, lens, lens, 2, 1, 32, dtype)
+        got = _run_packed(vla, q, k, v, lens, lens, 2, 1, 32, 0.125, True, same=True)
+        s = _starts(lens)
+        some = s if n < 1000 else s[:300]  # (the plain form is slow)
+        want, bound = ref.packed(q, k, v, some, some, 2, 1, 32, 0.125, True, base=torch.full_like(q, 5.0))
+        m = q.shape[0] if n < 1000 else some[-1]
+        ref.within(got[:m], want[:m], bound[:m])
+        if n > 1000:
+            # The others: a query alone in its sequence has weight 1 and gives its own value; in fp32 that
+            # value comes as three parts that hold it to u / 2, summed with two roundings of u = 2^-24.
+            alone = [s[i] for i in range(300, n) if lens[i] == 1]
+            want = v[alone].double().repeat(1, 2)
+            ref.within(got[alone], want, want.abs() * (3 * 2.0 ** -24 if dtype is F32 else 0.0))
     qlens, klens = [1, 2], [900, 1025]
     q, k, v = _packed_case(g, qlens, klens, 2, 1, 64, dtype)
     got = _run_packed(vla, q, k, v, qlens, klens, 2, 1, 64, 0.125, True)
@@ -232,6 +254,10 @@ def test_packed_infinite_scores(vla, dtype):
     k[7] = math.inf
     got = _run_packed(vla, q, k, v, lens, lens, 1, 1, 64, 0.125, True, same=True).cpu()
     assert bool(torch.isfinite(got[:7]).all()) and bool(got[7:].isnan().all())
+    k[7] = 1.0
+    k[0] = math.nan  # a query that sees nothing else
+    got = _run_packed(vla, q, k, v, lens, lens, 1, 1, 64, 0.125, True, same=True).cpu()
+    assert bool(got.isnan().all())
 
 
 def test_packed_offsets_are_clamped(vla):
@@ -628,6 +654,30 @@ def test_streams_and_graphs(vla):
         step(eager)
         torch.cuda.synchronize()
         assert torch.equal(got, eager) and torch.equal(pgot, po) and torch.equal(after, cache), i
+
+
+@pytest.mark.parametrize("dtype,hd", [(F32, 64), (F32, 128), (F32, 256), (BF16, 128), (F16, 256)])
+def test_prompt_graph(vla, dtype, hd):
+    """A captured prompt pass: replays follow other lengths in the same buffers."""
+    g = _gen(hd)
+    q, k, v = (t.to(DEV) for t in _packed_case(g, [150, 40], [150, 40], 2, 1, hd, dtype, extra=0))
+    start, out = _i32([0, 150, 190]), torch.zeros_like(q)
+    call = lambda o: vla.packed_attention_dev(o, q, k, v, 2, 1, hd, 0.1, start)
+    call(out)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=st):
+        call(out)
+    for cut in (1, 100, 190, 0):
+        start[1] = cut
+        v.copy_(v.flip(0))
+        out.zero_()
+        gr.replay()
+        eager = torch.zeros_like(out)
+        call(eager)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager), cut
 
 
 def test_repeated_calls_give_the_same_bits(vla):

@@ -811,8 +811,8 @@ def qk_norm_rope_dev(q_out, k_out, q, k, n_q, n_kv, head_dim, pos, sections, bas
         if w is not None and (w.dtype is not _torch.float32 or w.shape != (head_dim,) or not w.is_contiguous()):
             raise ValueError(f"{name}: need {head_dim} contiguous float32")
     _check_devices(pos, q_weight, k_weight, *((q_out, q) if n_q else ()), *((k_out, k) if n_kv else ()))
-    _call("vla_qk_norm_rope_dev", qop, ldqo, kop, ldko, qp, ldq, kp, ldk, _dp(q_weight), _dp(k_weight), eps, pos.data_ptr(),
-          pos.stride(0) if axes > 1 else T, (c_int32 * axes)(*sections), axes, base, T, n_q, n_kv, head_dim, dt,
+    _call("vla_qk_norm_rope_dev", qop, ldqo, kop, ldko, qp, ldq, kp, ldk, _dp(q_weight), _dp(k_weight), float(eps), pos.data_ptr(),
+          pos.stride(0) if axes > 1 else T, (c_int32 * axes)(*sections), axes, float(base), T, n_q, n_kv, head_dim, dt,
           _stream(stream))
 
 
@@ -826,7 +826,7 @@ def packed_attention_dev(out, Q, K, V, n_q, n_kv, head_dim, scale, q_start, k_st
         _check_ints("k_start", k_start, n + 1)
     _check_devices(out, Q, K, V, q_start, k_start)
     _call("vla_packed_attention_dev", out.data_ptr(), ldo, Q.data_ptr(), ldq, K.data_ptr(), ldk, V.data_ptr(), ldv,
-          q_start.data_ptr(), _dp(k_start), n, tq, tk, n_q, n_kv, head_dim, scale, 1 if causal else 0, dt,
+          q_start.data_ptr(), _dp(k_start), n, tq, tk, n_q, n_kv, head_dim, float(scale), 1 if causal else 0, dt,
           _stream(stream))
 
 
@@ -909,7 +909,7 @@ def kv4_attention_dev(out, Q, cache, n_q, n_kv, head_dim, page_size, scale, tabl
     _check_devices(out, Q, cache, table, lens, q_start, work)
     _call("vla_kv4_attention_dev", out.data_ptr(), ldo, Q.data_ptr(), ldq, cache.data_ptr(), pages, page_size, table.data_ptr(),
           ld, lens.data_ptr(), _dp(q_start), n, total, max_new, ld * page_size if max_len is None else max_len, n_q, n_kv,
-          head_dim, scale, dt, wp, wb, _stream(stream))
+          head_dim, float(scale), dt, wp, wb, _stream(stream))
 
 
 class LinearI8:

@@ -68,56 +68,66 @@ struct Job {
 
 __device__ __forceinline__ int clamp_row(int x, int total) { return x < 0 ? 0 : (x < total ? x : total); }
 
-// The block's tile number -> its job; false when there are fewer tiles. Starts
-// are read clamped to the buffers' rows, a sequence that would end before it
-// begins as empty, so that no offsets can lead out of the buffers. Every wave does the same
-// search, 64 sequences at a time; tiles are counted from the last one of the
-// last sequence, as queries late in a sequence see the most keys under a causal mask. (Counted by
-// their depth over all sequences, the deepest first, 12 mixed prompts took 224 us for 212: the
-// search is longer, and neighbours no longer share keys.)
+// The block's tile number -> its job; false for a number without a tile. Up to 64 sequences: tiles are
+// counted, a sequence to a lane. More: sequence s has the numbers from q_start[s] / QT + s on, of
+// which the next sequence's leave it at least as many as it has tiles, so that there is no sum over
+// the sequences, only a search among increasing numbers, 64 at a time. (For few sequences the
+// numbers without a tile cost more than the sum, as their blocks hold places when others are
+// dealt: 8 sequences of 177, 15 heads of 64, 9.9 us for 8.8. For many the sum
+// grows with their number in every block: 70 of 100 tokens, 32 heads of 128, 63.7 us for 59.5, 1000 of 30
+// 1118 for 432, 8000 of 16 42.5 ms for 3.4.)
+// Numbers run backwards, as queries late in a sequence see the most keys under a causal mask.
+// (Counted by their depth over all sequences, the deepest first, 12 mixed prompts took 224 us for
+// 212: neighbours no longer share keys.) Starts are read clamped to the buffers' rows, and a
+// sequence that would end before it begins is empty, so that no offsets can lead out of the buffers.
+// Every wave does the same search.
 template <int QT>
 __device__ __forceinline__ bool find_job(const PackedAttnArgs& a, int tile, Job& job) {
     const int lane = threadIdx.x & 63;
-    int q0 = 0, n = 0, k0 = 0, nk = 0, tiles = 0, incl = 0;  // of the lane's sequence; tiles up to it
-    auto load = [&](int base) {
-        const int s = base + lane;
-        q0 = n = k0 = nk = 0;
-        if (s < a.n_seqs) {
-            q0 = clamp_row(a.q_start[s], a.total_q);
-            n = clamp_row(a.q_start[s + 1], a.total_q) - q0;
-            k0 = clamp_row(a.k_start[s], a.total_k);
-            nk = clamp_row(a.k_start[s + 1], a.total_k) - k0;
-            n = n < 0 ? 0 : n;
-            nk = nk < 0 ? 0 : nk;
-        }
-        incl = tiles = (n + QT - 1) / QT;
+    int want = (int)(gridDim.x / a.n_q) - 1 - tile;
+    int lo = 0, count = a.n_seqs;  // the sequence is one of [lo, lo + count)
+    while (count > 64) {
+        const int step = (count + 63) / 64, s = lo + lane * step;
+        const bool in = lane * step < count && clamp_row(a.q_start[s], a.total_q) / QT + s <= want;
+        const int k = __popcll(__ballot(in));
+        const int first = lo + (k ? k - 1 : 0) * step;
+        count = count - (first - lo) < step ? count - (first - lo) : step;
+        lo = first;
+    }
+    const int s = lo + lane;
+    int q0 = 0, n = 0, k0 = 0, nk = 0;  // of the lane's sequence
+    if (lane < count) {
+        q0 = clamp_row(a.q_start[s], a.total_q);
+        n = clamp_row(a.q_start[s + 1], a.total_q) - q0;
+        k0 = clamp_row(a.k_start[s], a.total_k);
+        nk = clamp_row(a.k_start[s + 1], a.total_k) - k0;
+    }
+    int number = q0 / QT + s;  // of its first tile
+    if (a.n_seqs <= 64) {
+        const int tiles = n > 0 ? (n + QT - 1) / QT : 0;
+        int incl = tiles;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const int o = __shfl_up(incl, d);
             if (lane >= d) incl += o;
         }
-        return __builtin_amdgcn_readlane(incl, 63);
-    };
-    int total = load(0);
-    if (a.n_seqs > 64)
-        for (int base = 64; base < a.n_seqs; base += 64) total += load(base);
-    int want = total - 1 - tile;
-    if (want < 0) return false;
-    if (a.n_seqs > 64) {
-        for (int base = 0;; base += 64) {
-            const int sum = load(base);
-            if (want < sum) break;
-            want -= sum;
-        }
+        number = incl - tiles;
+        want = __builtin_amdgcn_readlane(incl, 63) - 1 - tile;
     }
+    const int found = __popcll(__ballot(lane < count && number <= want));
+    if (!found) return false;
     // the same in every lane: kept in scalar registers
-    const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(incl > want)) - 1);
-    job.at = (want - (__builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(tiles, l))) * QT;
-    job.q0 = __builtin_amdgcn_readlane(q0, l) + job.at;
+    const int l = __builtin_amdgcn_readfirstlane(found - 1);
+    const int start = __builtin_amdgcn_readlane(q0, l);
     job.len_q = __builtin_amdgcn_readlane(n, l);
+    const int64_t at = (int64_t)(want - __builtin_amdgcn_readlane(number, l)) * QT;
+    if (at < 0 || at >= job.len_q) return false;  // (below 0: starts out of order)
+    job.at = (int)at;
+    job.q0 = start + job.at;
     job.nq = job.len_q - job.at < QT ? job.len_q - job.at : QT;
     job.k0 = __builtin_amdgcn_readlane(k0, l);
     job.nk = __builtin_amdgcn_readlane(nk, l);
+    if (job.nk < 0) job.nk = 0;
     return true;
 }
 
@@ -928,8 +938,8 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
     }
 }
 
-// the most tiles of qt queries that n_seqs sequences of total_q rows can have
-int64_t max_tiles(const PackedAttnArgs& a, int qt) { return a.total_q / qt + (a.n_seqs < a.total_q ? a.n_seqs : a.total_q); }
+// tile numbers of find_job: the most tiles that n_seqs sequences of total_q rows can have
+int64_t max_tiles(const PackedAttnArgs& a, int qt) { return a.total_q / qt + (int64_t)a.n_seqs; }
 
 template <class F>
 void launch_tiles(F* kernel, const PackedAttnArgs& a, int qt, int threads, int lds, hipStream_t st) {

@@ -82,11 +82,13 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeHeadsArgs a, int 
             }
         }
         if (w) {
-            float sum = 0.0f;
+            // (in double: squares of fp32 and bf16 values leave fp32's range)
+            double sum = 0.0;
 #pragma unroll
-            for (int v = 0; v < VEC; v++) sum += lo[v] * lo[v] + hi[v] * hi[v];
+            for (int v = 0; v < VEC; v++) sum += (double)lo[v] * lo[v] + (double)hi[v] * hi[v];
             for (int m = 1; m < lp; m <<= 1) sum += __shfl_xor(sum, m);
-            const float r = 1.0f / sqrtf(sum / (float)a.head_dim + a.eps);
+            const double mean = sum / a.head_dim + a.eps;
+            const float r = mean > 1e-30 && mean < 1e30 ? 1.0f / sqrtf((float)mean) : (float)(1.0 / sqrt(mean));
             if (on) {
 #pragma unroll
                 for (int v = 0; v < VEC; v++) {
