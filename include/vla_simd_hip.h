@@ -410,9 +410,12 @@ VLA_API int32_t vla_dense_linear_dev(float* out, int32_t ldo, const float* x, in
  *
  * Sequences are packed: rows start[s] .. start[s + 1] - 1 belong to sequence s, with
  * start [n_seqs + 1] int32 on the device, ascending from 0. Rows behind
- * start[n_seqs] are neither read nor written. The host does not see the offsets,
+ * start[n_seqs] are not written and change nothing. At most 2^28 rows and sequences
+ * (2^26 tokens of vla_qk_norm_rope_dev). The host does not see the offsets,
  * lengths and page tables; kernels clamp them to the sizes given here, so that wrong
- * ones give wrong values but never an access outside the buffers. */
+ * ones give wrong values but never an access outside the buffers. Outputs overlap
+ * nothing that the call reads, but where that is said. A query with a NaN gives NaN,
+ * one with an infinity no defined values. */
 typedef enum { VLA_F32 = 0, VLA_BF16 = 1, VLA_F16 = 2 } vla_dtype;
 
 /* Per token and head, x / sqrt(mean(x^2) + eps) * weight (weight [head_dim] fp32,
@@ -420,9 +423,9 @@ typedef enum { VLA_F32 = 0, VLA_BF16 = 1, VLA_F16 = 2 } vla_dtype;
  * angle pos[axis of i][token] * base^(-2 i / head_dim). sections (host, [n_axes]) gives
  * how many of the head_dim / 2 pairs each axis has, in their order: one axis is
  * vla_rope_neox_dev's rotation, three (time, height, width) serve images and video.
- * pos: n_axes rows of seq int32 at stride ld_pos (device). q_out and k_out may be q
- * and k themselves, else they overlap nothing that is read. n_q or n_kv may be 0.
- * head_dim a multiple of 8 up to 256, n_axes up to 8. */
+ * pos: n_axes rows of seq int32 at stride ld_pos
+ * (device). q_out and k_out may be q and k themselves, else they overlap nothing that is
+ * read. n_q or n_kv may be 0. head_dim a multiple of 8 up to 256, n_axes up to 8. */
 VLA_API int32_t vla_qk_norm_rope_dev(void* q_out, int64_t ldqo, void* k_out, int64_t ldko,
                                      const void* q, int64_t ldq, const void* k, int64_t ldk,
                                      const float* q_weight, const float* k_weight, float eps,

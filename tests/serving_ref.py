@@ -26,9 +26,9 @@ def rounding(ref, dtype):
 def rope(x, heads, hd, pos, sections, base, w, eps):
     """(out, bound): norms per head and rotation, x [T, heads * hd].
 
-    Bound: the norm's sum of hd squares in fp32, at most 8 + 6 + 2 steps per lane and 6 over lanes,
-    would be off by 22 u (it is held in 64 bits), its root by half that and 4 u for mean, eps, root and
-    reciprocal; two more products make 17 u on y. Sine and cosine: the fraction of a turn rounded to fp32 moves the
+    Bound: the norm's sum of hd squares in at most 8 + 6 + 2 steps per lane and 6 over lanes
+    is off by 22 u, its root by half that and 4 u for mean, eps, root and reciprocal; two more
+    products make 17 u on y. Sine and cosine: the fraction of a turn rounded to fp32 moves the
     angle by at most pi u, the functions add 2 units in the last place (4 u), together 8 u. Product
     and sum add 2 u: 27 u of |y_i| + |y_(i + half)|."""
     T, h = x.shape[0], hd // 2

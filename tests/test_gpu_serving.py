@@ -88,7 +88,7 @@ def test_rope_far_positions(vla):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("size", [1e25, 1e-25])
+@pytest.mark.parametrize("size", [1e25, 1e-25, 1e-38, 1e37])
 def test_norm_beyond_the_range_of_squares(vla, dtype, size):
     """Values whose squares overflow or vanish in 32 bits are normed all the same."""
     x = (_rows(_gen(6), 5, 2 * 64, F32) * size).to(dtype)
@@ -497,9 +497,24 @@ def test_decode_bad_pages(vla):
         got = _run_decode(vla, q, cache, t, lens, new, 4, 2, 64, 32, 0.125, True).cpu()
         assert bool(got[0].isnan().all())
         ref.within(got[1:], want[1:], bound[1:])
-    # a length beyond the table is cut to it
-    got = _run_decode(vla, q, cache, table, [96 + 500, 40, 70], new, 4, 2, 64, 32, 0.125, True).cpu()
-    ref.within(got[1:], want[1:], bound[1:])
+    # a length beyond the table's pages names tokens without a page
+    room = table.shape[1] * 32
+    for n in (room + 1, room + 32, room + 500, 2 ** 31 - 1):
+        for split in (True, False):
+            got = _run_decode(vla, q, cache, table, [n, 40, 70], new, 4, 2, 64, 32, 0.125, split).cpu()
+            assert bool(got[0].isnan().all()), n
+            ref.within(got[1:], want[1:], bound[1:])
+
+
+def test_decode_chunk_across_the_tables_end(vla):
+    """Of a chunk of new tokens, those that the table has room for are right, the others NaN."""
+    lens, new = [96], [40]
+    q, cache, table, ks, vs = _decode_case(vla, lens, new, 4, 2, 64, 32, BF16, seed=15)
+    want, bound = ref.decode(q, ks, vs, new, 4, 2, 64, 0.125)
+    q2 = torch.cat([q[10:], q[:10]])  # rows 0..29 stand where rows 10..39 of the whole chunk stood
+    got = _run_decode(vla, q2, cache, table, [96 + 10], new, 4, 2, 64, 32, 0.125, True).cpu()
+    ref.within(got[:30], want[10:], bound[10:])
+    assert bool(got[30:].isnan().all())
 
 
 def test_decode_long_cache(vla):

@@ -38,7 +38,7 @@ def _rope(vla, **kw):
 
 
 @pytest.mark.parametrize("kw,msg", [
-    (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(seq=-1), "seq"), (dict(n_q=0, n_kv=0), "heads"),
+    (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(seq=-1), "seq"), (dict(seq=1 << 26), "2^26"), (dict(n_q=0, n_kv=0), "heads"),
     (dict(hd=0, sections=[0]), "head_dim"), (dict(hd=12, sections=[6]), "head_dim"), (dict(hd=264, sections=[132]), "head_dim"),
     (dict(sections=[31]), "sections"), (dict(sections=[16, 17]), "sections"), (dict(sections=[]), "axes"), (dict(sections=[4] * 9), "axes"),
     (dict(sections=[33, -1]), "section"), (dict(base=0.0), "base"), (dict(base=float("nan")), "base"), (dict(eps=-1.0), "eps"),
@@ -61,7 +61,9 @@ def _packed(vla, **kw):
     (dict(hd=4), "head_dim"), (dict(hd=264), "head_dim"), (dict(hd=0), "head_dim"), (dict(scale=float("inf")), "scale"),
     (dict(scale=float("nan")), "scale"), (dict(out=None), "null"), (dict(qs=None, ks=None), "null"), (dict(v=None), "null"),
     (dict(q=P + 2), "aligned"), (dict(ldk=65), "aligned"), (dict(ldo=120), "stride"), (dict(ldv=56), "stride"),
-    (dict(tq=2 ** 31 - 1, n=1, n_q=512, ldq=512 * 64, ldo=512 * 64), "too many"),
+    (dict(tq=2 ** 31 - 1), "2^28"), (dict(tk=2 ** 28 + 1), "2^28"), (dict(n=2 ** 30), "2^28"), (dict(ldk=1 << 22), "2^22"),
+    (dict(n_q=1 << 26, tq=1, n=1), "65536"),
+    (dict(tq=2 ** 28, n=1, n_q=512, ldq=512 * 64, ldo=512 * 64), "too many"),
 ])
 def test_packed_refusals(vla, kw, msg):
     assert msg in _packed(vla, **kw)
@@ -86,7 +88,7 @@ def _kv(vla, name, **kw):
     (dict(dtype=3), "dtype"), (dict(n=-1), "n_seqs"), (dict(n_kv=0), "kv heads"), (dict(hd=48), "head_dim"), (dict(hd=160), "head_dim"),
     (dict(page=0), "page_size"), (dict(page=48), "page_size"), (dict(page=4096), "page_size"), (dict(ld=2 ** 30), "2^30"),
     (dict(pages=-1), "2^30"), (dict(pages=0), "hold a page"), (dict(cache=None), "hold a page"), (dict(cache=P + 8), "aligned"),
-    (dict(table=None), "table"), (dict(ld=0), "table"),
+    (dict(table=None), "table"), (dict(ld=0), "table"), (dict(total=2 ** 31 - 1), "2^28"), (dict(n=2 ** 28 + 1), "2^28"),
 ])
 def test_cache_refusals(vla, name, kw, msg):
     assert msg in _kv(vla, name, **kw)
@@ -98,7 +100,7 @@ def test_cache_refusals(vla, name, kw, msg):
     ("attention", dict(n_q=5), "multiple"), ("attention", dict(scale=float("nan")), "scale"), ("attention", dict(max_new=0), "max_new"),
     ("attention", dict(max_len=-1), "max_len"), ("attention", dict(start=None, total=1), "one query row"), ("attention", dict(lens=None), "lens"),
     ("attention", dict(out=None), "null"), ("attention", dict(ldq=252), "stride"), ("attention", dict(q=P + 2), "aligned"),
-    ("attention", dict(n=70000, total=70000), "65535"),
+    ("attention", dict(n=70000, total=70000), "65535"), ("attention", dict(n_q=1 << 26), "65536"),
 ])
 def test_cache_call_refusals(vla, name, kw, msg):
     assert msg in _kv(vla, name, **kw)

@@ -745,6 +745,9 @@ def _import_torch():
     _torch = torch
 
 
+_MAX_I32 = 2 ** 31 - 1
+
+
 def _type_id(t):
     """The vla_dtype of a tensor's rows."""
     if _torch is None:
@@ -757,7 +760,7 @@ def _type_id(t):
 
 def _row_ld(name, t, rows, width, dtype):
     """The row stride of a [rows, width] tensor whose rows are contiguous and do not overlap."""
-    if t.dtype is not dtype or t.shape != (rows, width):
+    if t.dtype is not dtype or t.shape != (rows, width) or rows > _MAX_I32:
         raise ValueError(f"{name}: need [{rows}, {width}] of {dtype}, got {list(t.shape)} of {t.dtype}")
     ld, step = t.stride()
     if rows <= 1:
@@ -775,7 +778,7 @@ def _check_ints(name, t, n):
 def _seqs_of(name, t):
     """The number of sequences of an offsets tensor [n_seqs + 1]."""
     n = t.shape[0] if t.dim() == 1 else 0
-    if n < 1:
+    if not 1 <= n <= _MAX_I32:
         raise ValueError(f"{name}: need [n_seqs + 1] offsets, got {list(t.shape)}")
     _check_ints(name, t, n)
     return n - 1
@@ -853,7 +856,7 @@ def _cache_shape(cache, n_kv, head_dim, page_size, table):
     cs, ts = cache.shape, table.shape
     if cache.dtype is not _torch.uint8 or len(cs) != 2 or cs[1] != nb or not cache.is_contiguous():
         raise ValueError(f"cache: need contiguous [n_pages, {nb}] uint8, got {list(cs)} of {cache.dtype}")
-    if table.dtype is not _INT32 or len(ts) != 2 or not table.is_contiguous():
+    if table.dtype is not _INT32 or len(ts) != 2 or not table.is_contiguous() or max(ts) > _MAX_I32:
         raise ValueError(f"table: need contiguous [n_seqs, pages] int32, got {list(ts)} of {table.dtype}")
     return cs[0], ts[0], ts[1]
 

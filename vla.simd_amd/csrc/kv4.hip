@@ -348,12 +348,13 @@ struct Kv4Tile {
     }
 };
 
-// tiles of a sequence: at least one, whose block writes the zeros of an empty one
+// Tiles of a sequence: at least one, whose block writes the zeros of an empty one. Of a length
+// beyond the table the first tile behind it is among them and makes NaN of the rows that see it.
 __device__ __forceinline__ int seq_tiles(const Kv4Args& a, int cached, int& len) {
-    const int64_t cap = (int64_t)a.ld_table * a.page_size;
-    len = cached;
-    len = len < 0 ? 0 : ((int64_t)len > cap ? (int)cap : len);
-    return len > 0 ? (len + kTile - 1) / kTile : 1;
+    len = cached < 0 ? 0 : cached;
+    const int all = a.ld_table * (a.page_size / kTile) + 1;
+    const int tiles = len / kTile + (len % kTile != 0);
+    return tiles > all ? all : tiles > 0 ? tiles : 1;
 }
 
 // Where the run of tiles [run * per, (run + 1) * per) begins: sequence `seq`, whose first tile
@@ -765,7 +766,7 @@ size_t plan_bytes(const Kv4Run& r, int total_q, int n_q, int head_dim) {
 Kv4Run plan(int n_seqs, int max_new, int64_t max_len, int n_q, int n_kv, int head_dim) {
     Kv4Run r{};
     r.tok_tiles = row_tiles(max_new, n_q, n_kv, &r.head_tiles);
-    const int64_t most = ((int64_t)1 << 24) / ((int64_t)n_kv * r.head_tiles);  // (a block loops over the rest)
+    const int64_t most = ((int64_t)1 << 23) / ((int64_t)n_kv * r.head_tiles);  // (a launch has less than 2^32 threads; a block loops over the rest)
     if (r.tok_tiles > most) r.tok_tiles = (int)(most < 1 ? 1 : most);
     const int64_t heads = (int64_t)n_kv * r.head_tiles * r.tok_tiles;
     const int64_t card = attn_waves(head_dim) == 4 ? 512 : 1024;
@@ -810,6 +811,7 @@ void check_cache(const Kv4Args& a, const char* who) {
     const std::string w(who);
     VLA_REQUIRE(dtype_ok(a.dtype), w + ": dtype must be VLA_F32, VLA_BF16 or VLA_F16");
     VLA_REQUIRE(a.n_seqs >= 0 && a.total >= 0 && a.n_kv > 0 && a.n_kv <= 1024, w + ": need n_seqs, rows >= 0 and 1 to 1024 kv heads");
+    VLA_REQUIRE(a.n_seqs <= 1 << 28 && a.total <= 1 << 28, w + ": at most 2^28 sequences and rows");
     VLA_REQUIRE(head_dim_ok(a.head_dim), w + ": head_dim must be 32, 64, 96, 128, 192 or 256");
     VLA_REQUIRE(a.page_size > 0 && a.page_size % kTile == 0 && a.page_size <= kKv4MaxPage,
                 w + ": page_size must be a multiple of 32 in [32, 2048]");
@@ -877,7 +879,7 @@ size_t kv4_attention_work_bytes(int total_q, int n_seqs, int max_new, int max_le
 
 void launch_kv4_attention(const Kv4Args& a, hipStream_t st) {
     check_cache(a, "kv4_attention");
-    VLA_REQUIRE(a.n_q > 0 && a.n_q % a.n_kv == 0, "kv4_attention: n_q must be a multiple of n_kv");
+    VLA_REQUIRE(a.n_q > 0 && a.n_q <= 65536 && a.n_q % a.n_kv == 0, "kv4_attention: n_q must be a multiple of n_kv up to 65536");
     VLA_REQUIRE(std::isfinite(a.scale), "kv4_attention: scale must be finite");
     VLA_REQUIRE(a.max_new >= 0 && a.max_len >= 0, "kv4_attention: max_new and max_len must not be negative");
     VLA_REQUIRE(a.start || a.total >= a.n_seqs, "kv4_attention: without q_start every sequence has one query row");
@@ -894,8 +896,9 @@ void launch_kv4_attention(const Kv4Args& a, hipStream_t st) {
     VLA_REQUIRE((int64_t)a.total * a.n_q < (int64_t)1 << 31, "kv4_attention: too many query rows times heads");
     Kv4Run r = plan(a.n_seqs, a.max_new, a.max_len, a.n_q, a.n_kv, a.head_dim);
     // (the tiles of all sequences are counted in 32 bits)
-    const bool counts = (int64_t)a.n_seqs * ((int64_t)a.ld_table * a.page_size / kTile + 1) < (int64_t)1 << 30;
-    if (!counts || !a.work || !aligned(a.work, 16) || a.work_bytes < plan_bytes(r, a.total, a.n_q, a.head_dim)) r.runs = 0;
+    const bool counts = (int64_t)a.n_seqs * ((int64_t)a.ld_table * a.page_size / kTile + 2) < (int64_t)1 << 30;
+    const bool joins = (int64_t)a.total * a.n_q < (int64_t)1 << 24;  // blocks of 256 threads
+    if (!counts || !joins || !a.work || !aligned(a.work, 16) || a.work_bytes < plan_bytes(r, a.total, a.n_q, a.head_dim)) r.runs = 0;
     if (r.runs) {
         r.info = reinterpret_cast<int4*>(a.work);
         r.ml = reinterpret_cast<float*>(reinterpret_cast<char*>(a.work) + info_bytes(a.total));

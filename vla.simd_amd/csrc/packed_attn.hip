@@ -946,7 +946,7 @@ void launch_tiles(F* kernel, const PackedAttnArgs& a, int qt, int threads, int l
     if (lds > 65536)
         VLA_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     const int64_t blocks = max_tiles(a, qt) * a.n_q;
-    VLA_REQUIRE(blocks < (int64_t)1 << 31, "packed_attention: too many rows times heads for one call");
+    VLA_REQUIRE(blocks * threads < (int64_t)1 << 32, "packed_attention: too many rows times heads for one call");
     kernel<<<(unsigned)blocks, threads, lds, st>>>(a);
     VLA_LAUNCH_CHECK();
 }
@@ -1004,7 +1004,9 @@ void launch_packed_attention(const PackedAttnArgs& a, hipStream_t st) {
     VLA_REQUIRE(dtype_ok(a.dtype), "packed_attention: dtype must be VLA_F32, VLA_BF16 or VLA_F16");
     VLA_REQUIRE(a.n_seqs >= 0 && a.total_q >= 0 && a.total_k >= 0 && a.n_q > 0 && a.n_kv > 0,
                 "packed_attention: need n_seqs, total_q, total_k >= 0, n_q > 0, n_kv > 0");
-    VLA_REQUIRE(a.n_q % a.n_kv == 0, "packed_attention: n_q must be a multiple of n_kv");
+    VLA_REQUIRE(a.n_seqs <= 1 << 28 && a.total_q <= 1 << 28 && a.total_k <= 1 << 28,
+                "packed_attention: at most 2^28 sequences and rows");
+    VLA_REQUIRE(a.n_q <= 65536 && a.n_q % a.n_kv == 0, "packed_attention: n_q must be a multiple of n_kv up to 65536");
     VLA_REQUIRE(a.head_dim > 0 && a.head_dim <= 256 && a.head_dim % 8 == 0,
                 "packed_attention: head_dim must be a multiple of 8 in [8, 256]");
     VLA_REQUIRE(std::isfinite(a.scale), "packed_attention: scale must be finite");

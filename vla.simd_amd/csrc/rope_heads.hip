@@ -82,18 +82,29 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeHeadsArgs a, int 
             }
         }
         if (w) {
-            // (in double: squares of fp32 and bf16 values leave fp32's range)
-            double sum = 0.0;
+            float sum = 0.0f;
 #pragma unroll
-            for (int v = 0; v < VEC; v++) sum += (double)lo[v] * lo[v] + (double)hi[v] * hi[v];
+            for (int v = 0; v < VEC; v++) sum += lo[v] * lo[v] + hi[v] * hi[v];
             for (int m = 1; m < lp; m <<= 1) sum += __shfl_xor(sum, m);
-            const double mean = sum / a.head_dim + a.eps;
-            const float r = mean > 1e-30 && mean < 1e30 ? 1.0f / sqrtf((float)mean) : (float)(1.0 / sqrt(mean));
+            const float mean = sum / (float)a.head_dim + a.eps;
+            if (mean > 1e-30f && mean < 1e30f) {
+                const float r = 1.0f / sqrtf(mean);
+#pragma unroll
+                for (int v = 0; v < VEC; v++) lo[v] *= r, hi[v] *= r;
+            } else {  // the squares leave fp32's range, or are about to (all in double: 142 us for 127)
+                double wide = 0.0;
+#pragma unroll
+                for (int v = 0; v < VEC; v++) wide += (double)lo[v] * lo[v] + (double)hi[v] * hi[v];
+                for (int m = 1; m < lp; m <<= 1) wide += __shfl_xor(wide, m);
+                const double r = 1.0 / sqrt(wide / a.head_dim + a.eps);
+#pragma unroll
+                for (int v = 0; v < VEC; v++) lo[v] = (float)(lo[v] * r), hi[v] = (float)(hi[v] * r);
+            }
             if (on) {
 #pragma unroll
                 for (int v = 0; v < VEC; v++) {
-                    lo[v] *= r * w[i0 + v];
-                    hi[v] *= r * w[half + i0 + v];
+                    lo[v] *= w[i0 + v];
+                    hi[v] *= w[half + i0 + v];
                 }
             }
         }
@@ -115,7 +126,7 @@ template <class T, int VEC>
 void run_rope(const RopeHeadsArgs& a, hipStream_t st) {
     int lp = 1;
     while (lp * VEC < a.head_dim / 2) lp <<= 1;
-    qk_norm_rope_kernel<T, VEC><<<(a.seq + a.tokens_per_block - 1) / a.tokens_per_block, 256, 0, st>>>(a, lp);
+    qk_norm_rope_kernel<T, VEC><<<(unsigned)(((int64_t)a.seq + a.tokens_per_block - 1) / a.tokens_per_block), 256, 0, st>>>(a, lp);
     VLA_LAUNCH_CHECK();
 }
 
@@ -123,6 +134,7 @@ void run_rope(const RopeHeadsArgs& a, hipStream_t st) {
 
 void launch_qk_norm_rope(RopeHeadsArgs a, hipStream_t st) {
     VLA_REQUIRE(dtype_ok(a.dtype), "qk_norm_rope: dtype must be VLA_F32, VLA_BF16 or VLA_F16");
+    VLA_REQUIRE(a.seq < 1 << 26, "qk_norm_rope: seq must be below 2^26");  // a launch has less than 2^32 threads
     VLA_REQUIRE(a.seq >= 0 && a.n_q >= 0 && a.n_kv >= 0 && a.n_q + a.n_kv > 0 && a.n_q <= 4096 && a.n_kv <= 4096,
                 "qk_norm_rope: need seq >= 0 and heads");
     VLA_REQUIRE(a.head_dim >= 8 && a.head_dim <= 2 * kMaxHalf && a.head_dim % 8 == 0,
