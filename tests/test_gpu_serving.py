@@ -486,6 +486,111 @@ def test_decode_not_finite(vla, dtype, hd):
             ref.within(tail[:, :, :hd - 32], w, b, "other blocks")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("max_new", [33, 4])
+@pytest.mark.parametrize("n_q,n_kv,hd,page", [(15, 5, 64, 64), (8, 1, 128, 32), (40, 2, 32, 96), (2, 2, 256, 64), (4, 2, 192, 128)])
+def test_decode_chunks_in_runs(vla, dtype, max_new, n_q, n_kv, hd, page):
+    """Chunks, empty sequences and queries without a key where runs of tiles cut the sequences anywhere;
+    chunks past max_new are not cut."""
+    lens, new = [227, 33, 2, 0, 1100, 0, 64], [17, 33, 5, 0, 1, 3, 4]
+    q, cache, table, ks, vs = _decode_case(vla, lens, new, n_q, n_kv, hd, page, dtype, seed=hd + 3)
+    assert vla.kv4_attention_work_bytes(sum(new) + 2, 7, max_new, 4096, n_q, n_kv, hd) > 0
+    want, bound = ref.decode(q, ks, vs, new, n_q, n_kv, hd, hd ** -0.5)
+    for m in (1500, 4096, 1 << 20):
+        got = _run_decode(vla, q, cache, table, lens, new, n_q, n_kv, hd, page, hd ** -0.5, True, max_len=m, max_new=max_new)
+        ref.within(got, want, bound, f"max_len {m}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [32, 96, 256])
+def test_decode_not_finite_in_runs(vla, dtype, hd):
+    """The same as without runs: a NaN reaches the queries that see it, whatever block takes its tile."""
+    lens, new, page = [70, 40], [9, 1], 64
+    q, cache, table, ks, vs = _decode_case(vla, lens, new, 4, 2, hd, page, dtype, seed=5)
+    want, bound = ref.decode(q, ks, vs, new, 4, 2, hd, hd ** -0.5)
+    row = table.cpu().numpy()[0]
+    for part in (2, 3):
+        c = cache.clone()
+        c.view(-1)[vla.kv4_offset(row, 2, hd, page, cache.shape[0], 65, part, 1, hd // 32 - 1)] = 255
+        got = _run_decode(vla, q, c, table, lens, new, 4, 2, hd, page, hd ** -0.5, True, max_len=4096).cpu()
+        ref.within(got[:4], want[:4], bound[:4], "before")
+        ref.within(got[4:, :2 * hd], want[4:, :2 * hd], bound[4:, :2 * hd], "other kv head")
+        ref.within(got[9:], want[9:], bound[9:], "other sequence")
+        tail = got[4:9, 2 * hd:].reshape(5, 2, hd)
+        assert bool(tail[:, :, hd - 32:].isnan().all())
+        if part == 3 and hd > 32:
+            w, b = (x[4:9, 2 * hd:].reshape(5, 2, hd)[:, :, :hd - 32] for x in (want, bound))
+            ref.within(tail[:, :, :hd - 32], w, b, "other blocks")
+
+
+def test_decode_many_sequences(vla):
+    """As many sequences as one call takes, all reading the same page."""
+    n = 65535
+    q, cache, _, ks, vs = _decode_case(vla, [20], [1], 1, 1, 32, 32, BF16, seed=4)
+    table = torch.zeros(n, 1, dtype=torch.int32, device=DEV)
+    table[:] = int((cache[:, 0] != 0xFF).nonzero()[0])
+    lens = torch.arange(n, dtype=torch.int32, device=DEV) % 21
+    qd = q.to(DEV).repeat(n, 1)
+    out = torch.empty_like(qd)
+    for max_len in (32, 2048):
+        work = torch.full((max(16, vla.kv4_attention_work_bytes(n, n, 1, max_len, 1, 1, 32)),), 0xFF, dtype=torch.uint8, device=DEV)
+        out.fill_(5.0)
+        vla.kv4_attention_dev(out, qd, cache, 1, 1, 32, 32, 0.2, table, lens, max_len=max_len, work=work)
+        for m in range(21):
+            rows = out[m::21].cpu()
+            want, bound = ref.decode(q, [ks[0][:m]], [vs[0][:m]], [1], 1, 1, 32, 0.2)
+            ref.within(rows, want.expand_as(rows), bound.expand_as(rows), f"{m} keys")
+
+
+def test_shared_pages(vla):
+    """Two sequences with the same first pages: each appends to pages of its own and reads both."""
+    n_kv, hd, page, dtype = 2, 64, 32, BF16
+    g = _gen(81)
+    k, v = _rows(g, 64 + 20, n_kv * hd, dtype), _rows(g, 64 + 20, n_kv * hd, dtype)
+    cache = torch.full((5, vla.kv4_page_bytes(n_kv, hd, page)), 0xFF, dtype=torch.uint8, device=DEV)
+    table = torch.tensor([[3, 1, 0], [3, 1, 4]], dtype=torch.int32, device=DEV)
+    vla.kv4_append_dev(cache, k[:64].to(DEV), v[:64].to(DEV), n_kv, hd, page, table[:1].contiguous(), _i32([64]), _i32([0, 64]))
+    vla.kv4_append_dev(cache, k[64:].to(DEV), v[64:].to(DEV), n_kv, hd, page, table, _i32([76, 72]), _i32([0, 12, 20]))
+    own = [torch.cat([torch.arange(64), torch.arange(a, b)]) for a, b in ((64, 76), (76, 84))]
+    ks, vs = ([ref.values(*ref.quantize(x[i].reshape(-1, n_kv, hd))) for i in own] for x in (k, v))
+    q = _rows(g, 5, 4 * hd, dtype)
+    want, bound = ref.decode(q, ks, vs, [2, 3], 4, n_kv, hd, 0.125)
+    for m in (76, 2048):
+        ref.within(_run_decode(vla, q, cache, table, [76, 72], [2, 3], 4, n_kv, hd, page, 0.125, True, max_len=m), want, bound)
+
+
+def test_two_streams_at_once(vla):
+    """The same operators on two streams, each with its own workspace, against one after the other."""
+    n_q, n_kv, hd, page = 8, 2, 64, 32
+    jobs = []
+    for i, lens in enumerate(([3000, 40, 900], [77, 2500, 1])):
+        q, cache, table, _, _ = _decode_case(vla, lens, [1] * 3, n_q, n_kv, hd, page, BF16, seed=90 + i)
+        x = _rows(_gen(i), 700, n_q * hd, BF16).to(DEV)
+        work = torch.empty(vla.kv4_attention_work_bytes(3, 3, 1, 4096, n_q, n_kv, hd), dtype=torch.uint8, device=DEV)
+        jobs.append((q.to(DEV), cache, table, _i32(lens), x, x[:, :n_kv * hd].contiguous(), _i32([0, 300 + i, 700]), work))
+
+    def run(job):
+        q, cache, table, lens, x, kv, start, work = job
+        o, p, r = torch.empty_like(q), torch.empty_like(x), torch.empty_like(x)
+        pos = torch.arange(700, dtype=torch.int32, device=DEV)[None]
+        for _ in range(5):
+            vla.kv4_attention_dev(o, q, cache, n_q, n_kv, hd, page, 0.125, table, lens, max_len=4096, work=work)
+            vla.qk_norm_rope_dev(r, None, x, None, n_q, 0, hd, pos, [32], 1e4)
+            vla.packed_attention_dev(p, r, kv, kv, n_q, n_kv, hd, 0.125, start)
+        return o, p, r
+
+    alone = [run(j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    both = []
+    for st, j in zip(streams, jobs):
+        with torch.cuda.stream(st):
+            both.append(run(j))
+    torch.cuda.synchronize()
+    for a, b in zip(alone, both):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_decode_bad_pages(vla):
     """A sequence whose table names no page where it needs one reads NaN, the others are untouched."""
     lens, new = [70, 40, 70], [1, 1, 1]
