@@ -637,6 +637,40 @@ def test_decode_long_cache(vla):
     ref.within(_run_decode(vla, q, cache, table, [700], [1], 16, n_kv, hd, page, hd ** -0.5, True), want, bound)
 
 
+@pytest.mark.parametrize("dtype,hd", [(BF16, 64), (F32, 64), (F32, 256)])
+def test_rows_far_apart(vla, dtype, hd):
+    """Rows of one buffer whose offsets pass 32 bits, through every operator that takes rows."""
+    T, ld = 1100, (1 << 22) // (2 if dtype is F32 else 1)
+    if dtype is BF16:
+        ld //= 2
+    buf = torch.empty(T, ld, dtype=dtype, device=DEV)
+    assert buf.numel() * buf.element_size() > 1 << 32
+    g = _gen(12)
+    x = [_rows(g, T, n * hd, dtype) for n in (2, 1, 1)]
+    q, k, v, out, kb, vb = (buf[:, at * hd:(at + n) * hd] for at, n in ((0, 2), (2, 1), (3, 1), (4, 2), (6, 1), (7, 1)))
+    for d, s in zip((q, k, v), x):
+        d.copy_(s)
+    lens = [1000, 100]
+    s = _starts(lens)
+    vla.packed_attention_dev(out, q, k, v, 2, 1, hd, 0.125, _i32(s))
+    want, bound = ref.packed(*x, s, s, 2, 1, hd, 0.125, True)
+    ref.within(out, want, bound, "attention")
+    pos = torch.arange(T, dtype=torch.int32)[None]
+    vla.qk_norm_rope_dev(q, k, q, k, 2, 1, hd, pos.to(DEV), [hd // 2], 1e4)
+    for got, y, n in ((q, x[0], 2), (k, x[1], 1)):
+        want, bound = ref.rope(y, n, hd, pos, [hd // 2], 1e4, None, 0.0)
+        ref.within(got, want, bound, "rotation")
+    cache = torch.zeros(35, vla.kv4_page_bytes(1, hd, 32), dtype=torch.uint8, device=DEV)
+    table = torch.arange(35, dtype=torch.int32, device=DEV)[None].contiguous()
+    vla.kv4_append_dev(cache, v, v, 1, hd, 32, table, _i32([T]), _i32([0, T]))
+    vla.kv4_gather_dev(kb, vb, cache, 1, hd, 32, table, _i32([0, T]))
+    want = ref.values(*ref.quantize(x[2].reshape(T, 1, hd))).reshape(T, hd).to(dtype)
+    assert torch.equal(kb.cpu(), want) and torch.equal(vb.cpu(), want)
+    vla.kv4_attention_dev(out[:1], q[:1], cache, 2, 1, hd, 32, 0.125, table, _i32([T]))
+    vla.kv4_attention_dev(out[-2:-1], q[:1], cache, 2, 1, hd, 32, 0.125, table, _i32([T]))
+    assert torch.equal(out[:1], out[-2:-1])
+
+
 # --------------------------------------------------------- run together --
 
 def _decoder_pass(vla, bufs, steps):
