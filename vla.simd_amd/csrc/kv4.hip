@@ -294,7 +294,7 @@ struct Kv4Tile {
         const unsigned pn = page_no(run, tile), slot = (tile - pn * run.per_page) * kTile;
         const int page = uniform_page(table, a.ld_table, a.n_pages, pn);
         there = page >= 0;
-        const uint8_t* pg = a.cache + (size_t)(there ? page : 0) * (2 * (nc + ns));  // not there: read, and not used
+        const uint8_t* pg = a.cache + (size_t)__builtin_amdgcn_readfirstlane(there ? page : 0) * (2 * (nc + ns));  // not there: read, and not used
         const uint8_t* kc = pg + ((size_t)kvh * a.page_size + slot) * (HD / 2);
         const uint8_t* vc = kc + nc;
         const uint8_t* ks = pg + 2 * nc + (size_t)kvh * NB * a.page_size + slot;
@@ -454,7 +454,6 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attn_kernel(Kv4Args a, Kv4Run r
         const int tn = n - t0 < toks ? n - t0 : toks;
         const int tok = t0 + c / heads, hh = ht * 16 + c % heads;  // this lane's row
         const bool rok = c < heads * tn && hh < group;
-        const int head = kvh * group + hh;
         const int lim = rok ? (len - n + tok + 1 > 0 ? len - n + tok + 1 : 0) : 0;
         const int lim_lo = len - n + t0 + 1, lim_hi = len - n + t0 + tn;  // of the tile's rows
         const int k_begin = t_begin * kTile;
@@ -463,33 +462,42 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attn_kernel(Kv4Args a, Kv4Run r
 
         const int k_first = k_begin + wave * kTile;
         Kv4Tile<NB> ta;
-        if (k_first < k_end) ta.load(a, run, table, kvh, c, g, (unsigned)k_first / kTile);
+        // (a load behind the last tile reads the first again: always as many loads, so that waits can
+        // count them)
+        auto load = [&](Kv4Tile<NB>& t, int k) { t.load(a, run, table, kvh, c, g, k < k_end ? (unsigned)k / kTile : 0u); };
+        load(ta, k_first);
 
+        // (rows without a query read the first one's and take zeros, by a mask that the compiler
+        // cannot make a branch of: around the loads it would wait for each by itself)
         U4 qv[PQ][NB];
+        constexpr int QL = 8 * (int)sizeof(T) / 16;  // loads of 8 values
+        typedef Pack<T, 16 / (int)sizeof(T)> QPack;
+        QPack qx[NB][QL];
+        const T* qrow = static_cast<const T*>(a.Q) + (size_t)(q0 + (rok ? tok : t0)) * a.ldq + (kvh * group + (rok ? hh : ht * 16)) * HD;
+        unsigned keep = rok ? ~0u : 0u;
+        asm volatile("" : "+v"(keep));
         each_load<NL>([&]<int u>() {
             constexpr int VB = G::vb(u), BS = G::bs(u);
 #pragma unroll
-            for (int i = 0; i < VB; i++) {
-                float x[8] = {};
-                if (rok) {
-                    const T* src = static_cast<const T*>(a.Q) + (size_t)(q0 + tok) * a.ldq + head * HD + BS * 32 + g * 8 * VB + 8 * i;
+            for (int i = 0; i < VB; i++)
 #pragma unroll
-                    for (int j = 0; j < 8; j += 16 / (int)sizeof(T)) {
-                        const auto z = *reinterpret_cast<const Pack<T, 16 / sizeof(T)>*>(src + j);
-#pragma unroll
-                        for (int e = 0; e < 16 / (int)sizeof(T); e++) x[j + e] = to_f32(z.v[e]);
-                    }
-                }
-#pragma unroll
-                for (int p = 0; p < PQ; p++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        qv[p][BS + i].u[j] = pack_upper(x[2 * j], x[2 * j + 1]);
-                        x[2 * j] -= upper_part(x[2 * j]);
-                        x[2 * j + 1] -= upper_part(x[2 * j + 1]);
-                    }
-            }
+                for (int j = 0; j < QL; j++)
+                    qx[BS + i][j] = *reinterpret_cast<const QPack*>(qrow + BS * 32 + g * 8 * VB + 8 * i + j * (8 / QL));
         });
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = __uint_as_float(__float_as_uint(to_f32(qx[b][e / (8 / QL)].v[e % (8 / QL)])) & keep);
+#pragma unroll
+            for (int q = 0; q < PQ; q++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    qv[q][b].u[j] = pack_upper(x[2 * j], x[2 * j + 1]);
+                    x[2 * j] -= upper_part(x[2 * j]);
+                    x[2 * j + 1] -= upper_part(x[2 * j + 1]);
+                }
+        }
 
         v4f o[NT] = {};
         float m = -INFINITY, l = 0.0f;  // the reference of the weights, in log2, and their sum
@@ -577,17 +585,18 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attn_kernel(Kv4Args a, Kv4Run r
         };
         if constexpr (NB <= 4) {  // two tiles in turn: one is loaded while the other is worked on
             Kv4Tile<NB> tb;
-            for (int k0 = k_first; k0 < k_end; k0 += 2 * W * kTile) {
-                const int k1 = k0 + W * kTile, k2 = k1 + W * kTile;
-                if (k1 < k_end) tb.load(a, run, table, kvh, c, g, (unsigned)k1 / kTile);
+            for (int k0 = k_first; k0 < k_end;) {
+                const int k1 = k0 + W * kTile;
+                load(tb, k1);
                 step(ta, k0);
                 if (k1 >= k_end) break;
-                if (k2 < k_end) ta.load(a, run, table, kvh, c, g, (unsigned)k2 / kTile);
+                k0 = k1 + W * kTile;
+                load(ta, k0);
                 step(tb, k1);
             }
         } else {  // (registers for one)
             for (int k0 = k_first; k0 < k_end; k0 += W * kTile) {
-                if (k0 != k_first) ta.load(a, run, table, kvh, c, g, (unsigned)k0 / kTile);
+                if (k0 != k_first) load(ta, k0);
                 step(ta, k0);
             }
         }
