@@ -494,7 +494,7 @@ def test_decode_chunks_in_runs(vla, dtype, max_new, n_q, n_kv, hd, page):
     chunks past max_new are not cut."""
     lens, new = [227, 33, 2, 0, 1100, 0, 64], [17, 33, 5, 0, 1, 3, 4]
     q, cache, table, ks, vs = _decode_case(vla, lens, new, n_q, n_kv, hd, page, dtype, seed=hd + 3)
-    assert vla.kv4_attention_work_bytes(sum(new) + 2, 7, max_new, 4096, n_q, n_kv, hd) > 0
+    assert vla.kv4_attention_work_bytes(sum(new) + 2, 7, max_new, 1 << 20, n_q, n_kv, hd) > 0
     want, bound = ref.decode(q, ks, vs, new, n_q, n_kv, hd, hd ** -0.5)
     for m in (1500, 4096, 1 << 20):
         got = _run_decode(vla, q, cache, table, lens, new, n_q, n_kv, hd, page, hd ** -0.5, True, max_len=m, max_new=max_new)

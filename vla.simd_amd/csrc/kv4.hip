@@ -763,15 +763,17 @@ size_t plan_bytes(const Kv4Run& r, int total_q, int n_q, int head_dim) {
 }
 
 // How a call runs, from sizes the host knows. Equal runs of tiles (and a second kernel) or a
-// block per sequence: the latter costs 6 us and 5.9 us for every 1000 keys of the longest
-// sequence (32 heads on 8 of 128), the former 12 us and what the bytes take. Measured, us, runs |
-// sequences: 1 x 1000 keys 12.0 | 11.9, 1 x 2000 13.4 | 18.0, 16 x 500 12.5 | 9.2, 64 mixed up to
-// 1000 24.1 | 14.8, 48 mixed up to 8192 45 | 74; with more blocks than the card holds at once a
-// run has pieces of several sequences, each with its own beginning and end: 128 mixed up to
-// 2000 48 | 37, and only a sequence much longer than the others is worth them.
+// block per sequence: the latter costs 5 us and 0.7 us for every step of its waves (5.7 us for 1000
+// keys, heads of 128) until its blocks take the card's bandwidth among them; the former 12 us and
+// what the bytes take, more where runs are cut into pieces of several sequences. Measured, us,
+// runs | sequences (32 heads on 8 of 128): 1 x 1000 keys 11.6 | 11.3, 1 x 2000 13.1 | 17.2, 4 x 1500
+// 15.6 | 14.6, 4 x 2000 13.4 | 17.5, 16 x 2000 21.8 | 18.4, 16 x 4000 27.1 | 30.6, 64 mixed up to 2000
+// 34.9 | 21.5, 48 mixed up to 8192 42.6 | 67.5; where the sequences' blocks fill the card only
+// one much longer than the others is worth runs: 64 mixed up to 4000 37.8 | 35.3, 64 of 8192 108 | 104, 64
+// mixed up to 16384 95 | 118.
 // Runs: as many blocks as the card holds at once (two waves on a SIMD: 512 of 4 waves;
-// 768 and 1024 of them took 55 and 53 us for the 48), each with at least 8 tiles, two rounds
-// of its waves (4: one sequence of 8192 13.2 us for 12.4; 16: 14.0).
+// 768 and 1024 of them took 40.5 and 46 us for the 48, 118 and 115 for the 64 of 8192), each with at
+// least 8 tiles, two rounds of its waves (4: 1 x 2000 11.8 us, but 4 x 2000 16.9; 16: 14.4).
 Kv4Run plan(int n_seqs, int max_new, int64_t max_len, int n_q, int n_kv, int head_dim) {
     Kv4Run r{};
     r.tok_tiles = row_tiles(max_new, n_q, n_kv, &r.head_tiles);
@@ -779,7 +781,8 @@ Kv4Run plan(int n_seqs, int max_new, int64_t max_len, int n_q, int n_kv, int hea
     if (r.tok_tiles > most) r.tok_tiles = (int)(most < 1 ? 1 : most);
     const int64_t heads = (int64_t)n_kv * r.head_tiles * r.tok_tiles;
     const int64_t card = attn_waves(head_dim) == 4 ? 512 : 1024;
-    if (max_len <= 1024 || (heads * n_seqs >= 2 * card && max_len <= 8192)) return r;
+    const int64_t steps = max_len / (kTile * attn_waves(head_dim)), blocks = heads * n_seqs;
+    if (steps <= 64 && steps * (card - blocks) <= 12 * card) return r;
     const int64_t tiles = (max_len + kTile - 1) / kTile * n_seqs;
     int64_t runs = (card + heads - 1) / heads;
     runs = runs < tiles / 8 ? runs : tiles / 8;
