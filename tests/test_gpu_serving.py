@@ -166,6 +166,31 @@ def test_packed_heads_and_strides(vla, dtype, n_q, n_kv, hd, pad):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,n_q,n_kv,hd", [([700], 2, 1, 64), ([520, 1], 2, 2, 128), ([600], 1, 1, 40), ([300, 259], 28, 7, 64),
+                                              ([290, 270], 28, 4, 128)])
+def test_packed_keys_shared_by_waves(vla, dtype, causal, lens, n_q, n_kv, hd):
+    """Few blocks over some keys: waves that share queries are joined, values taken out of the product
+    come back in the queries that see them, whichever waves had their tile."""
+    g = _gen(hd + n_q)
+    q, k, v = _packed_case(g, lens, lens, n_q, n_kv, hd, dtype)
+    args = (_starts(lens), _starts(lens), n_q, n_kv, hd, hd ** -0.5, causal)
+    want, bound = ref.packed(q, k, v, *args, base=torch.full_like(q, 5.0))
+    ref.within(_run_packed(vla, q, k, v, lens, lens, n_q, n_kv, hd, hd ** -0.5, causal, same=True), want, bound)
+    if not causal:
+        return
+    at = (5, 69, lens[0] - 130, lens[0] - 2)
+    for j, bad in zip(at, (math.inf, math.nan, -math.inf, math.nan)):
+        v[j, 3] = bad
+    got = _run_packed(vla, q, k, v, lens, lens, n_q, n_kv, hd, hd ** -0.5, causal, same=True).cpu()
+    cols = [h * hd + 3 for h in range(n_q // n_kv)]  # of the first kv head's queries
+    hit = torch.zeros(got.shape, dtype=torch.bool)
+    hit[at[0]:lens[0], cols] = True
+    ref.within(got[~hit], want[~hit], bound[~hit], "others")
+    assert bool((got[at[0]:at[1], cols] == math.inf).all()) and bool(got[at[1]:lens[0], cols].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_packed_many_sequences(vla, dtype):
     """More sequences than lanes in the tile search, and single queries over long keys."""
     for n, long in ((150, 0), (65, 130), (4200, 0)):

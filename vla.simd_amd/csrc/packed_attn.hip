@@ -181,14 +181,15 @@ struct Rows {
 constexpr unsigned kNoRow = 0x80000000u;  // an offset behind every row
 
 // HC: columns worked on, head_dim rounded up (zeros behind it); HDP: those of an LDS row, a
-// power of two. SPLIT 2: waves 4 to 7 take every other tile of keys for the same
-// queries, joined at the end.
-template <class T, int HDP, int HC, int KT, int SPLIT>
-__global__ __launch_bounds__(256 * SPLIT, HDP <= 128 ? 2 : 1) void packed_attn_16(PackedAttnArgs a) {
+// power of two. QW: waves of 32 queries each. SPLIT 2: as many waves again take every other tile
+// of keys for the same queries, joined at the end.
+template <class T, int HDP, int HC, int KT, int SPLIT, int QW>
+__global__ __launch_bounds__(64 * QW * SPLIT, HDP == 64 || HDP == 128 && QW == 4 ? 2 : 1) void packed_attn_16(PackedAttnArgs a) {
     typedef typename Vec8<T>::type v8;
-    constexpr int QT = 128, NK = KT / 32;
+    constexpr int QT = 32 * QW, NK = KT / 32;
+    constexpr int NTH = 64 * QW;            // threads that share a tile of keys
     constexpr int CH = HDP / 8;             // chunks of a row
-    constexpr int LOADS = KT * CH / 256;    // chunks per thread of a K or V tile
+    constexpr int LOADS = KT * CH / NTH;    // chunks per thread of a K or V tile
     constexpr int DT = HC / 32, KS = HC / 16;
     constexpr int TILE = KT * HDP;
     constexpr unsigned kExp = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;  // exponent bits: all set where not finite
@@ -199,8 +200,8 @@ __global__ __launch_bounds__(256 * SPLIT, HDP <= 128 ? 2 : 1) void packed_attn_1
     Job job;
     if (!find_job<QT>(a, tile, job)) return;
 
-    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int part = SPLIT == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int tid = threadIdx.x % NTH, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int part = SPLIT == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NTH);
     const int n = lane & 31, hf = lane >> 5;
     const int hd = a.head_dim;
     const int kvh = __builtin_amdgcn_readfirstlane(head / (a.n_q / a.n_kv));
@@ -241,7 +242,7 @@ __global__ __launch_bounds__(256 * SPLIT, HDP <= 128 ? 2 : 1) void packed_attn_1
     unsigned ko[LOADS], vo[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
-        const int e = tid + 256 * i, row = e / CH, d = ((e % CH) ^ swz<HDP>(row)) * 8;
+        const int e = tid + NTH * i, row = e / CH, d = ((e % CH) ^ swz<HDP>(row)) * 8;
         const bool in = d < hd;  // behind head_dim: behind every row, zeros
         ko[i] = in ? (unsigned)(row * (int)a.ldk + d) * (int)sizeof(T) : kNoRow;
         vo[i] = in ? (unsigned)(row * (int)a.ldv + d) * (int)sizeof(T) : kNoRow;
@@ -254,8 +255,8 @@ __global__ __launch_bounds__(256 * SPLIT, HDP <= 128 ? 2 : 1) void packed_attn_1
         const Rows kt(Kg + (size_t)t * KT * a.ldk, kb), vt(Vg + (size_t)t * KT * a.ldv, vb);  // (no rows: nothing is read)
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
-            kt.to_lds(kd + part * TILE + (256 * i + wave * 64) * 8, ko[i]);
-            vt.to_lds(vd + part * TILE + (256 * i + wave * 64) * 8, vo[i]);
+            kt.to_lds(kd + part * TILE + (NTH * i + wave * 64) * 8, ko[i]);
+            vt.to_lds(vd + part * TILE + (NTH * i + wave * 64) * 8, vo[i]);
         }
     };
     v16f o[DT] = {};
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(256 * SPLIT, HDP <= 128 ? 2 : 1) void packed_attn_1
             int bad = 0;
 #pragma unroll 1
             for (int i = 0; i < LOADS; i++) {
-                const uint4 w = *reinterpret_cast<const uint4*>(Vt + (tid + 256 * i) * 8);
+                const uint4 w = *reinterpret_cast<const uint4*>(Vt + (tid + NTH * i) * 8);
                 const unsigned u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                 for (int x = 0; x < 4; x++) bad |= (u[x] & kExp) == kExp || (u[x] >> 16 & kExp) == kExp;
@@ -281,7 +282,7 @@ __global__ __launch_bounds__(256 * SPLIT, HDP <= 128 ? 2 : 1) void packed_attn_1
                 cleaned = cleaned < k0 - part * KT ? cleaned : k0 - part * KT;
                 unsigned short* w = reinterpret_cast<unsigned short*>(Vt);
 #pragma unroll 1
-                for (int e = tid; e < TILE; e += 256)
+                for (int e = tid; e < TILE; e += NTH)
                     if ((w[e] & kExp) == kExp) w[e] = 0;
                 __syncthreads();
             }
@@ -382,9 +383,9 @@ __global__ __launch_bounds__(256 * SPLIT, HDP <= 128 ? 2 : 1) void packed_attn_1
     if constexpr (SPLIT == 2) {
         // Every wave of the second half leaves its state to the one with its queries, lane by
         // lane: 32 x HC floats, half of what K0 or K1 holds.
-        static_assert(HDP <= 128);
+        static_assert(2 * 32 * HC * sizeof(float) <= sizeof(K0) && QW <= 4);
         float* x = reinterpret_cast<float*>(wave < 2 ? K0 : K1) + (wave & 1) * 32 * HC + lane;
-        __shared__ float ml[4][2][64];
+        __shared__ float ml[QW][2][64];
         if (part == 1) {
 #pragma unroll
             for (int d = 0; d < DT; d++)
@@ -951,19 +952,23 @@ void launch_tiles(F* kernel, const PackedAttnArgs& a, int qt, int threads, int l
     VLA_LAUNCH_CHECK();
 }
 
-template <class T, int HDP, int HC, int KT, int SPLIT>
+template <class T, int HDP, int HC, int KT, int SPLIT, int QW>
 void run_16_split(const PackedAttnArgs& a, hipStream_t st) {
-    launch_tiles(&packed_attn_16<T, HDP, HC, KT, SPLIT>, a, 128, 256 * SPLIT, 0, st);
+    launch_tiles(&packed_attn_16<T, HDP, HC, KT, SPLIT, QW>, a, 32 * QW, 64 * QW * SPLIT, 0, st);
 }
-// Two halves of the keys per block where the blocks would leave CUs idle or alone and the
-// sequences have some length. Measured, us, one half | two: 128 blocks of 512 keys 17.8 | 16.4,
-// 108 of 1024 (no mask, heads of 64) 17.1 | 15.0, 288 of 1024 27.6 | 24.2; the same where a
-// block has but one tile, 32 of 64 keys 8.0 | 10.2, and with more blocks, 324 of 1024 26.9 |
-// 29.4, 1024 of 512 46 | 57, one prompt of 8192 528 | 560.
+// Two halves of the keys per block, and blocks of 64 queries, where blocks of four waves would
+// leave CUs idle or alone and the sequences have some length. Measured, us, four waves with 128
+// queries | two halves | two halves with 64 (blocks of 128 named): 96 blocks of 256 keys 13.6 | 13.4 |
+// 11.4, 160 of 512 18.5 | 17.2 | 14.5, 108 of 1024 (no mask, heads of 64) 17.1 | 15.4 | 12.4, 216 of 1024
+// 18.2 | 16.6 | 16.7, 288 of 1024 (heads of 128) 28.4 | 25.1 | 30.1; one half is ahead where a block has but one tile, 32
+// of 64 keys 8.3 | 10.5 | 9.7, and with more blocks, 324 of 1024 (heads of 64) 26.5 | 29.9 | 26.1, 1280 of 512 46.6 |
+// 59.6 | 85.7, one prompt of 8192 528 | 560.
 template <class T, int HDP, int HC>
 void run_16_hc(const PackedAttnArgs& a, hipStream_t st) {
-    if (max_tiles(a, 128) * a.n_q <= 304 && a.total_k >= (int64_t)256 * a.n_seqs) run_16_split<T, HDP, HC, 64, 2>(a, st);
-    else run_16_split<T, HDP, HC, 64, 1>(a, st);
+    const bool keys = a.total_k >= (int64_t)256 * a.n_seqs;
+    if (keys && max_tiles(a, 64) * a.n_q <= 304) run_16_split<T, HDP, HC, 64, 2, 2>(a, st);
+    else if (keys && max_tiles(a, 128) * a.n_q <= 304) run_16_split<T, HDP, HC, 64, 2, 4>(a, st);
+    else run_16_split<T, HDP, HC, 64, 1, 4>(a, st);
 }
 template <class T>
 void run_16(const PackedAttnArgs& a, hipStream_t st) {
@@ -971,8 +976,8 @@ void run_16(const PackedAttnArgs& a, hipStream_t st) {
     else if (a.head_dim <= 64) run_16_hc<T, 64, 64>(a, st);
     else if (a.head_dim <= 96) run_16_hc<T, 128, 96>(a, st);
     else if (a.head_dim <= 128) run_16_hc<T, 128, 128>(a, st);
-    else if (a.head_dim <= 192) run_16_split<T, 256, 192, 32, 1>(a, st);
-    else run_16_split<T, 256, 256, 32, 1>(a, st);
+    else if (a.head_dim <= 192) run_16_split<T, 256, 192, 32, 1, 4>(a, st);
+    else run_16_split<T, 256, 256, 32, 1, 4>(a, st);
 }
 // Two waves to 32 queries where the blocks of four times 32 would leave CUs idle, four where
 // sequences have some length. Measured, us, one wave | two | four: 75 blocks of 512 keys (heads
