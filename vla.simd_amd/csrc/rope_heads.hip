@@ -8,7 +8,8 @@
 //   out[i + half] = y[i] sin(angle) + y[i + half] cos(angle)
 //
 // HBM bounds it: every value is read and written once, some ten operations
-// each. The angle needs 64 bits (a position of 10^6 leaves 4 bits of an fp32
+// each (32768 tokens of 40 heads of 128 in 125 us, 5.4 TB/s, where a large copy reaches 4.75; one
+// token of 20 heads of 64 in 3.9). The angle needs 64 bits (a position of 10^6 leaves 4 bits of an fp32
 // fraction), the rest 32: the product in double is brought to a fraction of a
 // turn, [-1/2, 1/2], whose fp32 sine and cosine carry fp32 errors whatever the
 // position. That costs a few hundred cycles per (token, pair) and is the same for
