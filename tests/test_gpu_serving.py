@@ -548,6 +548,38 @@ def test_decode_not_finite_in_runs(vla, dtype, hd):
             ref.within(tail[:, :, :hd - 32], w, b, "other blocks")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_packed_without_keys(vla, dtype, hd):
+    """No key rows at all, and no sequences: zeros, and nothing written."""
+    q = torch.ones(5, 2 * hd, dtype=dtype, device=DEV)
+    none = torch.empty(0, hd, dtype=dtype, device=DEV)
+    out = torch.full_like(q, 5.0)
+    vla.packed_attention_dev(out, q, none, none, 2, 1, hd, 0.1, _i32([0, 3, 4]), _i32([0, 0, 0]))
+    assert bool((out[:4] == 0).all()) and bool((out[4] == 5.0).all())
+    out.fill_(5.0)
+    vla.packed_attention_dev(out, q, none, none, 2, 1, hd, 0.1, _i32([0]))
+    vla.packed_attention_dev(none.new_empty(0, 2 * hd), none.new_empty(0, 2 * hd), none, none, 2, 1, hd, 0.1, _i32([0, 0]))
+    assert bool((out == 5.0).all())
+
+
+def test_decode_workspaces_and_rows(vla):
+    """A workspace that is too small or not aligned runs unsplit; without offsets, rows behind the sequences stay."""
+    lens = [3000, 70, 512]
+    q, cache, table, ks, vs = _decode_case(vla, lens, [1] * 3, 4, 2, 64, 64, BF16, seed=19)
+    want, bound = ref.decode(q, ks, vs, [1] * 3, 4, 2, 64, 0.125)
+    qd = torch.cat([q, q]).to(DEV)
+    nb = vla.kv4_attention_work_bytes(6, 3, 1, 3000, 4, 2, 64)
+    assert nb > 0
+    buf = torch.full((nb + 64,), 0xFF, dtype=torch.uint8, device=DEV)
+    for work in (buf, buf[:nb], buf[:nb - 1], buf[8:], buf[:0], None):
+        out = torch.full_like(qd, 5.0)
+        vla.kv4_attention_dev(out, qd, cache, 4, 2, 64, 64, 0.125, table, _i32(lens), max_len=3000, work=work)
+        ref.within(out[:3], want, bound)
+        assert bool((out[3:] == 5.0).all())
+    assert bool((buf[nb:] == 0xFF).all())
+
+
 def test_decode_many_sequences(vla):
     """As many sequences as one call takes, all reading the same page."""
     n = 65535
