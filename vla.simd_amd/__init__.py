@@ -803,10 +803,12 @@ def qk_norm_rope_dev(q_out, k_out, q, k, n_q, n_kv, head_dim, pos, sections, bas
     qp = kp = qop = kop = None
     ldq = ldk = ldqo = ldko = 0
     if n_q:
-        ldqo, ldq = _row_ld("q_out", q_out, T, n_q * head_dim, dtype), _row_ld("q", q, T, n_q * head_dim, dtype)
+        ldq = _row_ld("q", q, T, n_q * head_dim, dtype)
+        ldqo = ldq if q_out is q else _row_ld("q_out", q_out, T, n_q * head_dim, dtype)
         qp, qop = q.data_ptr(), q_out.data_ptr()
     if n_kv:
-        ldko, ldk = _row_ld("k_out", k_out, T, n_kv * head_dim, dtype), _row_ld("k", k, T, n_kv * head_dim, dtype)
+        ldk = _row_ld("k", k, T, n_kv * head_dim, dtype)
+        ldko = ldk if k_out is k else _row_ld("k_out", k_out, T, n_kv * head_dim, dtype)
         kp, kop = k.data_ptr(), k_out.data_ptr()
     if pos.dtype is not _INT32 or pos.shape != (axes, T) or (T > 1 and pos.stride(1) != 1):
         raise ValueError(f"pos: need [{axes}, {T}] int32 with contiguous rows, got {list(pos.shape)} of {pos.dtype}")

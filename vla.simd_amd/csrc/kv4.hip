@@ -776,7 +776,8 @@ size_t plan_bytes(const Kv4Run& r, int total_q, int n_q, int head_dim) {
 // mixed up to 16384 95 | 118.
 // Runs: as many blocks as the card holds at once (two waves on a SIMD: 512 of 4 waves;
 // 768 and 1024 of them took 40.5 and 46 us for the 48, 118 and 115 for the 64 of 8192), each with at
-// least 8 tiles, two rounds of its waves (4: 1 x 2000 11.8 us, but 4 x 2000 16.9; 16: 14.4).
+// least two rounds of its waves, 8 tiles for 4 waves (4: 1 x 2000 11.8 us, but 4 x 2000 16.9; 16: 14.4)
+// and 4 for 2 (heads of 256: 1 x 1000 14.8 us, with 8 tiles 16.6).
 Kv4Run plan(int n_seqs, int max_new, int64_t max_len, int n_q, int n_kv, int head_dim) {
     Kv4Run r{};
     r.tok_tiles = row_tiles(max_new, n_q, n_kv, &r.head_tiles);
@@ -788,7 +789,8 @@ Kv4Run plan(int n_seqs, int max_new, int64_t max_len, int n_q, int n_kv, int hea
     if (steps <= 64 && steps * (card - blocks) <= 12 * card) return r;
     const int64_t tiles = (max_len + kTile - 1) / kTile * n_seqs;
     int64_t runs = (card + heads - 1) / heads;
-    runs = runs < tiles / 8 ? runs : tiles / 8;
+    const int64_t rounds = tiles / (2 * attn_waves(head_dim));
+    runs = runs < rounds ? runs : rounds;
     runs = runs < kMaxPieces ? runs : kMaxPieces;
     r.runs = runs <= 1 && n_seqs == 1 ? 0 : (int)runs;
     r.tok_cap = max_new;
