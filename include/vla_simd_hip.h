@@ -493,7 +493,8 @@ VLA_API int32_t vla_kv4_gather_dev(void* K, int64_t ldk, void* V, int64_t ldv, c
  * when there are few rows, with the partial results in work
  * (vla_kv4_attention_work_bytes of the same numbers, 16-byte aligned; a smaller or
  * null one runs unsplit). Calls that may overlap need a workspace each. Softmax weights
- * enter the product with V to 16 bits (24 for fp32). */
+ * enter the product with V to 16 bits (24 for fp32). At most 65535 sequences and (as in
+ * vla_packed_attention_dev) 65536 query heads. */
 VLA_API int64_t vla_kv4_attention_work_bytes(int32_t total_q, int32_t n_seqs, int32_t max_new,
                                              int32_t max_len, int32_t n_q, int32_t n_kv,
                                              int32_t head_dim);
