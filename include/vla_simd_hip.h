@@ -489,7 +489,7 @@ VLA_API int32_t vla_kv4_gather_dev(void* K, int64_t ldk, void* V, int64_t ldv, c
 /* Attention of the newest tokens over the cache: of the n query rows of sequence s
  * (q_start; NULL: one each, row s), row i sees the keys j < lens[s] - n + i + 1. Rows that
  * see no key get zeros. max_new and max_len are upper bounds of n and lens that choose
- * the launch: too small ones cost time, not values. The key axis is split over blocks
+ * the launch: too small or large ones (any from 1 on) cost time, not values. The key axis is split over blocks
  * when there are few rows, with the partial results in work
  * (vla_kv4_attention_work_bytes of the same numbers, 16-byte aligned; a smaller or
  * null one runs unsplit). Calls that may overlap need a workspace each. Softmax weights

@@ -901,3 +901,14 @@ def test_repeated_calls_give_the_same_bits(vla):
     for _ in range(3):
         assert torch.equal(a, _run_packed(vla, q, k, v, lens, lens, 4, 2, 128, 0.1, True, same=True))
         assert torch.equal(b, _run_decode(vla, dq, cache, table, lens, [1, 1, 1], 4, 2, 64, 64, 0.125, True))
+
+
+@pytest.mark.parametrize("max_len", [64, 4096])
+def test_decode_without_a_bound_on_the_new_tokens(vla, max_len):
+    """2^31 - 1 where the caller knows no bound."""
+    lens, new = [70, 1500, 33], [3, 1, 20]
+    q, cache, table, ks, vs = _decode_case(vla, lens, new, 32, 8, 64, 64, BF16, seed=33)
+    want, bound = ref.decode(q, ks, vs, new, 32, 8, 64, 0.125)
+    for split in (True, False):
+        got = _run_decode(vla, q, cache, table, lens, new, 32, 8, 64, 64, 0.125, split, max_len=max_len, max_new=2 ** 31 - 1)
+        ref.within(got, want, bound)

@@ -227,3 +227,21 @@ def test_work_bytes(vla):
     assert w(1, 1, 1, 4096, 15, 4, 64) == 0         # refused shapes need none
     assert 0 < w(2, 2, 1, 131072, 32, 8, 128) < 1 << 22
     assert w(3, 3, 1, 4096, 32, 8, 128) > w(2, 2, 1, 4096, 32, 8, 128) > 0
+
+
+@pytest.mark.parametrize("total,n,max_len,n_q,n_kv,hd", [(64, 64, 1 << 20, 32, 8, 128), (64, 4, 2 ** 31 - 1, 32, 8, 128), (1, 1, 2 ** 31 - 1, 64, 16, 128),
+                                                         (300, 3, 1 << 17, 40, 2, 32), (7, 2, 1 << 17, 3, 1, 256)])
+def test_any_bound_on_the_new_tokens(vla, total, n, max_len, n_q, n_kv, hd):
+    """No sequence has more new tokens than there are rows: any larger bound plans the same launch."""
+    w = lambda m: vla.kv4_attention_work_bytes(total, n, m, max_len, n_q, n_kv, hd)
+    assert w(total) > 0
+    for m in (total + 1, 1 << 24, 2 ** 31 - 17, 2 ** 31 - 2, 2 ** 31 - 1):
+        assert w(m) == w(total), m
+
+
+def test_work_bytes_of_refused_sizes(vla):
+    """Sizes past what a call takes, or splits, need no workspace, and their products do not wrap."""
+    w, top = vla.kv4_attention_work_bytes, 2 ** 31 - 1
+    for args in ((top, top, top, top, 65536, 1, 256), (1 << 28, 65535, 1 << 28, top, 65536, 1, 256), (8, 70000, 1, 4096, 32, 8, 128), (8, 8, 1, 4096, 32, 8, 160),
+                 (8, 8, 1, 4096, 1 << 20, 8, 128), (8, 8, 1, 4096, 4096, 2048, 128), (1 << 20, 8, 1, 1 << 20, 32, 8, 128)):
+        assert w(*args) == 0, args

@@ -750,11 +750,11 @@ __global__ __launch_bounds__(N) void kv4_join_kernel(Kv4Args a, Kv4Run run) {
     *reinterpret_cast<Pack<T, 4>*>(static_cast<T*>(a.out) + (size_t)tok * a.ldo + head * a.head_dim + ln * 4) = o;
 }
 
-int row_tiles(int max_new, int n_q, int n_kv, int* head_tiles) {
+int64_t row_tiles(int max_new, int n_q, int n_kv, int* head_tiles) {
     const int group = n_q / n_kv;
     *head_tiles = group <= 16 ? 1 : (group + 15) / 16;
     const int toks = group <= 16 ? 16 / group : 1;
-    return (max_new + toks - 1) / toks;
+    return ((int64_t)max_new + toks - 1) / toks;
 }
 
 // waves of a block: the joined waves' rows stay within 64 KiB of LDS
@@ -778,11 +778,13 @@ size_t plan_bytes(const Kv4Run& r, int total_q, int n_q, int head_dim) {
 // 768 and 1024 of them took 40.5 and 46 us for the 48, 118 and 115 for the 64 of 8192), each with at
 // least two rounds of its waves, 8 tiles for 4 waves (4: 1 x 2000 11.8 us, but 4 x 2000 16.9; 16: 14.4)
 // and 4 for 2 (heads of 256: 1 x 1000 14.8 us, with 8 tiles 16.6).
-Kv4Run plan(int n_seqs, int max_new, int64_t max_len, int n_q, int n_kv, int head_dim) {
+// max_new is any bound, 2^31 - 1 where the caller knows none: no sequence has more than all rows.
+Kv4Run plan(int total_q, int n_seqs, int max_new, int64_t max_len, int n_q, int n_kv, int head_dim) {
     Kv4Run r{};
-    r.tok_tiles = row_tiles(max_new, n_q, n_kv, &r.head_tiles);
+    max_new = max_new < total_q ? max_new : total_q;
+    const int64_t tiles_of_rows = row_tiles(max_new, n_q, n_kv, &r.head_tiles);
     const int64_t most = ((int64_t)1 << 23) / ((int64_t)n_kv * r.head_tiles);  // (a launch has less than 2^32 threads; a block loops over the rest)
-    if (r.tok_tiles > most) r.tok_tiles = (int)(most < 1 ? 1 : most);
+    r.tok_tiles = (int)(tiles_of_rows < most ? tiles_of_rows : most);
     const int64_t heads = (int64_t)n_kv * r.head_tiles * r.tok_tiles;
     const int64_t card = attn_waves(head_dim) == 4 ? 512 : 1024;
     const int64_t steps = max_len / (kTile * attn_waves(head_dim)), blocks = heads * n_seqs;
@@ -821,6 +823,10 @@ void run_attn(const Kv4Args& a, const Kv4Run& r, hipStream_t st) {
     else kv4_join_kernel<T, 64><<<a.total * a.n_q, 64, 0, st>>>(a, r);
     VLA_LAUNCH_CHECK();
 }
+
+constexpr int kMaxSeqs = 65535;  // blocks of a launch in y
+// rows times heads that the second kernel has blocks of 256 threads for
+bool joins(int total_q, int n_q) { return (int64_t)total_q * n_q < (int64_t)1 << 24; }
 
 bool head_dim_ok(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 192 || hd == 256; }
 
@@ -891,7 +897,9 @@ void launch_kv4_gather(const Kv4Args& a, hipStream_t st) {
 
 size_t kv4_attention_work_bytes(int total_q, int n_seqs, int max_new, int max_len, int n_q, int n_kv, int head_dim) {
     if (total_q <= 0 || n_seqs <= 0 || max_new <= 0 || max_len <= 0 || n_kv <= 0 || n_q <= 0 || n_q % n_kv || head_dim <= 0) return 0;
-    return plan_bytes(plan(n_seqs, max_new, max_len, n_q, n_kv, head_dim), total_q, n_q, head_dim);
+    // sizes that the call refuses, or that it does not split
+    if (!head_dim_ok(head_dim) || n_kv > 1024 || n_q > 65536 || n_seqs > kMaxSeqs || !joins(total_q, n_q)) return 0;
+    return plan_bytes(plan(total_q, n_seqs, max_new, max_len, n_q, n_kv, head_dim), total_q, n_q, head_dim);
 }
 
 void launch_kv4_attention(const Kv4Args& a, hipStream_t st) {
@@ -902,7 +910,7 @@ void launch_kv4_attention(const Kv4Args& a, hipStream_t st) {
     VLA_REQUIRE(a.start || a.total >= a.n_seqs, "kv4_attention: without q_start every sequence has one query row");
     if (a.n_seqs == 0 || a.total == 0) return;
     VLA_REQUIRE(a.max_new >= 1, "kv4_attention: max_new must be at least 1");
-    VLA_REQUIRE(a.n_seqs <= 65535, "kv4_attention: at most 65535 sequences");
+    VLA_REQUIRE(a.n_seqs <= kMaxSeqs, "kv4_attention: at most 65535 sequences");
     VLA_REQUIRE(a.n_pages > 0 && a.cache && aligned(a.cache, 16), "kv4_attention: the cache must hold a page and be 16-byte aligned");
     VLA_REQUIRE(a.table && a.ld_table > 0 && a.lens, "kv4_attention: page table or lens missing");
     VLA_REQUIRE(a.out && a.Q, "kv4_attention: null buffer");
@@ -911,11 +919,10 @@ void launch_kv4_attention(const Kv4Args& a, hipStream_t st) {
     VLA_REQUIRE(aligned(a.Q, 16) && aligned(a.out, 16) && a.ldq * sz % 16 == 0 && a.ldo * sz % 16 == 0,
                 "kv4_attention: rows must be 16-byte aligned");
     VLA_REQUIRE((int64_t)a.total * a.n_q < (int64_t)1 << 31, "kv4_attention: too many query rows times heads");
-    Kv4Run r = plan(a.n_seqs, a.max_new, a.max_len, a.n_q, a.n_kv, a.head_dim);
+    Kv4Run r = plan(a.total, a.n_seqs, a.max_new, a.max_len, a.n_q, a.n_kv, a.head_dim);
     // (the tiles of all sequences are counted in 32 bits)
     const bool counts = (int64_t)a.n_seqs * ((int64_t)a.ld_table * a.page_size / kTile + 2) < (int64_t)1 << 30;
-    const bool joins = (int64_t)a.total * a.n_q < (int64_t)1 << 24;  // blocks of 256 threads
-    if (!counts || !joins || !a.work || !aligned(a.work, 16) || a.work_bytes < plan_bytes(r, a.total, a.n_q, a.head_dim)) r.runs = 0;
+    if (!counts || !joins(a.total, a.n_q) || !a.work || !aligned(a.work, 16) || a.work_bytes < plan_bytes(r, a.total, a.n_q, a.head_dim)) r.runs = 0;
     if (r.runs) {
         r.info = reinterpret_cast<int4*>(a.work);
         r.ml = reinterpret_cast<float*>(reinterpret_cast<char*>(a.work) + info_bytes(a.total));
