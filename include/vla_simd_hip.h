@@ -440,7 +440,8 @@ VLA_API int32_t vla_qk_norm_rope_dev(void* q_out, int64_t ldqo, void* k_out, int
  * that a query does not see adds nothing to it, infinities and NaN included.
  * k_start NULL: the keys are packed as the queries. total_q and total_k are the
  * buffers' rows. head_dim a multiple of 8 up to 256. In 16-bit types the softmax
- * weights are rounded to that type for the product with V. */
+ * weights are rounded to that type for the product with V (fp16: by half a step, or by 2^-34
+ * of the row's largest weight where that is more). */
 VLA_API int32_t vla_packed_attention_dev(void* out, int64_t ldo, const void* Q, int64_t ldq,
                                          const void* K, int64_t ldk, const void* V, int64_t ldv,
                                          const int32_t* q_start, const int32_t* k_start,

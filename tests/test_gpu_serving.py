@@ -912,3 +912,29 @@ def test_decode_without_a_bound_on_the_new_tokens(vla, max_len):
     for split in (True, False):
         got = _run_decode(vla, q, cache, table, lens, new, 32, 8, 64, 64, 0.125, split, max_len=max_len, max_new=2 ** 31 - 1)
         ref.within(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,n_q,hd", [(8192, 2, 64), (40000, 1, 128), (2048, 320, 32), (4096, 1, 256), (4096, 1, 192)])
+@pytest.mark.parametrize("below,last", [(16, False), (19, False), (22, False), (22, True)])
+def test_packed_sink(vla, dtype, n, n_q, hd, below, last):
+    """One key takes nearly all and its value is zero: the output is what thousands of weights
+    16 to 22 nats below it (2^-23 to 2^-32) add up to."""
+    g = _gen(n + below)
+    q, k = _rows(g, 3, n_q * hd, dtype), _rows(g, n, hd, dtype)
+    v = (1 + 0.1 * torch.randn(n, hd, generator=g)).to(dtype)
+    scale = hd ** -0.5  # the other keys' scores: standard normal
+    sink = n - 1 if last else 0
+    q.view(3, n_q, hd)[:, :, 0] = 8.0
+    k[:, 0] = 0.0
+    k[sink] = 0.0
+    k[sink, 0] = below / (8.0 * scale)
+    v[sink] = 0.0
+    got = _run_packed(vla, q, k, v, [3], [n], n_q, 1, hd, scale, False)
+    want, bound = ref.packed(q, k, v, [0, 3], [0, n], n_q, 1, hd, scale, False)
+    if dtype is F16:
+        # An fp16 below 2^-14 is off by half of its smallest step, 2^-25. The weights stand 2^9 times as large
+        # as relative to a reference that is at most the row's maximum, so their sum is 2^9 at least:
+        # 2^-34 of it for every key.
+        bound = bound + 2.0 ** -34 * n * v.double().abs().max()
+    ref.within(got, want, bound)

@@ -16,8 +16,10 @@
 //                transposed LDS read (ds_read_b64_tr_b16) of row-major V gives.
 //
 // 16-bit types: the weights are rounded to the operands' type for the second product
-// (2^-8 of a weight for bf16, 2^-11 for fp16, each on its own, as large as the
-// rounding of the result); the sum l is of the unrounded ones.
+// (bf16: each by 2^-8 of itself at most; fp16: by 2^-11 of itself or 2^-34 of the row's largest,
+// whichever is more); the sum l is of the unrounded ones. fp16 has few bits below 2^-14, and next to a key
+// that takes nearly all, what is left of the output may be just the small weights: they are all taken 2^9
+// times as large, which cancels in o / l.
 // fp32 up to 128 columns: both products from three bf16 parts of each operand, as exact as
 // fp32 products; past that on the fp32 matrix cores.
 //
@@ -200,6 +202,8 @@ __global__ __launch_bounds__(64 * QW * SPLIT, HDP == 64 || HDP == 128 && QW == 4
     constexpr int DT = HC / 32, KS = HC / 16;
     constexpr int TILE = KT * HDP;
     constexpr unsigned kExp = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;  // exponent bits: all set where not finite
+    // weights are exp2(score - m + kLift): with the reference's lag of 6 at most 2^15 in fp16
+    constexpr float kLift = __is_same(T, bf16_t) ? 0.0f : 9.0f;
     __shared__ __attribute__((aligned(16))) T K0[SPLIT * TILE], K1[SPLIT * TILE], V0[SPLIT * TILE], V1[SPLIT * TILE];
 
     int tile, head;
@@ -338,7 +342,7 @@ __global__ __launch_bounds__(64 * QW * SPLIT, HDP == 64 || HDP == 128 && QW == 4
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] *= alpha;
         }
-        const float mu = m == -INFINITY ? 0.0f : m;
+        const float mu = (m == -INFINITY ? 0.0f : m) - kLift;
         v8 p[NK][2];
 #pragma unroll
         for (int kt = 0; kt < NK; kt++)
