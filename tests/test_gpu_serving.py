@@ -938,3 +938,15 @@ def test_packed_sink(vla, dtype, n, n_q, hd, below, last):
         # 2^-34 of it for every key.
         bound = bound + 2.0 ** -34 * n * v.double().abs().max()
     ref.within(got, want, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_q,n_kv,hd", [(32, 8, 128), (3, 1, 256), (40, 2, 64)])
+def test_decode_a_chunk_among_single_tokens(vla, dtype, n_q, n_kv, hd):
+    """Runs of keys where one sequence has many row tiles and the others one."""
+    lens, new = [70, 900, 33, 513, 2], [1, 1, 70, 23, 1]  # one chunk is longer than its sequence
+    q, cache, table, ks, vs = _decode_case(vla, lens, new, n_q, n_kv, hd, 64, dtype, seed=hd + 1)
+    assert vla.kv4_attention_work_bytes(sum(new) + 2, 5, 70, 20000, n_q, n_kv, hd) > 0
+    want, bound = ref.decode(q, ks, vs, new, n_q, n_kv, hd, hd ** -0.5)
+    for split in (True, False):
+        ref.within(_run_decode(vla, q, cache, table, lens, new, n_q, n_kv, hd, 64, hd ** -0.5, split, max_len=20000), want, bound, f"split {split}")

@@ -245,3 +245,18 @@ def test_work_bytes_of_refused_sizes(vla):
     for args in ((top, top, top, top, 65536, 1, 256), (1 << 28, 65535, 1 << 28, top, 65536, 1, 256), (8, 70000, 1, 4096, 32, 8, 128), (8, 8, 1, 4096, 32, 8, 160),
                  (8, 8, 1, 4096, 1 << 20, 8, 128), (8, 8, 1, 4096, 4096, 2048, 128), (1 << 20, 8, 1, 1 << 20, 32, 8, 128)):
         assert w(*args) == 0, args
+
+
+@pytest.mark.parametrize("n,chunk,max_len", [(48, 256, 16384), (48, 128, 16384), (48, 50, 16384), (8, 50, 65536), (64, 1024, 32768), (2, 700, 1 << 20)])
+def test_runs_for_a_chunk_among_single_tokens(vla, n, chunk, max_len):
+    """The runs of keys are counted by the rows of all sequences: one chunk does not leave the others'
+    single tokens, 8 blocks a run here, to a run or two, one sequence behind the other."""
+    n_q, n_kv, hd, total = 32, 8, 128, chunk + n - 1
+    nb = vla.kv4_attention_work_bytes(total, n, chunk, max_len, n_q, n_kv, hd)
+    if nb == 0:  # a block per sequence
+        return
+    piece = chunk * n_q * (hd + 2) * 4
+    runs, rest = divmod(nb - -(-total * 16 // 256) * 256, piece)
+    assert rest == 0
+    # row tiles of 4 tokens (16 rows of 4 heads); 512 blocks fill the card
+    assert (runs - n) * n_kv * (total / 4 + n) / n >= 512

@@ -778,6 +778,9 @@ size_t plan_bytes(const Kv4Run& r, int total_q, int n_q, int head_dim) {
 // 768 and 1024 of them took 40.5 and 46 us for the 48, 118 and 115 for the 64 of 8192), each with at
 // least two rounds of its waves, 8 tiles for 4 waves (4: 1 x 2000 11.8 us, but 4 x 2000 16.9; 16: 14.4)
 // and 4 for 2 (heads of 256: 1 x 1000 14.8 us, with 8 tiles 16.6).
+// Blocks are counted by the row tiles that there are at most over all sequences, not by max_new in
+// each: one chunk of 128 new tokens among 47 single ones, 48 x 16384 keys, 3527 us with runs for 512 blocks of such
+// chunks, 563 now, 503 without runs (chunks of 50: 972, 262, 232; 8 x 65536, one of 50: 646, 288, 580).
 // max_new is any bound, 2^31 - 1 where the caller knows none: no sequence has more than all rows.
 Kv4Run plan(int total_q, int n_seqs, int max_new, int64_t max_len, int n_q, int n_kv, int head_dim) {
     Kv4Run r{};
@@ -785,16 +788,19 @@ Kv4Run plan(int total_q, int n_seqs, int max_new, int64_t max_len, int n_q, int 
     const int64_t tiles_of_rows = row_tiles(max_new, n_q, n_kv, &r.head_tiles);
     const int64_t most = ((int64_t)1 << 23) / ((int64_t)n_kv * r.head_tiles);  // (a launch has less than 2^32 threads; a block loops over the rest)
     r.tok_tiles = (int)(tiles_of_rows < most ? tiles_of_rows : most);
-    const int64_t heads = (int64_t)n_kv * r.head_tiles * r.tok_tiles;
+    // blocks with work among a block per sequence: of all row tiles, not of max_new in every sequence
+    const int toks = r.head_tiles == 1 ? 16 / (n_q / n_kv) : 1;
+    const int64_t spread = (int64_t)r.tok_tiles * n_seqs, sum = total_q / toks + (int64_t)n_seqs;
+    const int64_t blocks = (int64_t)n_kv * r.head_tiles * (spread < sum ? spread : sum);
     const int64_t card = attn_waves(head_dim) == 4 ? 512 : 1024;
-    const int64_t steps = max_len / (kTile * attn_waves(head_dim)), blocks = heads * n_seqs;
+    const int64_t steps = max_len / (kTile * attn_waves(head_dim));
     if (steps <= 64 && steps * (card - blocks) <= 12 * card) return r;
     const int64_t tiles = (max_len + kTile - 1) / kTile * n_seqs;
-    int64_t runs = (card + heads - 1) / heads;
+    int64_t runs = (card * n_seqs + blocks - 1) / blocks;
     const int64_t rounds = tiles / (2 * attn_waves(head_dim));
     runs = runs < rounds ? runs : rounds;
     runs = runs < kMaxPieces ? runs : kMaxPieces;
-    r.runs = runs <= 1 && n_seqs == 1 ? 0 : (int)runs;
+    r.runs = runs <= 1 ? 0 : (int)runs;
     r.tok_cap = max_new;
     r.slots = r.runs + n_seqs;
     if (plan_bytes(r, 0, n_q, head_dim) > (size_t)1 << 28) r.runs = 0;  // pieces of long chunks
