@@ -459,7 +459,9 @@ VLA_API int32_t vla_packed_attention_dev(void* out, int64_t ldo, const void* Q, 
  * 32 neighbouring values share the scale 2^(byte - 127), with the smallest exponent
  * >= -100 for which the largest magnitude is <= 7 * 2^e; a code is a sign and one of
  * 0, 0.5, 1, 1.5, 2, 3, 4, 6, the nearest, ties to the even code. A block with an
- * infinity or a NaN has byte 255 and reads as NaN. head_dim 32, 64, 96, 128, 192 or 256.
+ * infinity or a NaN has byte 255 and reads as NaN. Reading rounds to the type of the rows, and a value may
+ * round up to the next power of two: magnitudes past 57344 read back into fp16, and those past
+ * 1.75 * 2^127 into any type, are infinite. head_dim 32, 64, 96, 128, 192 or 256.
  * table (device): a row of ld_table page numbers per sequence, tokens in order. A
  * number outside [0, n_pages) or a token behind the table's row names no page: append
  * drops its rows, gather and attention read NaN. Sequences may share pages that
@@ -494,7 +496,9 @@ VLA_API int32_t vla_kv4_gather_dev(void* K, int64_t ldk, void* V, int64_t ldv, c
  * when there are few rows, with the partial results in work
  * (vla_kv4_attention_work_bytes of the same numbers, 16-byte aligned; a smaller or
  * null one runs unsplit). Calls that may overlap need a workspace each. Softmax weights
- * enter the product with V to 16 bits (24 for fp32). At most 65535 sequences and (as in
+ * enter the product with V to 16 bits (24 for fp32). Keys that a row does not see add nothing to it,
+ * whatever they hold; of a block with a magnitude past 1.75 * 2^127 the rows that see it get no defined
+ * values. At most 65535 sequences and (as in
  * vla_packed_attention_dev) 65536 query heads. */
 VLA_API int64_t vla_kv4_attention_work_bytes(int32_t total_q, int32_t n_seqs, int32_t max_new,
                                              int32_t max_len, int32_t n_q, int32_t n_kv,

@@ -950,3 +950,23 @@ def test_decode_a_chunk_among_single_tokens(vla, dtype, n_q, n_kv, hd):
     want, bound = ref.decode(q, ks, vs, new, n_q, n_kv, hd, hd ** -0.5)
     for split in (True, False):
         ref.within(_run_decode(vla, q, cache, table, lens, new, n_q, n_kv, hd, 64, hd ** -0.5, split, max_len=20000), want, bound, f"split {split}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [32, 64, 96, 256])
+@pytest.mark.parametrize("byte,codes", [(253, 0x71), (253, 0x6D), (254, 0xC9), (254, 0x53)])
+def test_decode_values_past_the_range(vla, dtype, hd, byte, codes):
+    """A block with values of 2^128 and more, which 32 bits read as infinities, is nothing to the queries that
+    do not see it."""
+    lens, new, page = [70, 40], [9, 1], 64
+    q, cache, table, ks, vs = _decode_case(vla, lens, new, 4, 2, hd, page, dtype, seed=5)
+    row = table.cpu().numpy()[0]
+    at = lambda part: vla.kv4_offset(row, 2, hd, page, cache.shape[0], 65, part, 1, hd // 32 - 1)
+    cache.view(-1)[at(1):at(1) + 16] = codes  # token 65 of 70: queries 4..8 of 9 see it
+    cache.view(-1)[at(3)] = byte
+    want, bound = ref.decode(q, ks, vs, new, 4, 2, hd, hd ** -0.5)
+    other = torch.ones(want.shape, dtype=torch.bool)
+    other[4:9].view(5, 4, hd)[:, 2:, hd - 32:] = False
+    for split, max_len in ((False, 70), (True, 4096)):
+        got = _run_decode(vla, q, cache, table, lens, new, 4, 2, hd, page, hd ** -0.5, split, max_len=max_len).cpu()
+        ref.within(got[other], want[other], bound[other], f"split {split}")

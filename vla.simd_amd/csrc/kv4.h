@@ -35,6 +35,7 @@ namespace hip {
 constexpr int kKv4Block = 32;
 constexpr int kKv4MinByte = 27;    // e = -100
 constexpr int kKv4NanByte = 255;
+constexpr int kKv4LargeByte = 253; // from here on the largest codes pass fp32's range
 constexpr int kKv4MaxPage = 2048;  // tokens of a page
 
 VLA_HD size_t kv4_code_bytes(int n_kv, int head_dim, int page_size) {

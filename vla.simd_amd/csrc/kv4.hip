@@ -530,11 +530,12 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attn_kernel(Kv4Args a, Kv4Run r
                     if (!t.there) x[i] = NAN;
                     if (kl + i >= lim) x[i] = -INFINITY;
                     // What no row sees is taken out, it may be anything; and so is, of the keys
-                    // that some rows see, what is not finite and must not meet the other rows'
-                    // zero weights: it is put in at the end.
+                    // that some rows see, blocks that may not be finite and must not meet the other rows'
+                    // zero weights: they are put in as NaN at the end. (Code by code, so that the finite
+                    // ones of a block at the end of fp32's range stay: 45 us for 43, 48 mixed up to 8192.)
 #pragma unroll
                     for (int u = 0; u < NL; u++) {
-                        const bool nan = kl + i >= lim_lo && t.vbyte(i, u) == kKv4NanByte;
+                        const bool nan = kl + i >= lim_lo && t.vbyte(i, u) >= kKv4LargeByte;
                         if (nan || kl + i >= k_end) t.hide(i, u);
                         cleaned |= nan;
                     }
@@ -614,7 +615,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attn_kernel(Kv4Args a, Kv4Run r
                     constexpr int VB = G::vb(u), BS = G::bs(u);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const bool nan = vs[(size_t)(BS + (4 * g + r) * VB / 16) * a.page_size] == kKv4NanByte;
+                        const bool nan = vs[(size_t)(BS + (4 * g + r) * VB / 16) * a.page_size] >= kKv4LargeByte;
 #pragma unroll
                         for (int e = 0; e < 2 * VB; e++)
                             if (nan && j < lim) o[2 * BS + e][r] = NAN;
