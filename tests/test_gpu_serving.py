@@ -970,3 +970,35 @@ def test_decode_values_past_the_range(vla, dtype, hd, byte, codes):
     for split, max_len in ((False, 70), (True, 4096)):
         got = _run_decode(vla, q, cache, table, lens, new, 4, 2, hd, page, hd ** -0.5, split, max_len=max_len).cpu()
         ref.within(got[other], want[other], bound[other], f"split {split}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,n_q,hd", [([40, 1, 2], 2, 64), ([700], 1, 128), ([600, 3], 2, 64), ([200, 90], 40, 96), ([150], 2, 136), ([90, 5], 1, 256)])
+def test_packed_large_values(vla, dtype, causal, lens, n_q, hd):
+    """Values at the end of fp32's range: their weighted mean is in range, so it comes out."""
+    g = _gen(hd + sum(lens))
+    q, k, _ = _packed_case(g, lens, lens, n_q, 1, hd, dtype)
+    k[:, 0] += 3.0 * torch.arange(k.shape[0]).remainder(7).to(dtype)  # maxima that grow, slowly and at once
+    v = (torch.rand(k.shape, generator=g) * 1e38 + 2e38).to(dtype)
+    v[:, 1::2] *= -1
+    s = _starts(lens)
+    want, bound = ref.packed(q, k, v, s, s, n_q, 1, hd, hd ** -0.5, causal, base=torch.full_like(q, 5.0))
+    ref.within(_run_packed(vla, q, k, v, lens, lens, n_q, 1, hd, hd ** -0.5, causal, same=True), want, bound)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("hd", [32, 128, 256])
+def test_decode_large_values(vla, dtype, hd):
+    lens, new, page = [70, 900, 40], [9, 1, 1], 64
+    q, cache, table, ks, _ = _decode_case(vla, lens, new, 4, 2, hd, page, F32, seed=5)
+    q = q.to(dtype)
+    g = _gen(hd)
+    k, v = _rows(g, sum(lens), 2 * hd, F32), torch.rand(sum(lens), 2 * hd, generator=g) * 1.9e38 + 1e38
+    v[:, 1::2] *= -1
+    vla.kv4_append_dev(cache, k.to(DEV), v.to(DEV), 2, hd, page, table, _i32(lens), _i32(_starts(lens)))
+    ks, vs = (ref.values(*ref.quantize(x.reshape(-1, 2, hd))).split(lens) for x in (k, v))
+    want, bound = ref.decode(q, ks, vs, new, 4, 2, hd, hd ** -0.5)
+    for split, max_len in ((False, 900), (True, 4096)):
+        got = _run_decode(vla, q, cache, table, lens, new, 4, 2, hd, page, hd ** -0.5, split, max_len=max_len)
+        ref.within(got, want, bound, f"split {split}")

@@ -548,7 +548,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attn_kernel(Kv4Args a, Kv4Run r
             // The reference only has to keep the weights in range: it follows the
             // maximum when a row's has grown by 2^6, so most tiles rescale nothing.
             if (__any(mx > m + 6.0f)) {
-                const float mn = fmaxf(m, mx);
+                const float mn = ceilf(fmaxf(m, mx));
                 const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
                 m = mn;
                 l *= alpha;
@@ -557,7 +557,9 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attn_kernel(Kv4Args a, Kv4Run r
 #pragma unroll
                     for (int r = 0; r < 4; r++) o[t][r] *= alpha;
             }
-            const float mu = m == -INFINITY ? 0.0f : m;
+            // Weights are exp2(score - m - 34), below 2^-28, so that sums over 2^28 keys of weights times any values stay
+            // in fp32's range; m is a whole number, so that this and the factors between references are exact.
+            const float mu = (m == -INFINITY ? 0.0f : m) + 34.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[i] = __builtin_amdgcn_exp2f(x[i] - mu);

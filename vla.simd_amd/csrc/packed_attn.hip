@@ -19,7 +19,7 @@
 // (bf16: each by 2^-8 of itself at most; fp16: by 2^-11 of itself or 2^-34 of the row's largest,
 // whichever is more); the sum l is of the unrounded ones. fp16 has few bits below 2^-14, and next to a key
 // that takes nearly all, what is left of the output may be just the small weights: they are all taken 2^9
-// times as large, which cancels in o / l.
+// times as large (lift, below).
 // fp32 up to 128 columns: both products from three bf16 parts of each operand, as exact as
 // fp32 products; past that on the fp32 matrix cores.
 //
@@ -68,6 +68,16 @@ __device__ __forceinline__ float halves_sum(float x) {
     const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+
+// Weights are exp2(score - m + lift), which cancels in o / l. The reference m only has to keep them in range:
+// it follows the row's maximum when that has grown by 2^6, so most tiles rescale nothing.
+// fp16: weights reach 2^15. bf16: they stay below 2^-28, so that sums over 2^28 keys of weights times values
+// of any size are in fp32's range before they are divided (weights 2^-92 of the largest vanish for
+// that). m - lift is off by 2^-19 at most for scores below 30, between tiles with another m; so are weights of 8 bits.
+// fp32: lift 0, as that would show; the values are taken 2^-34 as large instead, exactly.
+template <class T>
+constexpr float lift() { return __is_same(T, f16_t) ? 9.0f : -34.0f; }
+constexpr float kValueScale = 0x1p-34f;
 
 // What a block works on: query rows [q0, q0 + nq) of the packed buffers, at
 // offset `at` in their sequence, and its keys [k0, k0 + nk).
@@ -202,8 +212,6 @@ __global__ __launch_bounds__(64 * QW * SPLIT, HDP == 64 || HDP == 128 && QW == 4
     constexpr int DT = HC / 32, KS = HC / 16;
     constexpr int TILE = KT * HDP;
     constexpr unsigned kExp = __is_same(T, bf16_t) ? 0x7f80u : 0x7c00u;  // exponent bits: all set where not finite
-    // weights are exp2(score - m + kLift): with the reference's lag of 6 at most 2^15 in fp16
-    constexpr float kLift = __is_same(T, bf16_t) ? 0.0f : 9.0f;
     __shared__ __attribute__((aligned(16))) T K0[SPLIT * TILE], K1[SPLIT * TILE], V0[SPLIT * TILE], V1[SPLIT * TILE];
 
     int tile, head;
@@ -330,8 +338,6 @@ __global__ __launch_bounds__(64 * QW * SPLIT, HDP == 64 || HDP == 128 && QW == 4
 #pragma unroll
             for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[kt][i]);
         mx = halves_max(mx) * c2;
-        // The reference only has to keep the weights in range: it follows the
-        // maximum when a query's has grown by 2^6, so most tiles rescale nothing.
         if (__any(mx > m + 6.0f)) {
             const float mn = fmaxf(m, mx);
             const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
@@ -342,7 +348,7 @@ __global__ __launch_bounds__(64 * QW * SPLIT, HDP == 64 || HDP == 128 && QW == 4
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] *= alpha;
         }
-        const float mu = (m == -INFINITY ? 0.0f : m) - kLift;
+        const float mu = (m == -INFINITY ? 0.0f : m) - lift<T>();
         v8 p[NK][2];
 #pragma unroll
         for (int kt = 0; kt < NK; kt++)
@@ -582,6 +588,8 @@ __global__ __launch_bounds__(parts_threads(KP), KP == 4 || KT * HC <= 4096 && HC
                 for (int x = 0; x < 8; x++)
                     if (!(fabsf(vr[i][x]) < INFINITY)) vr[i][x] = 0.0f;
             }
+#pragma unroll
+            for (int x = 0; x < 8; x++) vr[i][x] *= kValueScale;
             put(Ks, e, kr[i]);
             put(Vs, e, vr[i]);
         }
@@ -754,7 +762,7 @@ __global__ __launch_bounds__(parts_threads(KP), KP == 4 || KT * HC <= 4096 && HC
     }
 
     l = halves_sum(l);
-    const float inv = 1.0f / l;
+    const float inv = (1.0f / kValueScale) / l;
     const Rows orows(static_cast<const float*>(a.out) + (size_t)job.q0 * a.ldo + head * hd, (int64_t)job.nq * a.ldo * 4);
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -839,7 +847,7 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
         for (int i = 0; i < LOADS; i++) {
             const int e = tid + 256 * i, row = e / (HDP / 4), d = 4 * (e % (HDP / 4));
             *reinterpret_cast<float4*>(Ks + row * SK + d) = kr[i];
-            *reinterpret_cast<float4*>(Vs + row * SK + d) = vr[i];
+            *reinterpret_cast<float4*>(Vs + row * SK + d) = make_float4(vr[i].x * kValueScale, vr[i].y * kValueScale, vr[i].z * kValueScale, vr[i].w * kValueScale);
         }
     };
 
@@ -938,7 +946,7 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
     }
 
     l = rows_sum(l);
-    const float inv = 1.0f / l;
+    const float inv = (1.0f / kValueScale) / l;
     if (!qok) return;
     float* dst = static_cast<float*>(a.out) + (size_t)(job.q0 + qi) * a.ldo + head * hd;
 #pragma unroll
