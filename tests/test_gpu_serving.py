@@ -1002,3 +1002,25 @@ def test_decode_large_values(vla, dtype, hd):
     for split, max_len in ((False, 900), (True, 4096)):
         got = _run_decode(vla, q, cache, table, lens, new, 4, 2, hd, page, hd ** -0.5, split, max_len=max_len)
         ref.within(got, want, bound, f"split {split}")
+
+
+def test_decode_many_sequences_without_a_bound(vla):
+    """Not knowing how many new tokens a sequence has costs some time, not a block for every possible one."""
+    n = 20000
+    q, cache, table, ks, vs = _decode_case(vla, [20], [1], 4, 1, 32, 32, BF16, seed=4)
+    table = table.expand(n, 1).contiguous()
+    lens, start = torch.full((n,), 20, dtype=torch.int32, device=DEV), torch.arange(n + 1, dtype=torch.int32, device=DEV)
+    qd = q.to(DEV).repeat(n, 1)
+    out = torch.empty_like(qd)
+    took = []
+    for max_new in (1, 2 ** 31 - 1):
+        for _ in range(2):  # the first call loads the kernel
+            ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            ev[0].record()
+            vla.kv4_attention_dev(out, qd, cache, 4, 1, 32, 32, 0.2, table, lens, start, max_new, 32)
+            ev[1].record()
+            torch.cuda.synchronize()
+        took.append(ev[0].elapsed_time(ev[1]))
+    want, bound = ref.decode(q, ks, vs, [1], 4, 1, 32, 0.2)
+    ref.within(out, want.expand(n, -1), bound.expand(n, -1))
+    assert took[1] < 20 * took[0], took

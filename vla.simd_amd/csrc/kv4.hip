@@ -768,6 +768,13 @@ size_t plan_bytes(const Kv4Run& r, int total_q, int n_q, int head_dim) {
     return r.runs ? info_bytes(total_q) + (size_t)r.slots * r.tok_cap * n_q * (head_dim + 2) * sizeof(float) : 0;
 }
 
+// Blocks with work where each sequence has its own: of all row tiles that there can be, not of as many in every sequence.
+int64_t row_blocks(const Kv4Run& r, int total_q, int n_seqs, int n_q, int n_kv) {
+    const int toks = r.head_tiles == 1 ? 16 / (n_q / n_kv) : 1;
+    const int64_t spread = (int64_t)r.tok_tiles * n_seqs, sum = total_q / toks + (int64_t)n_seqs;
+    return (int64_t)n_kv * r.head_tiles * (spread < sum ? spread : sum);
+}
+
 // How a call runs, from sizes the host knows. Equal runs of tiles (and a second kernel) or a
 // block per sequence: the latter costs 5 us and 0.7 us for every step of its waves (5.7 us for 1000
 // keys, heads of 128) until its blocks take the card's bandwidth among them; the former 12 us and
@@ -791,10 +798,7 @@ Kv4Run plan(int total_q, int n_seqs, int max_new, int64_t max_len, int n_q, int 
     const int64_t tiles_of_rows = row_tiles(max_new, n_q, n_kv, &r.head_tiles);
     const int64_t most = ((int64_t)1 << 23) / ((int64_t)n_kv * r.head_tiles);  // (a launch has less than 2^32 threads; a block loops over the rest)
     r.tok_tiles = (int)(tiles_of_rows < most ? tiles_of_rows : most);
-    // blocks with work among a block per sequence: of all row tiles, not of max_new in every sequence
-    const int toks = r.head_tiles == 1 ? 16 / (n_q / n_kv) : 1;
-    const int64_t spread = (int64_t)r.tok_tiles * n_seqs, sum = total_q / toks + (int64_t)n_seqs;
-    const int64_t blocks = (int64_t)n_kv * r.head_tiles * (spread < sum ? spread : sum);
+    const int64_t blocks = row_blocks(r, total_q, n_seqs, n_q, n_kv);
     const int64_t card = attn_waves(head_dim) == 4 ? 512 : 1024;
     const int64_t steps = max_len / (kTile * attn_waves(head_dim));
     if (steps <= 64 && steps * (card - blocks) <= 12 * card) return r;
@@ -939,6 +943,12 @@ void launch_kv4_attention(const Kv4Args& a, hipStream_t st) {
     }
     r.per_page = a.page_size / kTile;
     r.magic = r.per_page == 1 ? 0 : (unsigned)((((uint64_t)1 << 32) + r.per_page - 1) / r.per_page);
+    // Blocks without a row tile cost 2 to 6 ns of the launch each, so where max_new is far above most sequences' tokens, or
+    // is not known, there are 2^16 blocks or twice as many as can have work; they take several row tiles then. (2000 single tokens
+    // of 64 keys, max_new 2000: 15.1 ms without this, 0.41 now, 0.11 with max_new 1.)
+    const int64_t busy = row_blocks(r, a.total, a.n_seqs, a.n_q, a.n_kv), grid = 2 * busy > 1 << 16 ? 2 * busy : 1 << 16;
+    const int64_t most = grid / ((int64_t)a.n_kv * r.head_tiles * (r.runs ? r.runs : a.n_seqs));
+    if (r.tok_tiles > most) r.tok_tiles = (int)(most < 1 ? 1 : most);
     if (a.dtype == kF32) run_attn<float, 3, 3>(a, r, st);
     else if (a.dtype == kBf16) run_attn<bf16_t, 1, 2>(a, r, st);
     else run_attn<f16_t, 2, 2>(a, r, st);
