@@ -260,3 +260,11 @@ def test_runs_for_a_chunk_among_single_tokens(vla, n, chunk, max_len):
     assert rest == 0
     # row tiles of 4 tokens (16 rows of 4 heads); 512 blocks fill the card
     assert (runs - n) * n_kv * (total / 4 + n) / n >= 512
+
+
+@pytest.mark.parametrize("hd", [160, 224])
+def test_pages_of_refused_head_dims(vla, hd):
+    """No layout for heads that append and attention refuse."""
+    with pytest.raises(ValueError, match="head_dim"):
+        vla.kv4_page_bytes(1, hd, 32)
+    assert vla.kv4_offset([0], 1, hd, 32, 1, 0, 0, 0, 0) == -1

@@ -839,7 +839,7 @@ def kv4_page_bytes(n_kv, head_dim, page_size) -> int:
     """Bytes of a page of the 4-bit cache."""
     n = (_lib or lib()).vla_kv4_page_bytes(n_kv, head_dim, page_size)
     if n < 0:
-        raise ValueError("kv4: head_dim a multiple of 32 up to 256, page_size a multiple of 32 up to 2048")
+        raise ValueError("kv4: 1 to 1024 heads, head_dim 32, 64, 96, 128, 192 or 256, page_size a multiple of 32 up to 2048")
     return n
 
 

@@ -32,8 +32,7 @@ Kv4Args cache_args(void* cache, int32_t n_pages, int32_t page_size, const int32_
 }
 
 bool page_shape_ok(int32_t n_kv, int32_t head_dim, int32_t page_size) {
-    return n_kv > 0 && n_kv <= 1024 && head_dim > 0 && head_dim <= 256 && head_dim % kKv4Block == 0 && page_size > 0 &&
-           page_size % 32 == 0 && page_size <= kKv4MaxPage;
+    return n_kv > 0 && n_kv <= 1024 && kv4_head_dim_ok(head_dim) && page_size > 0 && page_size % 32 == 0 && page_size <= kKv4MaxPage;
 }
 
 }  // namespace

@@ -38,6 +38,8 @@ constexpr int kKv4NanByte = 255;
 constexpr int kKv4LargeByte = 253; // from here on the largest codes pass fp32's range
 constexpr int kKv4MaxPage = 2048;  // tokens of a page
 
+inline bool kv4_head_dim_ok(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 192 || hd == 256; }
+
 VLA_HD size_t kv4_code_bytes(int n_kv, int head_dim, int page_size) {
     return (size_t)n_kv * page_size * (head_dim / 2);
 }

@@ -841,14 +841,12 @@ constexpr int kMaxSeqs = 65535;  // blocks of a launch in y
 // rows times heads that the second kernel has blocks of 256 threads for
 bool joins(int total_q, int n_q) { return (int64_t)total_q * n_q < (int64_t)1 << 24; }
 
-bool head_dim_ok(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 192 || hd == 256; }
-
 void check_cache(const Kv4Args& a, const char* who) {
     const std::string w(who);
     VLA_REQUIRE(dtype_ok(a.dtype), w + ": dtype must be VLA_F32, VLA_BF16 or VLA_F16");
     VLA_REQUIRE(a.n_seqs >= 0 && a.total >= 0 && a.n_kv > 0 && a.n_kv <= 1024, w + ": need n_seqs, rows >= 0 and 1 to 1024 kv heads");
     VLA_REQUIRE(a.n_seqs <= 1 << 28 && a.total <= 1 << 28, w + ": at most 2^28 sequences and rows");
-    VLA_REQUIRE(head_dim_ok(a.head_dim), w + ": head_dim must be 32, 64, 96, 128, 192 or 256");
+    VLA_REQUIRE(kv4_head_dim_ok(a.head_dim), w + ": head_dim must be 32, 64, 96, 128, 192 or 256");
     VLA_REQUIRE(a.page_size > 0 && a.page_size % kTile == 0 && a.page_size <= kKv4MaxPage,
                 w + ": page_size must be a multiple of 32 in [32, 2048]");
     VLA_REQUIRE(a.n_pages >= 0 && a.ld_table >= 0 && (int64_t)a.ld_table * a.page_size <= (int64_t)1 << 30,
@@ -911,7 +909,7 @@ void launch_kv4_gather(const Kv4Args& a, hipStream_t st) {
 size_t kv4_attention_work_bytes(int total_q, int n_seqs, int max_new, int max_len, int n_q, int n_kv, int head_dim) {
     if (total_q <= 0 || n_seqs <= 0 || max_new <= 0 || max_len <= 0 || n_kv <= 0 || n_q <= 0 || n_q % n_kv || head_dim <= 0) return 0;
     // sizes that the call refuses, or that it does not split
-    if (!head_dim_ok(head_dim) || n_kv > 1024 || n_q > 65536 || n_seqs > kMaxSeqs || !joins(total_q, n_q)) return 0;
+    if (!kv4_head_dim_ok(head_dim) || n_kv > 1024 || n_q > 65536 || n_seqs > kMaxSeqs || !joins(total_q, n_q)) return 0;
     return plan_bytes(plan(total_q, n_seqs, max_new, max_len, n_q, n_kv, head_dim), total_q, n_q, head_dim);
 }
 
