@@ -1024,3 +1024,21 @@ def test_decode_many_sequences_without_a_bound(vla):
     want, bound = ref.decode(q, ks, vs, [1], 4, 1, 32, 0.2)
     ref.within(out, want.expand(n, -1), bound.expand(n, -1))
     assert took[1] < 20 * took[0], took
+
+
+def test_rope_small_sines(vla):
+    """Sines and cosines next to zero keep their bits: rows of (1, 0) come out as (cos, sin)."""
+    T, hd = 5000, 128
+    pos = torch.arange(T, dtype=torch.int32)[None]
+    x = torch.zeros(T, hd)
+    x[:, :hd // 2] = 1.0
+    o = torch.empty(T, hd, device=DEV)
+    vla.qk_norm_rope_dev(o, None, x.to(DEV), None, 1, 0, hd, pos.to(DEV), [hd // 2], 100.0)
+    want, _ = ref.rope(x, 1, hd, pos, [hd // 2], 100.0, None, 0.0)
+    small = want.abs() < 0.01
+    assert int(small.sum()) > 1000
+    # The functions are off by 4 units of 2^-23 at most, the turn by the rest and its rounding add 2. The
+    # angle: up to 5000 radians in 64 bits, of a power with some units of error: 2^13 * 2^-53 * 4, in the
+    # reference as well.
+    bound = 6 * 2.0 ** -23 * want.abs() + 2.0 ** -37
+    ref.within(o.cpu()[small], want[small], bound[small])

@@ -11,8 +11,8 @@
 // each (32768 tokens of 40 heads of 128 in 125 us, 5.4 TB/s, where a large copy reaches 4.75; one
 // token of 20 heads of 64 in 3.9). The angle needs 64 bits (a position of 10^6 leaves 4 bits of an fp32
 // fraction), the rest 32: the product in double is brought to a fraction of a
-// turn, [-1/2, 1/2], whose fp32 sine and cosine carry fp32 errors whatever the
-// position. That costs a few hundred cycles per (token, pair) and is the same for
+// turn, [-1/2, 1/2], whose fp32 sine and cosine, turned on by what the fraction's own rounding
+// left out, carry fp32 errors of their size whatever the position. That costs a few hundred cycles per (token, pair) and is the same for
 // every head, so a block first fills a table of its tokens' sines and cosines
 // in LDS and then streams all their heads past it.
 //
@@ -53,9 +53,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeHeadsArgs a, int 
         }
         double r = (double)pos[tt] * turns;
         r -= rint(r);
+        const float f = (float)r, rest = 6.28318530717958648f * (float)(r - f);  // rest: at most 2^-23
         float s, c;
-        sincospif(2.0f * (float)r, &s, &c);
-        cs[idx] = make_float2(c, s);
+        sincospif(2.0f * f, &s, &c);
+        cs[idx] = make_float2(fmaf(-s, rest, c), fmaf(c, rest, s));
     }
     __syncthreads();
 
