@@ -268,3 +268,10 @@ def test_pages_of_refused_head_dims(vla, hd):
     with pytest.raises(ValueError, match="head_dim"):
         vla.kv4_page_bytes(1, hd, 32)
     assert vla.kv4_offset([0], 1, hd, 32, 1, 0, 0, 0, 0) == -1
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 4])
+def test_work_parts_are_aligned(vla, n):
+    """The pieces' values, read 16 bytes at once, lie last in the workspace: a whole number of 16 bytes before them."""
+    nb = vla.kv4_attention_work_bytes(n, n, 1, 1 << 17, 1, 1, 32)
+    assert nb > 0 and nb % 16 == 0

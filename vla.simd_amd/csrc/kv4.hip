@@ -763,9 +763,11 @@ int64_t row_tiles(int max_new, int n_q, int n_kv, int* head_tiles) {
 // waves of a block: the joined waves' rows stay within 64 KiB of LDS
 constexpr int attn_waves(int head_dim) { return head_dim >= 192 ? 2 : 4; }
 
+// the workspace's parts, each 16-byte aligned
 size_t info_bytes(int total_q) { return ((size_t)total_q * sizeof(int4) + 255) / 256 * 256; }
+size_t ml_bytes(const Kv4Run& r, int n_q) { return ((size_t)r.slots * r.tok_cap * n_q * 2 * sizeof(float) + 255) / 256 * 256; }
 size_t plan_bytes(const Kv4Run& r, int total_q, int n_q, int head_dim) {
-    return r.runs ? info_bytes(total_q) + (size_t)r.slots * r.tok_cap * n_q * (head_dim + 2) * sizeof(float) : 0;
+    return r.runs ? info_bytes(total_q) + ml_bytes(r, n_q) + (size_t)r.slots * r.tok_cap * n_q * head_dim * sizeof(float) : 0;
 }
 
 // Blocks with work where each sequence has its own: of all row tiles that there can be, not of as many in every sequence.
@@ -936,8 +938,9 @@ void launch_kv4_attention(const Kv4Args& a, hipStream_t st) {
     if (!counts || !joins(a.total, a.n_q) || !a.work || !aligned(a.work, 16) || a.work_bytes < plan_bytes(r, a.total, a.n_q, a.head_dim)) r.runs = 0;
     if (r.runs) {
         r.info = reinterpret_cast<int4*>(a.work);
-        r.ml = reinterpret_cast<float*>(reinterpret_cast<char*>(a.work) + info_bytes(a.total));
-        r.o = r.ml + (size_t)r.slots * r.tok_cap * a.n_q * 2;
+        char* ml = reinterpret_cast<char*>(a.work) + info_bytes(a.total);
+        r.ml = reinterpret_cast<float*>(ml);
+        r.o = reinterpret_cast<float*>(ml + ml_bytes(r, a.n_q));
     }
     r.per_page = a.page_size / kTile;
     r.magic = r.per_page == 1 ? 0 : (unsigned)((((uint64_t)1 << 32) + r.per_page - 1) / r.per_page);
