@@ -1042,3 +1042,34 @@ def test_rope_small_sines(vla):
     # reference as well.
     bound = 6 * 2.0 ** -23 * want.abs() + 2.0 ** -37
     ref.within(o.cpu()[small], want[small], bound[small])
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF16, 64), (F32, 128)])
+def test_decode_rows_far_apart(vla, dtype, hd):
+    """Queries and results whose offsets in their buffer pass 32 bits, through the cache's attention."""
+    lens, new = [700, 130, 90], [600, 70, 30]
+    T, ld = sum(new), (1 << 22) // (2 if dtype is F32 else 1)
+    q, cache, table, ks, vs = _decode_case(vla, lens, new, 2, 1, hd, 32, dtype, seed=hd)
+    buf = torch.empty(T, ld, dtype=dtype, device=DEV)
+    assert buf.numel() * buf.element_size() > 1 << 32
+    qd, out = buf[:, :2 * hd], buf[:, 2 * hd:4 * hd]
+    qd.copy_(q)
+    want, bound = ref.decode(q, ks, vs, new, 2, 1, hd, hd ** -0.5)
+    for max_len in (700, 16384):
+        work = torch.empty(max(16, vla.kv4_attention_work_bytes(T, 3, 600, max_len, 2, 1, hd)), dtype=torch.uint8, device=DEV)
+        out.fill_(5.0)
+        vla.kv4_attention_dev(out, qd, cache, 2, 1, hd, 32, hd ** -0.5, table, _i32(lens), _i32(_starts(new)), 600, max_len, work)
+        ref.within(out, want, bound, f"max_len {max_len}")
+    assert work.numel() > 16
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_repeated_joins_give_the_same_bits(vla, dtype):
+    """Pieces of sequences are joined in their order, whichever block is done first."""
+    lens, new = [3000, 3, 700], [1, 1, 20]
+    q, cache, table, _, _ = _decode_case(vla, lens, new, 4, 2, 64, 64, dtype, seed=62)
+    assert vla.kv4_attention_work_bytes(sum(new) + 2, 3, 20, 20000, 4, 2, 64) > 0
+    run = lambda: _run_decode(vla, q, cache, table, lens, new, 4, 2, 64, 64, 0.125, True, max_len=20000)
+    first = run()
+    for _ in range(5):
+        assert torch.equal(run(), first)
