@@ -1073,3 +1073,21 @@ def test_repeated_joins_give_the_same_bits(vla, dtype):
     first = run()
     for _ in range(5):
         assert torch.equal(run(), first)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,n_q,hd", [([500], 2, 64), ([200], 2, 64), ([290, 250], 70, 32), ([300], 1, 128), ([260], 1, 200)])
+def test_packed_values_that_grow(vla, dtype, causal, lens, n_q, hd):
+    """Values that reach the end of the range late, where sums of small ones are under way; tiny values beside them,
+    in sequences and queries of their own, keep their bits."""
+    g = _gen(hd + sum(lens) + 1)
+    q, k, v = _packed_case(g, lens, lens, n_q, 1, hd, dtype)
+    v[140:] *= 1e-30
+    v[140:lens[0]] *= 1e38
+    v[140:lens[0]] = v[140:lens[0]].clamp(-2e8, 2e8)
+    v[140:lens[0]] *= 1e30
+    assert bool(torch.isfinite(v).all())
+    s = _starts(lens)
+    want, bound = ref.packed(q, k, v, s, s, n_q, 1, hd, hd ** -0.5, causal, base=torch.full_like(q, 5.0))
+    ref.within(_run_packed(vla, q, k, v, lens, lens, n_q, 1, hd, hd ** -0.5, causal, same=True), want, bound)

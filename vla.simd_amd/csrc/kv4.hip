@@ -271,6 +271,8 @@ struct Kv4Run {
     int slots;         // pieces in the workspace
     unsigned per_page; // tiles of a page, and 2^32 / per_page rounded up
     unsigned magic;
+    float lift;        // the weights' scale in log2, negated
+    float wscale;      // of the weights in the product with V against those in their sum: 2^-lift with 24 bits, else 1
     int4* info;        // workspace: [total queries] first piece, pieces, token in its sequence
     float* ml;         // [slots][tok_cap * n_q][2]
     float* o;          // [slots][tok_cap * n_q][head_dim]
@@ -548,7 +550,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attn_kernel(Kv4Args a, Kv4Run r
             // The reference only has to keep the weights in range: it follows the
             // maximum when a row's has grown by 2^6, so most tiles rescale nothing.
             if (__any(mx > m + 6.0f)) {
-                const float mn = ceilf(fmaxf(m, mx));
+                const float mn = fmaxf(m, mx);
                 const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
                 m = mn;
                 l *= alpha;
@@ -557,13 +559,14 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attn_kernel(Kv4Args a, Kv4Run r
 #pragma unroll
                     for (int r = 0; r < 4; r++) o[t][r] *= alpha;
             }
-            // Weights are exp2(score - m - 34), below 2^-28, so that sums over 2^28 keys of weights times any values stay
-            // in fp32's range; m is a whole number, so that this and the factors between references are exact.
-            const float mu = (m == -INFINITY ? 0.0f : m) + 34.0f;
+            // Weights reach 2^6, and no sum over all keys may leave fp32's range: they are 2^-lift as large, in the
+            // product alone where they have 24 bits, as their exponent's rounding to 2^-19 would show.
+            const float mu = (m == -INFINITY ? 0.0f : m) + (PP == 3 ? 0.0f : run.lift);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[i] = __builtin_amdgcn_exp2f(x[i] - mu);
                 l += x[i];
+                if (PP == 3) x[i] *= run.wscale;
             }
             U4 pb[PP];
 #pragma unroll
@@ -657,7 +660,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_attn_kernel(Kv4Args a, Kv4Run r
             }
             const int rhead = kvh * group + rhh;
             if (pieces == 1) {
-                static_cast<T*>(a.out)[(size_t)(q0 + rtok) * a.ldo + rhead * HD + d] = (T)(sum == 0.0f ? 0.0f : acc / sum);
+                static_cast<T*>(a.out)[(size_t)(q0 + rtok) * a.ldo + rhead * HD + d] = (T)(sum == 0.0f ? 0.0f : acc / (sum * run.wscale));
             } else {
                 const size_t rr = ((size_t)slot * run.tok_cap + rtok) * a.n_q + rhead;
                 run.o[rr * HD + d] = acc;
@@ -744,7 +747,7 @@ __global__ __launch_bounds__(N) void kv4_join_kernel(Kv4Args a, Kv4Run run) {
         acc.z += v.z;
         acc.w += v.w;
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / (sum * run.wscale);
     Pack<T, 4> o;
     o.v[0] = (T)(acc.x * inv);
     o.v[1] = (T)(acc.y * inv);
@@ -950,6 +953,10 @@ void launch_kv4_attention(const Kv4Args& a, hipStream_t st) {
     const int64_t busy = row_blocks(r, a.total, a.n_seqs, a.n_q, a.n_kv), grid = 2 * busy > 1 << 16 ? 2 * busy : 1 << 16;
     const int64_t most = grid / ((int64_t)a.n_kv * r.head_tiles * (r.runs ? r.runs : a.n_seqs));
     if (r.tok_tiles > most) r.tok_tiles = (int)(most < 1 ? 1 : most);
+    int log2_n = 0;
+    while (1 << log2_n < a.ld_table * a.page_size) log2_n++;
+    r.lift = 6.0f + (float)log2_n;
+    r.wscale = a.dtype == kF32 ? std::ldexp(1.0f, -6 - log2_n) : 1.0f;
     if (a.dtype == kF32) run_attn<float, 3, 3>(a, r, st);
     else if (a.dtype == kBf16) run_attn<bf16_t, 1, 2>(a, r, st);
     else run_attn<f16_t, 2, 2>(a, r, st);

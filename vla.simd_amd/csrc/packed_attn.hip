@@ -69,15 +69,23 @@ __device__ __forceinline__ float halves_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Weights are exp2(score - m + lift), which cancels in o / l. The reference m only has to keep them in range:
-// it follows the row's maximum when that has grown by 2^6, so most tiles rescale nothing.
-// fp16: weights reach 2^15. bf16: they stay below 2^-28, so that sums over 2^28 keys of weights times values
-// of any size are in fp32's range before they are divided (weights 2^-92 of the largest vanish for
-// that). m - lift is off by 2^-19 at most for scores below 30, between tiles with another m; so are weights of 8 bits.
-// fp32: lift 0, as that would show; the values are taken 2^-34 as large instead, exactly.
-template <class T>
-constexpr float lift() { return __is_same(T, f16_t) ? 9.0f : -34.0f; }
-constexpr float kValueScale = 0x1p-34f;
+// Sums of weights times values are divided at the end only, and must be in range before. The reference m of
+// the weights follows the row's maximum when that has grown by 2^6, so weights reach 2^6 and a sum over n
+// keys 2^6 n times the largest value.
+// 16-bit types: weights are exp2(score - m + lift), which cancels in o / l. fp16: 9, for the small weights' sake;
+// sums have room enough. bf16: -(6 + log2 n), so that no values overflow; the sum m - lift is rounded to 2^-19 or so
+// of a weight, of which 8 bits are kept. What vanishes for it are weights below 2^-100 of the largest.
+// fp32: such a rounding would show. A block whose values reach 2^90 (2^28 keys of them still add up) takes them and its
+// sums 2^-34 as large from there on, exactly; others keep their small values. (All weights times a factor of
+// one or 2^-34: 2% slower.)
+float lift_of(const PackedAttnArgs& a) {
+    if (a.dtype == kF16) return 9.0f;
+    int log2_n = 0;
+    while ((int64_t)1 << log2_n < a.total_k) log2_n++;
+    return -(6.0f + (float)log2_n);
+}
+constexpr unsigned kLargeBits = 0x6c800000u;  // 2^90
+constexpr float kLargeScale = 0x1p-34f;
 
 // What a block works on: query rows [q0, q0 + nq) of the packed buffers, at
 // offset `at` in their sequence, and its keys [k0, k0 + nk).
@@ -348,7 +356,7 @@ __global__ __launch_bounds__(64 * QW * SPLIT, HDP == 64 || HDP == 128 && QW == 4
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] *= alpha;
         }
-        const float mu = (m == -INFINITY ? 0.0f : m) - lift<T>();
+        const float mu = (m == -INFINITY ? 0.0f : m) - a.lift;
         v8 p[NK][2];
 #pragma unroll
         for (int kt = 0; kt < NK; kt++)
@@ -508,6 +516,7 @@ __global__ __launch_bounds__(parts_threads(KP), KP == 4 || KT * HC <= 4096 && HC
     __shared__ __attribute__((aligned(16))) bf16_t Ks[3 * PLANE], Vs[3 * PLANE];
     __shared__ unsigned long long kbad[2][KT <= 64 ? 1 : 2];  // rows of the tile with values that are not finite
     __shared__ int vbad;                    // first key of the first tile with such values of V
+    __shared__ int vlarge;                  // values of V have reached 2^90
 
     int tile, head;
     tile_and_head(a, tile, head);
@@ -557,14 +566,14 @@ __global__ __launch_bounds__(parts_threads(KP), KP == 4 || KT * HC <= 4096 && HC
                 vr[i][4 * h] = v.x, vr[i][4 * h + 1] = v.y, vr[i][4 * h + 2] = v.z, vr[i][4 * h + 3] = v.w;
             }
     };
-    auto finite8 = [](const float* x) {
+    auto top8 = [](const float* x) {  // bits of the largest magnitude, those of what is not finite above all others
         unsigned top = 0;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const unsigned u = __float_as_uint(x[i]) & 0x7fffffffu;
             top = u > top ? u : top;
         }
-        return top < 0x7f800000u;
+        return top;
     };
     auto put = [&](bf16_t* planes, int e, const float* x) {
         const Parts p = split8(x);
@@ -573,24 +582,31 @@ __global__ __launch_bounds__(parts_threads(KP), KP == 4 || KT * HC <= 4096 && HC
         *reinterpret_cast<v8bf*>(planes + PLANE + at) = p.m;
         *reinterpret_cast<v8bf*>(planes + 2 * PLANE + at) = p.l;
     };
+    bool large = false;  // V in LDS and o are 2^-34 as large
     auto land = [&](int t) {
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             const int e = tid + NTH * i;
-            if (!finite8(kr[i])) {
+            if (top8(kr[i]) >= 0x7f800000u) {
                 atomicOr(&kbad[t & 1][e / CH >> 6], 1ull << (e / CH & 63));
 #pragma unroll
                 for (int x = 0; x < 8; x++) kr[i][x] = 0.0f;
             }
-            if (!finite8(vr[i])) {
-                atomicMin(&vbad, t * KT);
+            const unsigned top = top8(vr[i]);
+            if (__builtin_expect(top >= kLargeBits, 0)) {
+                vlarge = 1;
+                if (top >= 0x7f800000u) {
+                    atomicMin(&vbad, t * KT);
 #pragma unroll
-                for (int x = 0; x < 8; x++)
-                    if (!(fabsf(vr[i][x]) < INFINITY)) vr[i][x] = 0.0f;
+                    for (int x = 0; x < 8; x++)
+                        if (!(fabsf(vr[i][x]) < INFINITY)) vr[i][x] = 0.0f;
+                }
             }
-#pragma unroll
-            for (int x = 0; x < 8; x++) vr[i][x] *= kValueScale;
             put(Ks, e, kr[i]);
+            if (large) {
+#pragma unroll
+                for (int x = 0; x < 8; x++) vr[i][x] *= kLargeScale;
+            }
             put(Vs, e, vr[i]);
         }
     };
@@ -615,6 +631,7 @@ __global__ __launch_bounds__(parts_threads(KP), KP == 4 || KT * HC <= 4096 && HC
         for (auto& w : kbad)
             for (auto& x : w) x = 0;
         vbad = 0x7fffffff;
+        vlarge = 0;
     }
 
     v16f o[DT] = {};
@@ -625,6 +642,20 @@ __global__ __launch_bounds__(parts_threads(KP), KP == 4 || KT * HC <= 4096 && HC
         __syncthreads();  // the previous tile is read
         land(t);
         __syncthreads();
+        if (__builtin_expect(!large && __builtin_amdgcn_readfirstlane(vlarge), 0)) {  // the first such tile: its values again
+            large = true;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+#pragma unroll
+                for (int x = 0; x < 8; x++) vr[i][x] *= kLargeScale;
+                put(Vs, tid + NTH * i, vr[i]);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] *= kLargeScale;
+            __syncthreads();
+        }
         if (t + 1 < tiles) fetch(t + 1);
         const unsigned long long marked = kbad[t & 1][kw >> 6] >> (kw & 63);  // of the wave's keys on
         if (tid == 0)
@@ -762,7 +793,7 @@ __global__ __launch_bounds__(parts_threads(KP), KP == 4 || KT * HC <= 4096 && HC
     }
 
     l = halves_sum(l);
-    const float inv = (1.0f / kValueScale) / l;
+    const float inv = 1.0f / (large ? l * kLargeScale : l);
     const Rows orows(static_cast<const float*>(a.out) + (size_t)job.q0 * a.ldo + head * hd, (int64_t)job.nq * a.ldo * 4);
 #pragma unroll
     for (int d = 0; d < DT; d++)
@@ -790,6 +821,7 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* Ks = reinterpret_cast<float*>(smem);  // [KT][SK]
     float* Vs = Ks + KT * SK;
+    __shared__ int vlarge;  // as in the kernel above
 
     int tile, head;
     tile_and_head(a, tile, head);
@@ -829,6 +861,7 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
     const int tiles = (end + KT - 1) / KT;
 
     float4 kr[LOADS], vr[LOADS];
+    auto small = [](float4 x) { return make_float4(x.x * kLargeScale, x.y * kLargeScale, x.z * kLargeScale, x.w * kLargeScale); };
     auto gload = [&](int t) {
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
@@ -842,24 +875,42 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
             }
         }
     };
+    bool large = false;
     auto lstore = [&]() {
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
+            if (large) vr[i] = small(vr[i]);
             const int e = tid + 256 * i, row = e / (HDP / 4), d = 4 * (e % (HDP / 4));
             *reinterpret_cast<float4*>(Ks + row * SK + d) = kr[i];
-            *reinterpret_cast<float4*>(Vs + row * SK + d) = make_float4(vr[i].x * kValueScale, vr[i].y * kValueScale, vr[i].z * kValueScale, vr[i].w * kValueScale);
+            *reinterpret_cast<float4*>(Vs + row * SK + d) = vr[i];
+            const float top = fmaxf(fmaxf(fabsf(vr[i].x), fabsf(vr[i].y)), fmaxf(fabsf(vr[i].z), fabsf(vr[i].w)));
+            if (__float_as_uint(top) >= kLargeBits) vlarge = 1;
         }
     };
 
     v4f o[DT] = {};
     float m = -INFINITY, l = 0.0f;
     const float c2 = a.scale * kLog2e;
+    if (tid == 0) vlarge = 0;
     if (tiles) gload(0);
     for (int t = 0; t < tiles; t++) {
         const int k0 = t * KT;
         __syncthreads();
         lstore();
         __syncthreads();
+        if (__builtin_expect(!large && __builtin_amdgcn_readfirstlane(vlarge), 0)) {  // as in the kernel above
+            large = true;
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const int e = tid + 256 * i, row = e / (HDP / 4), d = 4 * (e % (HDP / 4));
+                *reinterpret_cast<float4*>(Vs + row * SK + d) = small(vr[i]);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) o[d][r] *= kLargeScale;
+            __syncthreads();
+        }
         if (t + 1 < tiles) gload(t + 1);
         bool rare = false;
         if (k0 + KT > limit(0)) {
@@ -946,7 +997,7 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
     }
 
     l = rows_sum(l);
-    const float inv = (1.0f / kValueScale) / l;
+    const float inv = 1.0f / (large ? l * kLargeScale : l);
     if (!qok) return;
     float* dst = static_cast<float*>(a.out) + (size_t)(job.q0 + qi) * a.ldo + head * hd;
 #pragma unroll
@@ -1024,7 +1075,7 @@ void run_f32(const PackedAttnArgs& a, hipStream_t st) {
 
 }  // namespace
 
-void launch_packed_attention(const PackedAttnArgs& a, hipStream_t st) {
+void launch_packed_attention(PackedAttnArgs a, hipStream_t st) {
     VLA_REQUIRE(dtype_ok(a.dtype), "packed_attention: dtype must be VLA_F32, VLA_BF16 or VLA_F16");
     VLA_REQUIRE(a.n_seqs >= 0 && a.total_q >= 0 && a.total_k >= 0 && a.n_q > 0 && a.n_kv > 0,
                 "packed_attention: need n_seqs, total_q, total_k >= 0, n_q > 0, n_kv > 0");
@@ -1046,6 +1097,7 @@ void launch_packed_attention(const PackedAttnArgs& a, hipStream_t st) {
     VLA_REQUIRE(a.ldq >= a.n_q * a.head_dim && a.ldo >= a.n_q * a.head_dim && a.ldk >= a.n_kv * a.head_dim &&
                     a.ldv >= a.n_kv * a.head_dim,
                 "packed_attention: row stride shorter than heads * head_dim");
+    a.lift = lift_of(a);
     if (a.dtype == kBf16) run_16<bf16_t>(a, st);
     else if (a.dtype == kF16) run_16<f16_t>(a, st);
     else run_f32(a, st);

@@ -46,8 +46,9 @@ struct PackedAttnArgs {
     int n_seqs, total_q, total_k, n_q, n_kv, head_dim;
     float scale;
     int causal, dtype;
+    float lift;  // set by the launcher
 };
-void launch_packed_attention(const PackedAttnArgs& a, hipStream_t st);
+void launch_packed_attention(PackedAttnArgs a, hipStream_t st);
 
 // kv4.hip: the paged cache of 4-bit values (layout in kv4.h)
 struct Kv4Args {
