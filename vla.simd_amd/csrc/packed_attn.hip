@@ -1027,7 +1027,8 @@ void run_16_split(const PackedAttnArgs& a, hipStream_t st) {
     launch_tiles(&packed_attn_16<T, HDP, HC, KT, SPLIT, QW>, a, 32 * QW, 64 * QW * SPLIT, 0, st);
 }
 // Two halves of the keys per block, and blocks of 64 queries, where blocks of four waves would
-// leave CUs idle or alone and the sequences have some length. Measured, us, four waves with 128
+// leave CUs idle or alone and the sequences have some length. (304 is of blocks as max_tiles counts them, up to one tile
+// a sequence more than there are: some more than the 256 CUs for a few sequences.) Measured, us, four waves with 128
 // queries | two halves | two halves with 64 (blocks of 128 named): 96 blocks of 256 keys 13.6 | 13.4 |
 // 11.4, 160 of 512 18.5 | 17.2 | 14.5, 108 of 1024 (no mask, heads of 64) 17.1 | 15.4 | 12.4, 216 of 1024
 // 18.2 | 16.6 | 16.7, 288 of 1024 (heads of 128) 28.4 | 25.1 | 30.1; one half is ahead where a block has but one tile, 32

@@ -163,7 +163,7 @@ void launch_qk_norm_rope(RopeHeadsArgs a, hipStream_t st) {
                     "qk_norm_rope: rows must be 16-byte aligned");
     }
     // Tokens of a block: several share the first half's latency, but blocks for every CU come
-    // first. Measured, us, 1 | 2 | 4 tokens (24 heads of 128, bf16): 100 tokens 4.4 | 5.5 | 6.5, 2371
+    // first. By the tokens alone, as measured, us, 1 | 2 | 4 tokens (24 heads of 128, bf16): 100 tokens 4.4 | 5.5 | 6.5, 2371
     // 9.0 | 9.2 | 10.2, 4000 13.2 | 12.5 | 12.7, 8000 20.8 | 19.9 | 19.3, 16000 35.2 | 34.0 | 33.5 (5.9 TB/s);
     // 32768 of 40 heads 129 | 126 | 127 (5.3 TB/s).
     a.tokens_per_block = a.seq < 4000 ? 1 : a.seq < 8000 ? 2 : 4;

@@ -1,7 +1,7 @@
 // serving.h - the operators of a decoder that serves several prompts: their
 // launchers, and the device helpers that their kernels share. Values are
-// fp32, bf16 or fp16 (vla_dtype); every sum and statistic is fp32, and a result
-// is rounded to its type once.
+// fp32, bf16 or fp16 (vla_dtype); every sum and statistic is held in fp32 or more (angles, and the
+// norm's squares where they leave fp32's range, in 64 bits), and a result is rounded to its type once.
 #pragma once
 
 #include "common.h"
