@@ -1091,3 +1091,15 @@ def test_packed_values_that_grow(vla, dtype, causal, lens, n_q, hd):
     s = _starts(lens)
     want, bound = ref.packed(q, k, v, s, s, n_q, 1, hd, hd ** -0.5, causal, base=torch.full_like(q, 5.0))
     ref.within(_run_packed(vla, q, k, v, lens, lens, n_q, 1, hd, hd ** -0.5, causal, same=True), want, bound)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("hd", [64, 128, 200])
+def test_packed_tiny_values_beside_unseen_ones(vla, hd, bad):
+    """An infinity or NaN that a query does not see does not cost the small values it does see any bits."""
+    q, k, v = _packed_case(_gen(hd), [150], [150], 2, 1, hd, F32)
+    v *= 1e-33
+    want, bound = ref.packed(q, k, v, [0, 150], [0, 150], 2, 1, hd, hd ** -0.5, True, base=torch.full_like(q, 5.0))
+    v[100, 3] = bad
+    got = _run_packed(vla, q, k, v, [150], [150], 2, 1, hd, hd ** -0.5, True)
+    ref.within(got[:100], want[:100], bound[:100])

@@ -77,7 +77,8 @@ __device__ __forceinline__ float halves_sum(float x) {
 // of a weight, of which 8 bits are kept. What vanishes for it are weights below 2^-100 of the largest.
 // fp32: such a rounding would show. A block whose values reach 2^90 (2^28 keys of them still add up) takes them and its
 // sums 2^-34 as large from there on, exactly; others keep their small values. (All weights times a factor of
-// one or 2^-34: 2% slower.)
+// one or 2^-34: 2% slower.) Past 128 columns the weights are 2^lift as large in the product, exactly (the same check of
+// the values there: 7% slower).
 float lift_of(const PackedAttnArgs& a) {
     if (a.dtype == kF16) return 9.0f;
     int log2_n = 0;
@@ -592,15 +593,14 @@ __global__ __launch_bounds__(parts_threads(KP), KP == 4 || KT * HC <= 4096 && HC
 #pragma unroll
                 for (int x = 0; x < 8; x++) kr[i][x] = 0.0f;
             }
-            const unsigned top = top8(vr[i]);
-            if (__builtin_expect(top >= kLargeBits, 0)) {
-                vlarge = 1;
-                if (top >= 0x7f800000u) {
+            if (__builtin_expect(top8(vr[i]) >= kLargeBits, 0)) {
+                if (top8(vr[i]) >= 0x7f800000u) {
                     atomicMin(&vbad, t * KT);
 #pragma unroll
                     for (int x = 0; x < 8; x++)
                         if (!(fabsf(vr[i][x]) < INFINITY)) vr[i][x] = 0.0f;
                 }
+                if (top8(vr[i]) >= kLargeBits) vlarge = 1;
             }
             put(Ks, e, kr[i]);
             if (large) {
@@ -821,7 +821,6 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* Ks = reinterpret_cast<float*>(smem);  // [KT][SK]
     float* Vs = Ks + KT * SK;
-    __shared__ int vlarge;  // as in the kernel above
 
     int tile, head;
     tile_and_head(a, tile, head);
@@ -861,7 +860,6 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
     const int tiles = (end + KT - 1) / KT;
 
     float4 kr[LOADS], vr[LOADS];
-    auto small = [](float4 x) { return make_float4(x.x * kLargeScale, x.y * kLargeScale, x.z * kLargeScale, x.w * kLargeScale); };
     auto gload = [&](int t) {
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
@@ -875,42 +873,24 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
             }
         }
     };
-    bool large = false;
     auto lstore = [&]() {
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
-            if (large) vr[i] = small(vr[i]);
             const int e = tid + 256 * i, row = e / (HDP / 4), d = 4 * (e % (HDP / 4));
             *reinterpret_cast<float4*>(Ks + row * SK + d) = kr[i];
             *reinterpret_cast<float4*>(Vs + row * SK + d) = vr[i];
-            const float top = fmaxf(fmaxf(fabsf(vr[i].x), fabsf(vr[i].y)), fmaxf(fabsf(vr[i].z), fabsf(vr[i].w)));
-            if (__float_as_uint(top) >= kLargeBits) vlarge = 1;
         }
     };
 
     v4f o[DT] = {};
     float m = -INFINITY, l = 0.0f;
-    const float c2 = a.scale * kLog2e;
-    if (tid == 0) vlarge = 0;
+    const float c2 = a.scale * kLog2e, ws = __builtin_amdgcn_exp2f(a.lift);
     if (tiles) gload(0);
     for (int t = 0; t < tiles; t++) {
         const int k0 = t * KT;
         __syncthreads();
         lstore();
         __syncthreads();
-        if (__builtin_expect(!large && __builtin_amdgcn_readfirstlane(vlarge), 0)) {  // as in the kernel above
-            large = true;
-#pragma unroll
-            for (int i = 0; i < LOADS; i++) {
-                const int e = tid + 256 * i, row = e / (HDP / 4), d = 4 * (e % (HDP / 4));
-                *reinterpret_cast<float4*>(Vs + row * SK + d) = small(vr[i]);
-            }
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) o[d][r] *= kLargeScale;
-            __syncthreads();
-        }
         if (t + 1 < tiles) gload(t + 1);
         bool rare = false;
         if (k0 + KT > limit(0)) {
@@ -962,6 +942,7 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
                 for (int r = 0; r < 4; r++) {
                     s[kt][r] = __builtin_amdgcn_exp2f(s[kt][r] - mu);
                     l += s[kt][r];
+                    s[kt][r] *= ws;
                 }
             if (!rare) {
 #pragma unroll
@@ -997,7 +978,7 @@ __global__ __launch_bounds__(256) void packed_attn_f32(PackedAttnArgs a) {
     }
 
     l = rows_sum(l);
-    const float inv = 1.0f / (large ? l * kLargeScale : l);
+    const float inv = 1.0f / (l * ws);
     if (!qok) return;
     float* dst = static_cast<float*>(a.out) + (size_t)(job.q0 + qi) * a.ldo + head * hd;
 #pragma unroll
