@@ -511,6 +511,101 @@ VLA_API int32_t vla_kv4_attention_dev(void* out, int64_t ldo, const void* Q, int
                                       int32_t head_dim, float scale, int32_t dtype, void* work,
                                       int64_t work_bytes, void* stream);
 
+/* --------------------------------------------- steps with drafted tokens -- */
+/* A step that drafts several tokens for every sequence, lets the target read them all
+ * at once and keeps a path of them, over the cache above (no counterpart in the
+ * reference). Rows, sequences, types and errors as above.
+ *
+ * The n packed rows of a sequence are the nodes of a tree: row 0 its last certain
+ * token, behind it drafted ones. parent (device, int32 per row) is a row's parent by its
+ * number in the sequence; a number outside [0, its own) is none. NULL: the row before, a chain. The
+ * nodes are the newest n of the sequence's lens[s] tokens, in the order of their rows.
+ *
+ * Positions and masks of the nodes: pos [total] = lens[s] - n + depth, and in see
+ * [total, ld_see] bit t % 32 of word t / 32 for a node itself and every node t above
+ * it, all other bits of its row 0. Bits from 32 * ld_see on are left out. */
+VLA_API int32_t vla_draft_tree_dev(int32_t* pos, uint32_t* see, int32_t ld_see, const int32_t* parent,
+                                   const int32_t* lens, const int32_t* start, int32_t n_seqs,
+                                   int32_t total, void* stream);
+
+/* Angles by which a position turns each of rot_dim / 2 pairs (host): base^(-2 i / rot_dim), and
+ * for positions beyond a trained length
+ *   LINEAR  all divided by factor (position interpolation);
+ *   BASE    of the base times factor^(rot_dim / (rot_dim - 2));
+ *   PARTS   a pair that makes `turns` turns over `trained` positions is divided by factor where turns <= low,
+ *           left where turns >= high, and mixed in between by (turns - low) / (high - low).
+ * magnitude (may be NULL): 1, for PARTS 0.1 ln(factor) + 1, to scale the rotated values by. */
+typedef enum { VLA_ROPE_PLAIN = 0, VLA_ROPE_LINEAR = 1, VLA_ROPE_BASE = 2, VLA_ROPE_PARTS = 3 } vla_rope_scaling;
+VLA_API int32_t vla_rope_freqs(double* freqs, double* magnitude, int32_t rot_dim, double base,
+                               int32_t scaling, double factor, double trained, double low, double high);
+
+/* vla_qk_norm_rope_dev's norms, a rotation, and vla_kv4_append_dev in one pass. The first rot_dim (a
+ * multiple of 8, 0 for none) values of a head are pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1)
+ * where interleaved != 0; pair i turns by pos[row] * freqs[i] (pos NULL: the row's number in its sequence,
+ * lens[s] - n + i; freqs [rot_dim / 2] double on the device) and is multiplied by magnitude; the other values of
+ * the head stay. Queries go to q_out (n_q may be 0), keys to k_out unless it is NULL, keys and V into the
+ * cache as vla_kv4_append_dev writes rows, but from the rotated keys in 64 bits, before they are rounded to their
+ * type (a value past fp32's range counts as infinite). cache NULL: nothing is stored, V, table and the page
+ * sizes are not used. q_out may be q, k_out may be K. head_dim as for the cache; fewer than 2^26 rows. */
+VLA_API int32_t vla_rope_kv4_append_dev(void* q_out, int64_t ldqo, void* k_out, int64_t ldko, void* cache,
+                                        int32_t n_pages, int32_t page_size, const void* q, int64_t ldq,
+                                        const void* K, int64_t ldk, const void* V, int64_t ldv,
+                                        const float* q_weight, const float* k_weight, float eps,
+                                        const int32_t* pos, const double* freqs, int32_t rot_dim,
+                                        double magnitude, int32_t interleaved, const int32_t* table,
+                                        int32_t ld_table, const int32_t* lens, const int32_t* start,
+                                        int32_t n_seqs, int32_t total, int32_t n_q, int32_t n_kv,
+                                        int32_t head_dim, int32_t dtype, void* stream);
+
+/* vla_kv4_attention_dev with a mask among the newest tokens: row i of the n of sequence s sees
+ * the keys j < lens[s] - n, and key lens[s] - n + t (t < n) where bit t of its words in see [total_q, ld_see]
+ * is set, itself included. Words that a row does not have are 0. A row that sees no key gets
+ * zeros. Everything else as there, the workspace by its own function. */
+VLA_API int64_t vla_kv4_tree_attention_work_bytes(int32_t total_q, int32_t n_seqs, int32_t max_new,
+                                                  int32_t max_len, int32_t n_q, int32_t n_kv,
+                                                  int32_t head_dim);
+VLA_API int32_t vla_kv4_tree_attention_dev(void* out, int64_t ldo, const void* Q, int64_t ldq,
+                                           const void* cache, int32_t n_pages, int32_t page_size,
+                                           const int32_t* table, int32_t ld_table, const int32_t* lens,
+                                           const int32_t* q_start, const uint32_t* see, int32_t ld_see,
+                                           int32_t n_seqs, int32_t total_q, int32_t max_new,
+                                           int32_t max_len, int32_t n_q, int32_t n_kv, int32_t head_dim,
+                                           float scale, int32_t dtype, void* work, int64_t work_bytes,
+                                           void* stream);
+
+/* Which drafted tokens the target accepts, and the token behind them, so that all of them
+ * are distributed as the target's own. p [total, vocab]: the target's probabilities behind each node; q (NULL:
+ * none) the draft's there, from which the node's children were drawn independently; both of one type, rows
+ * aligned to it. tokens [total] the nodes' tokens, u [total] and u_next [n_seqs] uniform in [0, 1). From row 0
+ * on, at node x with the rows p and q, its children c in order:
+ *   with q:  a = 0, S = 1; c is accepted if u[c] * S * q(c) < p(c) - a * q(c), otherwise a += S and
+ *            S = sum over v of max(p(v) - a q(v), 0); where S is 0 no further child is tried;
+ *   without: S = 1; c is accepted if u[c] * S < p(c), taken as 0 for a token refused at x before,
+ *            otherwise S -= p(c).
+ * The walk goes on at an accepted child and ends where none is. The next token is the first v whose
+ * sum of w(0) .. w(v) exceeds u_next[s] times the sum of all, w = max(p - a q, 0) at the last node, or p without
+ * the refused tokens, or where that has no sum max(p, 0); the last v with w(v) > 0 where none exceeds it, -1 where
+ * there is none. NaN counts as 0 in w and accepts nothing, a token outside [0, vocab) has probability 0; infinite
+ * probabilities give some token of [-1, vocab). Sums are of 64 bits. path [total], packed as the rows:
+ * the accepted nodes' numbers, row 0 first, then -1; count [n_seqs] how many, row 0 among them (0 where a
+ * sequence has no rows); token [n_seqs]. At most 65535 sequences. */
+VLA_API int32_t vla_verify_drafts_dev(int32_t* path, int32_t* count, int32_t* token, const void* p,
+                                      int64_t ldp, const void* q, int64_t ldq, const int32_t* tokens,
+                                      const int32_t* parent, const int32_t* start, const float* u,
+                                      const float* u_next, int32_t n_seqs, int32_t total, int32_t vocab,
+                                      int32_t dtype, void* stream);
+
+/* Keeps a path of the newest n tokens: the cached token lens[s] - n + path[i] becomes token lens[s] - n + i
+ * for i < count[s], in place (path packed as the rows, ascending, path[i] >= i, as vla_verify_drafts_dev gives
+ * it), and new_lens[s] (NULL: not wanted; not lens itself) lens[s] - n + count[s]. count is clamped to [0, n]. What
+ * lies behind keeps its bytes. A token without a page is dropped, or moves as NaN. Every layer's cache is kept
+ * with the same path. At most 65535 sequences. */
+VLA_API int32_t vla_kv4_keep_dev(void* cache, int32_t n_pages, int32_t page_size, const int32_t* table,
+                                 int32_t ld_table, const int32_t* lens, const int32_t* start,
+                                 const int32_t* path, const int32_t* count, int32_t* new_lens,
+                                 int32_t n_seqs, int32_t total, int32_t n_kv, int32_t head_dim,
+                                 void* stream);
+
 /* ------------------------------------------------------------ convolution -- */
 /* W8A8 2-D convolution, tcpu::conv2d_i8 (src/ops/conv_ops.h:31-35,
  * src/hal/common/conv.cpp:424-526): x [H, Wd, Cin] fp32 NHWC -> out

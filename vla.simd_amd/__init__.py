@@ -63,6 +63,8 @@ EXPORTS = (
     "vla_dense_linear", "vla_dense_linear_dev",
     "vla_qk_norm_rope_dev", "vla_packed_attention_dev", "vla_kv4_page_bytes", "vla_kv4_offset",
     "vla_kv4_append_dev", "vla_kv4_gather_dev", "vla_kv4_attention_work_bytes", "vla_kv4_attention_dev",
+    "vla_draft_tree_dev", "vla_rope_freqs", "vla_rope_kv4_append_dev", "vla_kv4_tree_attention_work_bytes",
+    "vla_kv4_tree_attention_dev", "vla_verify_drafts_dev", "vla_kv4_keep_dev",
     "vla_act_tf_load", "vla_act_tf_free", "vla_act_tf_chunk", "vla_act_tf_action_dim",
     "vla_act_tf_state_dim", "vla_act_tf_dim", "vla_act_tf_int8_layers", "vla_act_tf_graph_nodes",
     "vla_act_tf_forward", "vla_act_tf_forward_dev", "vla_act_tf_load_ex", "vla_act_tf_n_text",
@@ -126,7 +128,7 @@ _lib = None
 
 def _declare(L):
     P = c_void_p
-    i32, f32, i64 = c_int32, c_float, c_int64
+    i32, f32, i64, f64 = c_int32, c_float, c_int64, ctypes.c_double
     sig = {
         "vla_abi_version": (i32, []),
         "vla_backend_name": (c_char_p, []),
@@ -221,6 +223,15 @@ def _declare(L):
         "vla_kv4_attention_work_bytes": (i64, [i32, i32, i32, i32, i32, i32, i32]),
         "vla_kv4_attention_dev": (i32, [P, i64, P, i64, P, i32, i32, P, i32, P, P, i32, i32, i32, i32, i32, i32, i32,
                                         f32, i32, P, i64, P]),
+        "vla_draft_tree_dev": (i32, [P, P, i32, P, P, P, i32, i32, P]),
+        "vla_rope_freqs": (i32, [P, P, i32, f64, i32, f64, f64, f64, f64]),
+        "vla_rope_kv4_append_dev": (i32, [P, i64, P, i64, P, i32, i32, P, i64, P, i64, P, i64, P, P, f32, P, P, i32, f64,
+                                          i32, P, i32, P, P, i32, i32, i32, i32, i32, i32, P]),
+        "vla_kv4_tree_attention_work_bytes": (i64, [i32, i32, i32, i32, i32, i32, i32]),
+        "vla_kv4_tree_attention_dev": (i32, [P, i64, P, i64, P, i32, i32, P, i32, P, P, P, i32, i32, i32, i32, i32, i32,
+                                             i32, i32, f32, i32, P, i64, P]),
+        "vla_verify_drafts_dev": (i32, [P, P, P, P, i64, P, i64, P, P, P, P, P, i32, i32, i32, i32, P]),
+        "vla_kv4_keep_dev": (i32, [P, i32, i32, P, i32, P, P, P, P, P, i32, i32, i32, i32, P]),
         "vla_act_tf_load": (P, [c_char_p, i32, i32]),
         "vla_act_tf_free": (None, [P]),
         "vla_act_tf_chunk": (i32, [P]),
@@ -915,6 +926,149 @@ def kv4_attention_dev(out, Q, cache, n_q, n_kv, head_dim, page_size, scale, tabl
     _call("vla_kv4_attention_dev", out.data_ptr(), ldo, Q.data_ptr(), ldq, cache.data_ptr(), pages, page_size, table.data_ptr(),
           ld, lens.data_ptr(), _dp(q_start), n, total, max_new, ld * page_size if max_len is None else max_len, n_q, n_kv,
           head_dim, float(scale), dt, wp, wb, _stream(stream))
+
+
+def draft_tree_dev(pos, see, parent, lens, start, stream=None):
+    """Positions pos [total] and masks see [total, words] (int32, bit t % 32 of word t / 32: it sees node t) of drafted
+    tokens: rows start[s] .. start[s + 1] - 1 are the newest of sequence s' lens[s] tokens, parent [total] their parents'
+    numbers in the sequence (None: the row before)."""
+    if _torch is None:
+        _import_torch()
+    n, total = _seqs_of("start", start), pos.shape[0] if pos.dim() == 1 else -1
+    _check_ints("pos", pos, total)
+    words = _check_see(see, total)
+    _check_ints("lens", lens, n)
+    if parent is not None:
+        _check_ints("parent", parent, total)
+    _check_devices(pos, see, parent, lens, start)
+    _call("vla_draft_tree_dev", pos.data_ptr(), see.data_ptr(), words, _dp(parent), lens.data_ptr(), start.data_ptr(), n, total,
+          _stream(stream))
+
+
+def _check_see(see, total):
+    """The words of a row of masks [total, words]."""
+    if see.dtype is not _INT32 or see.dim() != 2 or see.shape[0] != total or not 1 <= see.shape[1] <= 1 << 20 or not see.is_contiguous():
+        raise ValueError(f"see: need contiguous [{total}, words] int32, got {list(see.shape)} of {see.dtype}")
+    return see.shape[1]
+
+
+ROPE_SCALINGS = {"plain": 0, "linear": 1, "base": 2, "parts": 3}  # vla_rope_scaling
+
+
+def rope_freqs(rot_dim, base=10000.0, scaling="plain", factor=1.0, trained=0.0, low=1.0, high=32.0):
+    """(freqs, magnitude): the angles [rot_dim / 2] float64 that a position turns each pair by, base^(-2 i / rot_dim),
+    and what the rotated values are multiplied by. For positions beyond a trained length scaling
+    is "linear" (all divided by factor), "base" (of a larger base) or "parts" (divided by factor where a pair
+    turns at most `low` times over the `trained` positions, as it was where at least `high` times, mixed between)."""
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"scaling must be one of {sorted(ROPE_SCALINGS)}")
+    out = np.empty(max(0, rot_dim // 2), np.float64)
+    mag = ctypes.c_double()
+    _call("vla_rope_freqs", _ptr(out), ctypes.addressof(mag), rot_dim, float(base), ROPE_SCALINGS[scaling], float(factor), float(trained),
+          float(low), float(high))
+    return out, mag.value
+
+
+def rope_kv4_append_dev(q_out, cache, q, k, v, n_q, n_kv, head_dim, page_size, table, lens, start, freqs, pos=None, magnitude=1.0,
+                        interleaved=False, q_weight=None, k_weight=None, eps=1e-6, k_out=None, stream=None):
+    """Norms per head (where a float32 weight [head_dim] is given) and rotation of packed queries and keys, and the keys
+    and values into the cache as the newest tokens of their sequences, in one pass. freqs: a float64 tensor
+    [rot_dim / 2] on the GPU (rope_freqs); pairs are (i, i + rot_dim / 2), or neighbours where interleaved. pos [total]
+    int32 (None: a token's number in its sequence). k_out takes the rotated keys as rows too. cache, v and table None:
+    only rotated; q and q_out None with n_q 0. q_out may be q, k_out may be k."""
+    dt, dtype, total, n = _type_id(k), k.dtype, k.shape[0], _seqs_of("start", start)
+    ldk = _row_ld("k", k, total, n_kv * head_dim, dtype)
+    ldq = ldqo = ldv = ldko = pages = ld = 0
+    if n_q:
+        ldq = _row_ld("q", q, total, n_q * head_dim, dtype)
+        ldqo = ldq if q_out is q else _row_ld("q_out", q_out, total, n_q * head_dim, dtype)
+    if k_out is not None:
+        ldko = ldk if k_out is k else _row_ld("k_out", k_out, total, n_kv * head_dim, dtype)
+    if cache is not None:
+        pages, rows, ld = _cache_shape(cache, n_kv, head_dim, page_size, table)
+        if rows != n:
+            raise ValueError(f"table: need a row for each of {n} sequences, got {rows}")
+        ldv = _row_ld("v", v, total, n_kv * head_dim, dtype)
+    _check_ints("lens", lens, n)
+    if pos is not None:
+        _check_ints("pos", pos, total)
+    if freqs.dtype is not _torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous():
+        raise ValueError("freqs: need a contiguous float64 vector")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.dtype is not _torch.float32 or w.shape != (head_dim,) or not w.is_contiguous()):
+            raise ValueError(f"{name}: need {head_dim} contiguous float32")
+    _check_devices(k, lens, start, freqs, pos, q_weight, k_weight, k_out, *((q, q_out) if n_q else ()),
+                   *((cache, v, table) if cache is not None else ()))
+    _call("vla_rope_kv4_append_dev", q_out.data_ptr() if n_q else None, ldqo, _dp(k_out), ldko, _dp(cache), pages, page_size,
+          q.data_ptr() if n_q else None, ldq, k.data_ptr(), ldk, v.data_ptr() if cache is not None else None, ldv, _dp(q_weight),
+          _dp(k_weight), float(eps), _dp(pos), freqs.data_ptr(), 2 * freqs.shape[0], float(magnitude), 1 if interleaved else 0,
+          table.data_ptr() if cache is not None else None, ld, lens.data_ptr(), start.data_ptr(), n, total, n_q, n_kv, head_dim,
+          dt, _stream(stream))
+
+
+def kv4_tree_attention_work_bytes(total_q, n_seqs, max_new, max_len, n_q, n_kv, head_dim) -> int:
+    """Bytes of kv4_tree_attention_dev's workspace for these sizes (0: it needs none)."""
+    return int(lib().vla_kv4_tree_attention_work_bytes(total_q, n_seqs, max_new, max_len, n_q, n_kv, head_dim))
+
+
+def kv4_tree_attention_dev(out, Q, cache, n_q, n_kv, head_dim, page_size, scale, table, lens, q_start, see, max_new, max_len=None,
+                           work=None, stream=None):
+    """Attention of drafted tokens, Q [total, n_q * head_dim], over the cache: of the n rows of sequence s row i sees the
+    keys before the newest n, and of those the ones whose bits are set in see [total, words] (draft_tree_dev). max_new and
+    max_len bound n and lens (max_len None: what the table can hold); work: a uint8 tensor of
+    kv4_tree_attention_work_bytes, or None to run without splitting the keys."""
+    pages, n, ld = _cache_shape(cache, n_kv, head_dim, page_size, table)
+    dt, dtype, total = _type_id(Q), Q.dtype, Q.shape[0]
+    ldo, ldq = _row_ld("out", out, total, n_q * head_dim, dtype), _row_ld("Q", Q, total, n_q * head_dim, dtype)
+    words = _check_see(see, total)
+    _check_ints("lens", lens, n)
+    _check_ints("q_start", q_start, n + 1)
+    wp, wb = None, 0
+    if work is not None:
+        if work.dtype is not _torch.uint8 or not work.is_contiguous():
+            raise ValueError("work: need contiguous uint8")
+        wp, wb = work.data_ptr(), work.numel()
+    _check_devices(out, Q, cache, table, lens, q_start, see, work)
+    _call("vla_kv4_tree_attention_dev", out.data_ptr(), ldo, Q.data_ptr(), ldq, cache.data_ptr(), pages, page_size, table.data_ptr(),
+          ld, lens.data_ptr(), q_start.data_ptr(), see.data_ptr(), words, n, total, max_new,
+          ld * page_size if max_len is None else max_len, n_q, n_kv, head_dim, float(scale), dt, wp, wb, _stream(stream))
+
+
+def verify_drafts_dev(path, count, token, p, tokens, start, u, u_next, parent=None, q=None, stream=None):
+    """Which drafted tokens the target accepts: p [total, vocab] its probabilities behind each packed row, q (None: drafted
+    with certainty) the draft's, tokens and parent (None: a chain) of the rows, u [total] and u_next [n_seqs]
+    uniform float32. Writes path [total] (the accepted rows' numbers in their sequence, then -1), count and the next
+    token [n_seqs], all int32."""
+    dt, dtype, n = _type_id(p), p.dtype, _seqs_of("start", start)
+    if p.dim() != 2:
+        raise ValueError(f"p: need [total, vocab], got {list(p.shape)}")
+    total, vocab = p.shape
+    ldp = _row_ld("p", p, total, vocab, dtype)
+    ldq = _row_ld("q", q, total, vocab, dtype) if q is not None else 0
+    for name, t, size in (("path", path, total), ("tokens", tokens, total), ("count", count, n), ("token", token, n)):
+        _check_ints(name, t, size)
+    if parent is not None:
+        _check_ints("parent", parent, total)
+    for name, t, size in (("u", u, total), ("u_next", u_next, n)):
+        if t.dtype is not _torch.float32 or t.shape != (size,) or not t.is_contiguous():
+            raise ValueError(f"{name}: need {size} contiguous float32")
+    _check_devices(path, count, token, p, q, tokens, start, u, u_next, parent)
+    _call("vla_verify_drafts_dev", path.data_ptr(), count.data_ptr(), token.data_ptr(), p.data_ptr(), ldp, _dp(q), ldq,
+          tokens.data_ptr(), _dp(parent), start.data_ptr(), u.data_ptr(), u_next.data_ptr(), n, total, vocab, dt, _stream(stream))
+
+
+def kv4_keep_dev(cache, n_kv, head_dim, page_size, table, lens, start, path, count, new_lens=None, stream=None):
+    """Keeps the accepted ones of each sequence's newest n tokens in the cache, in place: token lens[s] - n + path[i]
+    becomes token lens[s] - n + i for i < count[s] (verify_drafts_dev's); new_lens (not lens itself) takes the new lengths."""
+    pages, n, ld = _cache_shape(cache, n_kv, head_dim, page_size, table)
+    total = path.shape[0] if path.dim() == 1 else -1
+    for name, t, size in (("lens", lens, n), ("start", start, n + 1), ("path", path, total), ("count", count, n)):
+        _check_ints(name, t, size)
+    if new_lens is not None:
+        _check_ints("new_lens", new_lens, n)
+    _check_devices(cache, table, lens, start, path, count, new_lens)
+    _call("vla_kv4_keep_dev", cache.data_ptr(), pages, page_size, table.data_ptr(), ld, lens.data_ptr(), start.data_ptr(),
+          path.data_ptr(), count.data_ptr(), _dp(new_lens), n, total, n_kv, head_dim, _stream(stream))
 
 
 class LinearI8:

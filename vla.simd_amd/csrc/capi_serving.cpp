@@ -185,4 +185,158 @@ VLA_API int32_t vla_kv4_attention_dev(void* out, int64_t ldo, const void* Q, int
     });
 }
 
+VLA_API int32_t vla_draft_tree_dev(int32_t* pos, uint32_t* see, int32_t ld_see, const int32_t* parent, const int32_t* lens,
+                                   const int32_t* start, int32_t n_seqs, int32_t total, void* stream) {
+    return guarded("vla_draft_tree_dev", [&] {
+        DraftTreeArgs a{};
+        a.pos = pos;
+        a.see = see;
+        a.ld_see = ld_see;
+        a.parent = parent;
+        a.lens = lens;
+        a.start = start;
+        a.n_seqs = n_seqs;
+        a.total = total;
+        launch_draft_tree(a, as_stream(stream));
+    });
+}
+
+VLA_API int32_t vla_rope_freqs(double* freqs, double* magnitude, int32_t rot_dim, double base, int32_t scaling, double factor,
+                               double trained, double low, double high) {
+    return guarded("vla_rope_freqs", [&] {
+        VLA_REQUIRE(freqs && rot_dim >= 2 && rot_dim % 2 == 0 && rot_dim <= 1 << 20, "rope_freqs: rot_dim must be even, from 2 to 2^20");
+        VLA_REQUIRE(base > 0.0 && std::isfinite(base), "rope_freqs: base must be positive");
+        VLA_REQUIRE(scaling >= VLA_ROPE_PLAIN && scaling <= VLA_ROPE_PARTS, "rope_freqs: unknown scaling");
+        VLA_REQUIRE(scaling == VLA_ROPE_PLAIN || (factor >= 1.0 && std::isfinite(factor)), "rope_freqs: factor must be at least 1");
+        VLA_REQUIRE(scaling != VLA_ROPE_BASE || rot_dim > 2, "rope_freqs: a scaled base needs more than one pair");
+        VLA_REQUIRE(scaling != VLA_ROPE_PARTS || (trained > 0.0 && std::isfinite(trained) && low >= 0.0 && high > low && std::isfinite(high)),
+                    "rope_freqs: parts need a trained length and 0 <= low < high");
+        const double b = scaling == VLA_ROPE_BASE ? base * std::pow(factor, (double)rot_dim / (rot_dim - 2)) : base;
+        for (int i = 0; i < rot_dim / 2; i++) {
+            double f = std::pow(b, -2.0 * i / rot_dim);
+            if (scaling == VLA_ROPE_LINEAR) f /= factor;
+            if (scaling == VLA_ROPE_PARTS) {
+                const double turns = trained * f / (2.0 * M_PI), ramp = (turns - low) / (high - low);
+                const double keep = ramp < 0.0 ? 0.0 : ramp > 1.0 ? 1.0 : ramp;
+                f = f / factor + (f - f / factor) * keep;
+            }
+            freqs[i] = f;
+        }
+        if (magnitude) *magnitude = scaling == VLA_ROPE_PARTS ? 0.1 * std::log(factor) + 1.0 : 1.0;
+    });
+}
+
+VLA_API int32_t vla_rope_kv4_append_dev(void* q_out, int64_t ldqo, void* k_out, int64_t ldko, void* cache, int32_t n_pages,
+                                        int32_t page_size, const void* q, int64_t ldq, const void* K, int64_t ldk, const void* V,
+                                        int64_t ldv, const float* q_weight, const float* k_weight, float eps, const int32_t* pos,
+                                        const double* freqs, int32_t rot_dim, double magnitude, int32_t interleaved,
+                                        const int32_t* table, int32_t ld_table, const int32_t* lens, const int32_t* start,
+                                        int32_t n_seqs, int32_t total, int32_t n_q, int32_t n_kv, int32_t head_dim, int32_t dtype,
+                                        void* stream) {
+    return guarded("vla_rope_kv4_append_dev", [&] {
+        RopeAppendArgs a{};
+        // without a cache no token has a page
+        a.kv = cache_args(cache, cache ? n_pages : 0, cache ? page_size : kKv4Block, cache ? table : nullptr, cache ? ld_table : 0, n_seqs,
+                          n_kv, head_dim, dtype);
+        a.kv.K = const_cast<void*>(K);
+        a.kv.ldk = ldk;
+        a.kv.V = const_cast<void*>(V);
+        a.kv.ldv = ldv;
+        a.kv.lens = lens;
+        a.kv.start = start;
+        a.kv.total = total;
+        a.q = q;
+        a.ldq = ldq;
+        a.q_out = q_out;
+        a.ldqo = ldqo;
+        a.k_out = k_out;
+        a.ldko = ldko;
+        a.wq = q_weight;
+        a.wk = k_weight;
+        a.eps = eps;
+        a.pos = pos;
+        a.freqs = freqs;
+        a.rot = rot_dim;
+        a.magnitude = magnitude;
+        a.interleaved = interleaved != 0;
+        a.n_q = n_q;
+        launch_rope_kv4_append(a, as_stream(stream));
+    });
+}
+
+VLA_API int64_t vla_kv4_tree_attention_work_bytes(int32_t total_q, int32_t n_seqs, int32_t max_new, int32_t max_len, int32_t n_q,
+                                                  int32_t n_kv, int32_t head_dim) {
+    return (int64_t)kv4_tree_attention_work_bytes(total_q, n_seqs, max_new, max_len, n_q, n_kv, head_dim);
+}
+
+VLA_API int32_t vla_kv4_tree_attention_dev(void* out, int64_t ldo, const void* Q, int64_t ldq, const void* cache, int32_t n_pages,
+                                           int32_t page_size, const int32_t* table, int32_t ld_table, const int32_t* lens,
+                                           const int32_t* q_start, const uint32_t* see, int32_t ld_see, int32_t n_seqs,
+                                           int32_t total_q, int32_t max_new, int32_t max_len, int32_t n_q, int32_t n_kv,
+                                           int32_t head_dim, float scale, int32_t dtype, void* work, int64_t work_bytes,
+                                           void* stream) {
+    return guarded("vla_kv4_tree_attention_dev", [&] {
+        Kv4TreeArgs t{};
+        Kv4Args& a = t.kv;
+        a = cache_args(const_cast<void*>(cache), n_pages, page_size, table, ld_table, n_seqs, n_kv, head_dim, dtype);
+        a.lens = lens;
+        a.start = q_start;
+        a.total = total_q;
+        a.out = out;
+        a.ldo = ldo;
+        a.Q = Q;
+        a.ldq = ldq;
+        a.n_q = n_q;
+        a.max_new = max_new;
+        a.max_len = max_len;
+        a.scale = scale;
+        a.work = static_cast<float*>(work);
+        a.work_bytes = work_bytes > 0 ? (size_t)work_bytes : 0;
+        t.see = see;
+        t.ld_see = ld_see;
+        launch_kv4_tree_attention(t, as_stream(stream));
+    });
+}
+
+VLA_API int32_t vla_verify_drafts_dev(int32_t* path, int32_t* count, int32_t* token, const void* p, int64_t ldp, const void* q,
+                                      int64_t ldq, const int32_t* tokens, const int32_t* parent, const int32_t* start, const float* u,
+                                      const float* u_next, int32_t n_seqs, int32_t total, int32_t vocab, int32_t dtype, void* stream) {
+    return guarded("vla_verify_drafts_dev", [&] {
+        VerifyArgs a{};
+        a.path = path;
+        a.count = count;
+        a.token = token;
+        a.p = p;
+        a.ldp = ldp;
+        a.q = q;
+        a.ldq = ldq;
+        a.tokens = tokens;
+        a.parent = parent;
+        a.start = start;
+        a.u = u;
+        a.u_next = u_next;
+        a.n_seqs = n_seqs;
+        a.total = total;
+        a.vocab = vocab;
+        a.dtype = dtype;
+        launch_verify_drafts(a, as_stream(stream));
+    });
+}
+
+VLA_API int32_t vla_kv4_keep_dev(void* cache, int32_t n_pages, int32_t page_size, const int32_t* table, int32_t ld_table,
+                                 const int32_t* lens, const int32_t* start, const int32_t* path, const int32_t* count,
+                                 int32_t* new_lens, int32_t n_seqs, int32_t total, int32_t n_kv, int32_t head_dim, void* stream) {
+    return guarded("vla_kv4_keep_dev", [&] {
+        Kv4KeepArgs a{};
+        a.kv = cache_args(cache, n_pages, page_size, table, ld_table, n_seqs, n_kv, head_dim, kF32);
+        a.kv.lens = lens;
+        a.kv.start = start;
+        a.kv.total = total;
+        a.path = path;
+        a.count = count;
+        a.new_lens = new_lens;
+        launch_kv4_keep(a, as_stream(stream));
+    });
+}
+
 }  // extern "C"

@@ -76,6 +76,69 @@ void launch_kv4_gather(const Kv4Args& a, hipStream_t st);
 void launch_kv4_attention(const Kv4Args& a, hipStream_t st);
 size_t kv4_attention_work_bytes(int total_q, int n_seqs, int max_new, int max_len, int n_q, int n_kv, int head_dim);
 
+// kv4_tree.hip: the attention of drafted tokens (Kv4Args as for launch_kv4_attention)
+struct Kv4TreeArgs {
+    Kv4Args kv;
+    const uint32_t* see;  // [total] rows of ld_see words: bit t of a row's words, it sees new token t
+    int ld_see;
+};
+void launch_kv4_tree_attention(const Kv4TreeArgs& a, hipStream_t st);
+size_t kv4_tree_attention_work_bytes(int total_q, int n_seqs, int max_new, int max_len, int n_q, int n_kv, int head_dim);
+
+// rope_append.hip: norms and rotation of packed rows, keys and values into the cache
+struct RopeAppendArgs {
+    Kv4Args kv;          // K, V: the rows; cache null: only rotated
+    const void* q; int64_t ldq;
+    void* q_out; int64_t ldqo;
+    void* k_out; int64_t ldko;  // null: not wanted
+    const float* wq;     // [head_dim] or null: no norm
+    const float* wk;
+    float eps;
+    const int32_t* pos;  // [total] or null: a token's number in its sequence
+    const double* freqs; // [rot / 2] angles per position
+    int rot;             // values of a head that turn
+    double magnitude;
+    int interleaved;
+    int n_q;
+    int tokens_per_block;  // set by the launcher
+};
+void launch_rope_kv4_append(RopeAppendArgs a, hipStream_t st);
+
+// draft.hip
+struct DraftTreeArgs {
+    int32_t* pos;        // [total]
+    uint32_t* see;       // [total] rows of ld_see words
+    int ld_see;
+    const int32_t* parent;  // [total], in its sequence; null: the row before
+    const int32_t* lens;
+    const int32_t* start;
+    int n_seqs, total;
+};
+void launch_draft_tree(const DraftTreeArgs& a, hipStream_t st);
+
+struct VerifyArgs {
+    int32_t* path;       // [total]
+    int32_t* count;      // [n_seqs]
+    int32_t* token;      // [n_seqs]
+    const void* p; int64_t ldp;
+    const void* q; int64_t ldq;  // null: drafted with certainty
+    const int32_t* tokens;  // [total]
+    const int32_t* parent;  // [total], in its sequence; null: the row before
+    const int32_t* start;
+    const float* u;      // [total]
+    const float* u_next; // [n_seqs]
+    int n_seqs, total, vocab, dtype;
+};
+void launch_verify_drafts(const VerifyArgs& a, hipStream_t st);
+
+struct Kv4KeepArgs {
+    Kv4Args kv;
+    const int32_t* path;   // [total]
+    const int32_t* count;  // [n_seqs]
+    int32_t* new_lens;     // [n_seqs] or null
+};
+void launch_kv4_keep(const Kv4KeepArgs& a, hipStream_t st);
+
 #ifdef __HIPCC__
 
 typedef __bf16 bf16_t;
