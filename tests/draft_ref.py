@@ -51,11 +51,14 @@ def rotated(x, heads, hd, pos, freqs, magnitude, inter, w, eps):
 
 def attend(q, ks, vs, new, see, n_q, n_kv, hd, scale):
     """(out, bound): q [sum(new), n_q * hd]; ks, vs [len, n_kv, hd] cached values; see: per sequence [n, n] truth values
-    among the new tokens. Weights enter the product to 16 bits in 16-bit types (2^-15 of themselves), to 24 in fp32."""
+    among the new tokens. Weights enter the product to 24 bits in fp32, to 16 in fp16 (2^-15 of themselves). In bf16 they
+    may be fp16 numbers: rounded by half a step, eps / 2 = 2^-11 of themselves. In both 16-bit types a weight may be a subnormal
+    fp16 number: with the largest of its 64 neighbours at least 2^-16 of the row's, which stands at 2^9, that is off by half of
+    2^-24, which is 2^-34 of the row's largest and at most 2^-18 of the neighbours' largest, so of the row's."""
     G = n_q // n_kv
     out = torch.zeros(q.shape, dtype=torch.float64)
     bound = torch.zeros_like(out)
-    p_err = 0.0 if q.dtype == torch.float32 else 2.0 ** -15
+    p_err = {torch.float32: 0.0, torch.float16: 2.0 ** -15, torch.bfloat16: 2.0 ** -11}[q.dtype]
     at = 0
     for m, k, v, mine in zip(new, ks, vs, see):
         n = k.shape[0]
@@ -68,6 +71,10 @@ def attend(q, ks, vs, new, see, n_q, n_kv, hd, scale):
             o, b = ref.softmax_rows(q[at:at + m, cols].double(), k[:, h // G], v[:, h // G], full, scale, p_err)
             out[at:at + m, cols] = o
             bound[at:at + m, cols] = b + ref.rounding(o, q.dtype)
+            if q.dtype != torch.float32 and n:
+                z = torch.where(full, q[at:at + m, cols].double() @ k[:, h // G].T * scale, -math.inf)
+                top = torch.softmax(z, 1).nan_to_num(0.0).amax(1, keepdim=True)
+                bound[at:at + m, cols] += 2.0 ** -18 * top * v[:, h // G].abs().sum(0)
         at += m
     return out, bound
 

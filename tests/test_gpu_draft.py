@@ -316,11 +316,13 @@ def test_tree_attention_split_keys(vla, dtype, lens, new, n_q, n_kv, hd, page):
 
 
 def test_tree_attention_of_a_chain_is_causal(vla):
-    """A chain's bits give the attention of a causal chunk: the same keys, the same bounds."""
+    """A chain's bits give the attention of a causal chunk."""
     lens, new, n_q, n_kv, hd, page = [300, 40], [33, 40], 8, 2, 64, 64
     q, cache, table, ks, vs = _decode_case(vla, lens, new, n_q, n_kv, hd, page, BF16, seed=3)
-    _, see = _masks(new, 0, 1)
-    want, bound = ref.decode(q, ks, vs, new, n_q, n_kv, hd, 0.125)
+    truth, see = _masks(new, 0, 1)
+    want, _ = ref.decode(q, ks, vs, new, n_q, n_kv, hd, 0.125)
+    same, bound = dref.attend(q, ks, vs, new, truth, n_q, n_kv, hd, 0.125)
+    assert float((want - same).abs().max()) < 1e-12
     ref.within(_attend(vla, q, cache, table, lens, new, see, n_q, n_kv, hd, page, 0.125), want, bound)
 
 
@@ -411,6 +413,78 @@ def test_tree_attention_large_values(vla, dtype, hd):
     want, bound = dref.attend(q, ks, [v], new, truth, 2, 1, hd, 0.1)
     for kw in (dict(), dict(max_len=1 << 20)):
         ref.within(_attend(vla, q, c, table, lens, new, see, 2, 1, hd, page, 0.1, **kw), want, bound, str(kw))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 192, 256])
+@pytest.mark.parametrize("shift,where", [(-40, "early"), (-40, "late"), (25, "late"), (-95, "all"), (90, "all"), (-22, "all"), (8, "all"), (-100, "zero")])
+def test_tree_attention_of_any_magnitude(vla, dtype, hd, shift, where):
+    """Keys' and values' blocks of other magnitudes than fp16 takes, from the first tile on, from a later one, or in all: the
+    results keep their bits whatever form the products take."""
+    n_q, n_kv, page, n, m = 8, 1, 32, 500, 40
+    q, cache, table, ks, vs = _decode_case(vla, [n], [m], n_q, n_kv, hd, page, dtype, seed=hd)
+    c, row = cache.cpu(), table.cpu().numpy()[0]
+    v, k, at = vs[0].clone(), ks[0].clone(), lambda t, part: vla.kv4_offset(row, n_kv, hd, page, c.shape[0], t, part, 0, hd // 32 - 1)
+    cols = slice(hd - 32, hd)
+    for t in {"early": [3], "late": range(300, 310), "all": range(n), "zero": range(0, n, 7)}[where]:
+        for part, x in ((2, k), (3, v)):
+            if part == 2 and shift > 0:
+                continue  # (keys that large would leave one weight)
+            byte = int(c.view(-1)[at(t, part)])
+            if where == "zero":  # zeros of the smallest exponent count for nothing
+                lo = at(t, part - 2)
+                c.view(-1)[lo:lo + 16] = 0
+                new, x[t, :, cols] = 27, 0.0
+            else:
+                new = max(27, byte + shift)
+                x[t, :, cols] *= 2.0 ** (new - byte)
+            c.view(-1)[at(t, part)] = new
+    truth, see = _masks([m], 4, 7)
+    want, bound = dref.attend(q, [k], [v], [m], truth, n_q, n_kv, hd, hd ** -0.5)
+    for kw in (dict(), dict(max_len=1 << 20), dict(split=False)):
+        got = _attend(vla, q, c.to(DEV), table, [n], [m], see, n_q, n_kv, hd, page, hd ** -0.5, **kw).double().cpu()
+        # results past the type's range round to infinity, and may from where the bound reaches it
+        top = torch.finfo(dtype).max
+        over = (want.abs() + bound > top) & got.isinf() & (got.sign() == want.sign())
+        assert bool(got[want.abs() - bound > top * (1 + ref.half(dtype))].isinf().all())
+        ref.within(torch.where(over, want, got), want, bound, str(kw))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("below", [12, 17, 22, 30])
+@pytest.mark.parametrize("m", [3, 40])
+def test_tree_attention_sink(vla, dtype, hd, below, m):
+    """One key takes nearly all of every row's weight and has the value zero: the others' small weights keep their bits."""
+    n_q, n_kv, page, n = 4, 1, 64, 2000
+    q, cache, table, ks, vs = _decode_case(vla, [n], [m], n_q, n_kv, hd, page, dtype, seed=below)
+    c, row = cache.cpu(), table.cpu().numpy()[0]
+    q = torch.zeros_like(q)
+    q[:, ::hd] = 1.0  # a row's score is its key's first value
+    k, v = ks[0].clone(), vs[0].clone()
+    k[0, 0, 0], v[0] = 4.0, 0.0
+    scale = below / 4.0
+    for t in range(n):
+        lo = vla.kv4_offset(row, n_kv, hd, page, c.shape[0], t, 0, 0, 0)
+        sc = vla.kv4_offset(row, n_kv, hd, page, c.shape[0], t, 2, 0, 0)
+        c.view(-1)[lo:lo + 16] = 0
+        c.view(-1)[lo] = 6 if t == 0 else 0  # 4 * 2^0, others 0
+        c.view(-1)[sc] = 127
+        k[t, 0, :32] = 0.0
+        k[t, 0, 0] = 4.0 if t == 0 else 0.0
+    for b in range(hd // 32):
+        lo = vla.kv4_offset(row, n_kv, hd, page, c.shape[0], 0, 1, 0, b)
+        c.view(-1)[lo:lo + 16] = 0
+    truth, see = _masks([m], 3, 7)
+    want, bound = dref.attend(q, [k], [v], [m], truth, n_q, n_kv, hd, scale)
+    # keys of the sink's own 64 lose at most 2^-18 of it, as the bound says; all others 2^-18 of their own largest, which is theirs
+    w = math.exp(-below) / (1 + (n - 1) * math.exp(-below))
+    tight = want.abs() * ref.half(dtype) + torch.finfo(dtype).smallest_normal * ref.half(dtype) \
+        + v[:, 0].abs().sum(0).repeat(n_q) * w * (2.0 ** -11 + 64 * ref.U * below) + v[:64, 0].abs().sum(0).repeat(n_q) * 2.0 ** -18 / (1 + n * math.exp(-below)) \
+        + v[:, 0].abs().sum(0).repeat(n_q) * w * (n + 24) * ref.U
+    for kw in (dict(), dict(max_len=1 << 20)):
+        got = _attend(vla, q, c.to(DEV), table, [n], [m], see, n_q, n_kv, hd, page, scale, **kw)
+        ref.within(got, want, torch.minimum(bound, tight), str(kw))
 
 
 def test_tree_attention_many_sequences(vla):
