@@ -22,22 +22,13 @@ __device__ __forceinline__ Nodes nodes_of(const int32_t* start, int s, int total
 }
 
 // ---------------------------------------------------------------- tree ----
-// depth and bits of row i: those of its parent, and its own. A thread walks from its row up
-// to the root, whose numbers fall, so it writes its words from the last to the first. Latency bounds it
-// (a walk's steps depend on each other); the parents of a block's rows are in LDS.
-__global__ __launch_bounds__(256) void draft_tree_kernel(DraftTreeArgs a) {
-    __shared__ int32_t up[256];
-    const int row0 = blockIdx.x * 256, row = row0 + threadIdx.x;
-    if (a.parent) {
-        up[threadIdx.x] = row < a.total ? a.parent[row] : -1;
-        __syncthreads();
-    }
-    if (row >= a.total) return;
-    const int s = seq_of_row(a.start, a.n_seqs, row);
-    if (s >= a.n_seqs) return;
-    const Nodes nd = nodes_of(a.start, s, a.total);
-    if (row < nd.first || row >= nd.first + nd.n) return;
-    const int i = row - nd.first;
+// depth and bits of row i: those of its parent, and its own. Latency bounds it.
+
+// Row i of a sequence by a walk up to its root. Numbers fall on the way, so its words are
+// written from the last to the first. up(at): the parent of row `at` as given.
+template <class F>
+__device__ __forceinline__ void walk_up(const DraftTreeArgs& a, const Nodes& nd, int s, int i, F&& up) {
+    const int row = nd.first + i;
     uint32_t* see = a.see + (int64_t)row * a.ld_see;
     for (int w = a.ld_see - 1; w > i >> 5; w--) see[w] = 0;
     int depth = 0, w = i >> 5;
@@ -48,11 +39,7 @@ __global__ __launch_bounds__(256) void draft_tree_kernel(DraftTreeArgs a) {
             bits = 0;
         }
         bits |= 1u << (at & 31);
-        int p = at - 1;
-        if (a.parent) {
-            const int r = nd.first + at;
-            p = r >= row0 ? up[r - row0] : a.parent[r];
-        }
+        const int p = up(at);
         if (p < 0 || p >= at) break;
         at = p;
         depth++;
@@ -62,6 +49,60 @@ __global__ __launch_bounds__(256) void draft_tree_kernel(DraftTreeArgs a) {
         bits = 0;
     }
     a.pos[row] = (int)((unsigned)a.lens[s] - (unsigned)nd.n + (unsigned)depth);
+}
+
+// A thread for each row; the parents of a block's rows are in LDS.
+__global__ __launch_bounds__(256) void draft_tree_rows_kernel(DraftTreeArgs a) {
+    __shared__ int32_t parent[256];
+    const int row0 = blockIdx.x * 256, row = row0 + threadIdx.x;
+    if (a.parent) {
+        parent[threadIdx.x] = row < a.total ? a.parent[row] : -1;
+        __syncthreads();
+    }
+    if (row >= a.total) return;
+    const int s = seq_of_row(a.start, a.n_seqs, row);
+    if (s >= a.n_seqs) return;
+    const Nodes nd = nodes_of(a.start, s, a.total);
+    if (row < nd.first || row >= nd.first + nd.n) return;
+    walk_up(a, nd, s, row - nd.first, [&](int at) {
+        if (!a.parent) return at - 1;
+        const int r = nd.first + at;
+        return r >= row0 ? parent[r - row0] : a.parent[r];
+    });
+}
+
+// A wave for each sequence: up to 64 rows take as many steps as the depth has bits, each joining a row's bits and depth with those of
+// the row that it has got to. (256 trees of 64 rows 2.6 us, by walks 5.4; as many chains 2.8 and 13.7.)
+__global__ __launch_bounds__(64) void draft_tree_wave_kernel(DraftTreeArgs a) {
+    const int lane = threadIdx.x;
+    for (int s = blockIdx.x; s < a.n_seqs; s += gridDim.x) {
+        const Nodes nd = nodes_of(a.start, s, a.total);
+        if (nd.n > 64) {
+            for (int i = lane; i < nd.n; i += 64) walk_up(a, nd, s, i, [&](int at) { return a.parent ? a.parent[nd.first + at] : at - 1; });
+            continue;
+        }
+        int up = lane < nd.n ? a.parent ? a.parent[nd.first + lane] : lane - 1 : -1;
+        up = up >= 0 && up < lane ? up : -1;
+        uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
+        int depth = up >= 0;
+        while (__any(up >= 0)) {
+            const int from = up >= 0 ? up : lane;
+            const uint32_t l = __shfl(lo, from), h = __shfl(hi, from);
+            const int d = __shfl(depth, from), u = __shfl(up, from);
+            if (up >= 0) {
+                lo |= l;
+                hi |= h;
+                depth += d;
+                up = u;
+            }
+        }
+        if (lane >= nd.n) continue;
+        uint32_t* see = a.see + (int64_t)(nd.first + lane) * a.ld_see;
+        see[0] = lo;
+        if (a.ld_see > 1) see[1] = hi;
+        for (int w = 2; w < a.ld_see; w++) see[w] = 0;
+        a.pos[nd.first + lane] = (int)((unsigned)a.lens[s] - (unsigned)nd.n + (unsigned)depth);
+    }
 }
 
 // -------------------------------------------------------------- verify ----
@@ -75,11 +116,15 @@ __global__ __launch_bounds__(256) void draft_tree_kernel(DraftTreeArgs a) {
 // all of them, and the rows are never written.
 //
 // Sums are of 64 bits, so that their order moves a result only where a random number lies
-// within 2^-50 of a border.
+// within 2^-50 of a border. A block takes a sequence. Children in front of the first refusal
+// need two probabilities each; every refusal with q, and the draw, go through rows of the vocabulary. What bounds that
+// are the 64-bit instructions, five a value (49280 values of fp32 or of bf16: 3.3 us a time, 120 GB/s of a CU); a chain of four
+// drafted tokens over them takes 14.6 us, 48 trees of 32 take 36, the time of the tree with most refusals.
+// (Loading six chunks ahead for four changes nothing; more blocks to a sequence would have to wait for each other.)
 constexpr int kVerifyNodes = 512;   // probabilities held in LDS
 constexpr int kVerifyThreads = 1024;
 
-__device__ __forceinline__ double above_zero(double x) { return x > 0.0 ? x : 0.0; }  // (0 for NaN)
+__device__ __forceinline__ double above_zero(double x) { return fmax(x, 0.0); }  // (0 for NaN)
 
 template <class T>
 __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
@@ -158,7 +203,11 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
     // those kept and refused never need more.
     int n_refused = 0;
     auto refused_at = [&](int j) { return j < kVerifyNodes ? refused[j] : path[n - 1 - (j - kVerifyNodes)]; };
-    auto drop = [&](int v, double (&w)[VEC]) {  // the refused tokens among them
+    // (A lane holds the one of its number among the first 64, so that a chunk without any is seen at once.)
+    int held = -1;
+    auto drop = [&](int v, double (&w)[VEC]) {
+        const int at = v - lane * VEC;
+        if (n_refused <= 64 && !__any(held >= at && held < at + chunk)) return;
         for (int i = 0; i < n_refused; i++) {
             const int t = refused_at(i);
 #pragma unroll
@@ -167,17 +216,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
         }
     };
     int turn = 0;
-    // the sum of what is left, the same bits in every thread; sums[turn] holds the waves' parts
-    auto total_of = [&](double coef) {
-        double sum = 0.0;
-        const int begin = wave * share - phase, end = begin + share < V ? begin + share : V;
-        for (int v = begin + lane * VEC; v < end; v += chunk) {
-            double w[VEC];
-            weights(v, coef, w);
-            if (n_refused) drop(v, w);
-#pragma unroll
-            for (int e = 0; e < VEC; e++) sum += w[e];
-        }
+    // the sums of the waves, the same bits in every thread; they stay in sums[turn]
+    auto all_of = [&](double sum) {
         sum = wave_sum_f64(sum);
         turn ^= 1;
         if (lane == 0) sums[turn][wave] = sum;
@@ -185,6 +225,31 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
         double all = 0.0;
         for (int i = 0; i < W; i++) all += sums[turn][i];
         return all;
+    };
+    auto sum_of = [&](int v0, double coef) {  // of a lane's values of the chunk at v0, which all lanes go through
+        const int v = v0 + lane * VEC;
+        double w[VEC], sum = 0.0;
+        weights(v, coef, w);
+        if (n_refused) drop(v, w);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) sum += w[e];
+        return sum;
+    };
+    // the sum of what is left (some chunks at a time, so that their loads are under way together)
+    auto total_of = [&](double coef) {
+        constexpr int U = 16 / VEC;
+        const int begin = wave * share - phase, end = begin + share < V ? begin + share : V;
+        double sum = 0.0;
+        int v = begin;
+        for (; v + (U - 1) * chunk < end; v += U * chunk) {
+            double part[U];
+#pragma unroll
+            for (int i = 0; i < U; i++) part[i] = sum_of(v + i * chunk, coef);
+#pragma unroll
+            for (int i = 0; i < U; i++) sum += part[i];
+        }
+        for (; v < end; v += chunk) sum += sum_of(v, coef);
+        return all_of(sum);
     };
 
     int node = 0, kept = 1;
@@ -223,6 +288,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
                 S = 1.0;
                 known = false;
                 n_refused = 0;
+                held = -1;
             } else if (Q) {
                 coef += S;
                 S = total_of(coef);
@@ -235,6 +301,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
                 S -= pi;
                 __syncthreads();
                 if (tid == 0) (n_refused < kVerifyNodes ? refused[n_refused] : path[n - 1 - (n_refused - kVerifyNodes)]) = t;
+                if (lane == n_refused) held = t;
                 n_refused++;
                 __syncthreads();
             }
@@ -245,59 +312,72 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
     if (!known) S = total_of(coef);
     if (!(S > 0.0)) {
         n_refused = 0;
+        held = -1;
         coef = 0.0;
         S = total_of(0.0);
     }
     const double want = fmax((double)a.u_next[s], 0.0) * S;
+    // The part that holds it, or the last with any weight where rounding leaves none; `before`: what lies in front of it.
+    auto pick = [&](double& before) {
+        int at = -1, last = -1;
+        double front = before;
+        for (int i = 0; i < W; i++) {
+            const double x = sums[turn][i];
+            if (at < 0 && x > 0.0) {
+                last = i;
+                before = front;
+                if (front + x > want) at = i;
+            }
+            front += x;
+        }
+        return at >= 0 ? at : last;
+    };
+    // first the wave's share, then, with all waves on that share, a 16th of it, which its wave goes through
     double before = 0.0;
-    int w0 = -1, last = -1;  // the wave whose share holds it, and the last one with any weight
-    for (int i = 0; i < W; i++) {
-        const double x = sums[turn][i];
-        if (x > 0.0) last = i;
-        if (w0 < 0 && before + x > want) w0 = i;
-        if (w0 < 0) before += x;
-    }
-    if (wave == (w0 >= 0 ? w0 : last)) {
-        int best = -1, some = -1;  // the first value past `want`, the last with weight
-        const int begin = wave * share - phase, end = begin + share < V ? begin + share : V;
-        for (int v0 = begin; v0 < end && best < 0; v0 += chunk) {
-            const int v = v0 + lane * VEC;
-            double w[VEC], sum = 0.0;
-            weights(v, coef, w);
-            if (n_refused) drop(v, w);
-            int mine = -1;
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                sum += w[e];
-                if (w[e] > 0.0) mine = v + e;
-            }
-            double incl = sum;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const double o = __shfl_up(incl, d);
-                if (lane >= d) incl += o;
-            }
-            const unsigned long long has = __ballot(mine >= 0);
-            if (has) some = __builtin_amdgcn_readlane(mine, 63 - __clzll(has));
-            const unsigned long long over = __ballot(before + incl > want);
-            if (over && w0 >= 0) {
-                const int l = __ffsll(over) - 1;
-                double at = before + (incl - sum);
-                int pick = mine;
-                bool done = false;
+    const int outer = pick(before);
+    if (outer >= 0) {
+        const int part = (share / chunk + W - 1) / W * chunk;
+        const int first = outer * share - phase, stop = first + share < V ? first + share : V;
+        const int begin = first + wave * part, end = begin + part < stop ? begin + part : stop;
+        double sum = 0.0;
+        for (int v = begin; v < end; v += chunk) sum += sum_of(v, coef);
+        all_of(sum);
+        const int inner = pick(before);
+        if (wave == inner) {
+            int best = -1, some = -1;  // the first value past `want`, the last with weight
+            for (int v0 = begin; v0 < end && best < 0; v0 += chunk) {
+                const int v = v0 + lane * VEC;
+                double w[VEC], mass = 0.0;
+                weights(v, coef, w);
+                if (n_refused) drop(v, w);
+                int mine = -1;
 #pragma unroll
                 for (int e = 0; e < VEC; e++) {
-                    at += w[e];
-                    if (!done && at > want && w[e] > 0.0) {
-                        pick = v + e;
-                        done = true;
-                    }
+                    mass += w[e];
+                    if (w[e] > 0.0) mine = v + e;
                 }
-                best = __builtin_amdgcn_readlane(pick, l);
+                double incl = mass;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const double o = __shfl_up(incl, d);
+                    if (lane >= d) incl += o;
+                }
+                const unsigned long long has = __ballot(mine >= 0), over = __ballot(mine >= 0 && before + incl > want);
+                if (has) some = __builtin_amdgcn_readlane(mine, 63 - __clzll(has));
+                if (over) {
+                    double at = before + (incl - mass);
+                    int choice = -1;
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) {
+                        at += w[e];
+                        if (choice < 0 && at > want && w[e] > 0.0) choice = v + e;
+                    }
+                    best = __builtin_amdgcn_readlane(choice < 0 ? mine : choice, __ffsll(over) - 1);
+                }
+                before += __shfl(incl, 63);
             }
-            before += __shfl(incl, 63);
+            if (lane == 0) found = best >= 0 ? best : some;
         }
-        if (lane == 0) found = best >= 0 ? best : some;
     }
     __syncthreads();
     for (int i = kept + tid; i < n; i += kVerifyThreads) path[i] = -1;
@@ -346,18 +426,19 @@ __global__ __launch_bounds__(kKeepThreads) void kv4_keep_kernel(Kv4KeepArgs k) {
         const int i = i0 + tt;
         const bool on = tt < per && i < count;
         const int from = on ? k.path[nd.first + i] : 0;
-        const bool moves = on && from != i;
+        uint8_t *codes = nullptr, *scale = nullptr, *codes_to = nullptr, *scale_to = nullptr;
+        const bool to = on && place(base + i, codes_to, scale_to);  // (looked up while the path is on its way)
+        const bool moves = to && from != i;
         Codes16 c{};
         int byte = kKv4NanByte;  // a token without a page reads as NaN
-        uint8_t *codes = nullptr, *scale = nullptr;
         if (moves && place(base + from, codes, scale)) {
             c = *reinterpret_cast<const Codes16*>(codes);
             byte = *scale;
         }
         __syncthreads();
-        if (moves && place(base + i, codes, scale)) {
-            *reinterpret_cast<Codes16*>(codes) = c;
-            *scale = (uint8_t)byte;
+        if (moves) {
+            *reinterpret_cast<Codes16*>(codes_to) = c;
+            *scale_to = (uint8_t)byte;
         }
         __syncthreads();
     }
@@ -370,7 +451,9 @@ void launch_draft_tree(const DraftTreeArgs& a, hipStream_t st) {
     VLA_REQUIRE(a.ld_see >= 1 && a.ld_see <= 1 << 20, "draft_tree: rows of 1 to 2^20 words");
     if (a.n_seqs == 0 || a.total == 0) return;
     VLA_REQUIRE(a.pos && a.see && a.lens && a.start, "draft_tree: null buffer");
-    draft_tree_kernel<<<(a.total + 255) / 256, 256, 0, st>>>(a);
+    // a wave for each sequence where they are small on average
+    if (a.total <= (int64_t)64 * a.n_seqs) draft_tree_wave_kernel<<<a.n_seqs < 1 << 20 ? a.n_seqs : 1 << 20, 64, 0, st>>>(a);
+    else draft_tree_rows_kernel<<<(a.total + 255) / 256, 256, 0, st>>>(a);
     VLA_LAUNCH_CHECK();
 }
 
