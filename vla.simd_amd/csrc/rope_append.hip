@@ -12,12 +12,14 @@
 // are normed and turned in 64 bits and quantized from there: a code then is the nearest of
 // the exact value but where that lies within 2^-40 or so of a border. A result is rounded once.
 //
-// HBM bounds it. A block takes a few tokens and fills a table of their sines and cosines in
+// Few rows are bound by latency (the chain from the offsets to the table, the sines, a store: 5.5 us), many by HBM and by the lanes'
+// own work on heads, norms in 64 bits above all: FIGS. A block takes a few tokens and fills a table of their sines and cosines in
 // LDS, the same for all heads. A group of lanes stays with one token, a lane with 16 bytes of a row
 // at the same place of every head, so that it keeps its sines and cosines in registers. The other
 // value of a pair is another lane's of the group where pairs are halves.
 
 #include "kv4_device.h"
+#include "wave.h"
 
 #include <cmath>
 
@@ -27,6 +29,7 @@ namespace {
 
 constexpr int kMaxTokens = 16;   // of a block
 constexpr int kTableEntries = 1024;
+constexpr int kCus = 256;
 
 // d for a later rounding to fewer bits than an fp32 has: cut off, the last bit set where anything
 // was lost. Past fp32's range it is infinite.
@@ -43,6 +46,41 @@ __device__ __forceinline__ T round_once(double d) {
     else return (T)to_odd(d);
 }
 
+// 16 bytes of a row
+struct alignas(16) Words {
+    unsigned w[4];
+};
+
+template <class T>
+__device__ __forceinline__ float value_of(const Words& x, int e) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(x.w[e]);
+    else return to_f32(__builtin_bit_cast(T, (unsigned short)(x.w[e >> 1] >> (16 * (e & 1)))));
+}
+
+// 1 / sqrt(x) to the last bits of a double: the hardware's number and two steps of Newton's
+__device__ __forceinline__ double rsqrt_wide(double x) {
+    double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+    for (int i = 0; i < 2; i++) y = y * fma(-0.5 * x * y, y, 1.5);
+    return y;
+}
+
+// Sums over the lp lanes of a group, a power of two, in all of them: by lane permutations of the vector ALU.
+template <class F>
+__device__ __forceinline__ F group_sum(F x, int lp) {
+    auto step = [&]<int CTRL>() {
+        if constexpr (sizeof(F) == 8) x += dpp_f64<CTRL, 0xf>(0.0, x);
+        else x += dpp_f32<CTRL, 0xf>(0.0f, x);
+    };
+    if (lp > 1) step.template operator()<0xb1>();   // quad_perm [1,0,3,2]
+    if (lp > 2) step.template operator()<0x4e>();   // quad_perm [2,3,0,1]
+    if (lp > 4) step.template operator()<0x141>();  // row_half_mirror
+    if (lp > 8) step.template operator()<0x140>();  // row_mirror
+    if (lp > 16) x += __shfl_xor(x, 16);
+    if (lp > 32) x += __shfl_xor(x, 32);
+    return x;
+}
+
 template <class T, bool INTER>
 __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int lp) {
     constexpr int EPL = RowGeo<T>::EPL;
@@ -53,91 +91,156 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int 
     const int tb = a.tokens_per_block, t0 = blockIdx.x * tb;
     const int nt = c.total - t0 < tb ? c.total - t0 : tb;
     const int half = a.rot >> 1, hd = c.head_dim;
-    locate_rows(c, t0, nt, false, starts, place);
-
-    for (int idx = threadIdx.x; idx < nt * half; idx += 256) {
-        const int tt = idx / half, i = idx - tt * half;
-        int p;
-        if (a.pos) {
-            p = a.pos[t0 + tt];
-        } else {  // its number in its sequence
-            const int s = place[tt].seq;
-            p = s < 0 ? 0 : c.lens[s] - (c.start[s + 1] - c.start[s]) + (t0 + tt - c.start[s]);
-        }
-        double sn, co;
-        sincos((double)p * a.freqs[i], &sn, &co);
-        cs[idx] = make_double2(co * a.magnitude, sn * a.magnitude);
-    }
-    __syncthreads();
-
     const int group = threadIdx.x / lp, ln = threadIdx.x & (lp - 1);
-    const int tt = group % tb, step = 256 / lp / tb;
-    const int i0 = ln * EPL;
-    const bool on = i0 < hd && tt < nt && place[tt].seq >= 0;  // (rows behind the last sequence are left as they are)
-    const Where w = place[tt < nt ? tt : 0];
-    // this lane's sines and cosines: 1 and 0 behind the part that turns; the sign is that of b's share
-    double co[EPL], si[EPL];
+    const int tt = group % tb, i0 = ln * EPL;
+    const bool in = i0 < hd && tt < nt;
+    const size_t t = t0 + (tt < nt ? tt : 0);
+    const int step = gridDim.y * (256 / lp / tb);
+    int h = blockIdx.y * (256 / lp / tb) + group / tb;
+    // a row's 16 bytes of query, key or value head h
+    auto row = [&](int h) -> Words {
+        const T* src = h < a.n_q ? static_cast<const T*>(a.q) + t * a.ldq + h * hd
+                     : h < a.n_q + c.n_kv ? static_cast<const T*>(c.K) + t * c.ldk + (h - a.n_q) * hd
+                                          : static_cast<const T*>(c.V) + t * c.ldv + (h - a.n_q - c.n_kv) * hd;
+        return *reinterpret_cast<const Words*>(src + i0);
+    };
+    const int n_all = a.n_q + c.n_kv + (c.cache ? c.n_kv : 0);
+    Words x{};  // the first one is on its way while the table is filled
+    if (in && h < n_all) x = row(h);
+
+    auto fill = [&] {
+        for (int idx = threadIdx.x; idx < nt * half; idx += 256) {
+            const int k = idx / half, i = idx - k * half;
+            int p;
+            if (a.pos) {
+                p = a.pos[t0 + k];
+            } else {  // its number in its sequence
+                const int s = place[k].seq;
+                p = s < 0 ? 0 : c.lens[s] - (c.start[s + 1] - c.start[s]) + (t0 + k - c.start[s]);
+            }
+            double sn, co;
+            sincos((double)p * a.freqs[i], &sn, &co);
+            cs[idx] = make_double2(co * a.magnitude, sn * a.magnitude);
+        }
+    };
+    if (a.pos) fill();
+    locate_rows(c, t0, nt, false, starts, place);
+    if (!a.pos) {
+        fill();
+        __syncthreads();
+    }
+    const Where where = place[tt < nt ? tt : 0];
+    const bool on = in && where.seq >= 0;  // (rows behind the last sequence are left as they are)
+    // This lane's sines and cosines, 1 and 0 behind the part that turns; the sine's sign is that of the other value's share.
+    auto angles = [&]<class F>(F (&co)[EPL], F (&si)[EPL]) {
 #pragma unroll
-    for (int e = 0; e < EPL; e++) {
-        const int v = i0 + e;
-        co[e] = 1.0;
-        si[e] = 0.0;
-        if (on && v < a.rot) {
-            const int pair = INTER ? v >> 1 : v < half ? v : v - half;
-            const bool second = INTER ? v & 1 : v >= half;
-            const double2 z = cs[tt * half + pair];
-            co[e] = z.x;
-            si[e] = second ? z.y : -z.y;
+        for (int e = 0; e < EPL; e++) {
+            const int v = i0 + e;
+            co[e] = 1;
+            si[e] = 0;
+            if (on && v < a.rot) {
+                const int pair = INTER ? v >> 1 : v < half ? v : v - half;
+                const bool second = INTER ? v & 1 : v >= half;
+                const double2 z = cs[tt * half + pair];
+                co[e] = (F)z.x;
+                si[e] = (F)(second ? z.y : -z.y);
+            }
+        }
+    };
+    // Where the other values of the lane's pairs are: of halves, four neighbours belong to four neighbours of one lane, in the same
+    // half of it or (odd) the other. Behind the part that turns they are not used.
+    const int d = half >> 2;  // fours between them
+    const bool odd = EPL == 8 && (d & 1);
+    int from[EPL / 4], other[EPL / 4];  // the lane, and the first of the other values, for the weights
+#pragma unroll
+    for (int j = 0; j < EPL / 4; j++) {
+        const int g = ln * (EPL / 4) + j, o = g < d ? g + d : g < 2 * d ? g - d : g;
+        from[j] = (threadIdx.x & 63 & ~(lp - 1)) + o / (EPL / 4);
+        other[j] = 4 * o;
+    }
+    auto others = [&](const Words& x) {
+        Words z;
+        if constexpr (INTER) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) z.w[i] = EPL == 8 ? __builtin_amdgcn_alignbit(x.w[i], x.w[i], 16) : x.w[i ^ 1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (EPL == 4) z.w[i] = __shfl(x.w[i], from[0]);
+                else z.w[i] = __shfl(odd ? x.w[i ^ 2] : x.w[i], from[i >> 1]);
+            }
+        }
+        return z;
+    };
+    // the norm's weights of the lane's values and of the others
+    auto weights = [&](const float* w, float (&mine)[EPL], float (&theirs)[EPL]) {
+#pragma unroll
+        for (int e = 0; e < EPL; e++) {
+            mine[e] = w && on ? w[i0 + e] : 1.0f;
+            theirs[e] = w && on ? w[INTER ? i0 + (e ^ 1) : other[e >> 2] + (e & 3)] : 1.0f;
+        }
+    };
+
+    // (a head's load is under way while the one before it is worked on; lanes without a row keep what they have)
+    auto take = [&] {
+        const Words now = x;
+        if (in && h + step < n_all) x = row(h + step);
+        return now;
+    };
+    if (h < a.n_q) {  // queries, in 32 bits
+        float cf[EPL], sf[EPL], wy[EPL], wz[EPL];
+        weights(a.wq, wy, wz);
+        angles(cf, sf);
+        T* dst = static_cast<T*>(a.q_out) + t * a.ldqo + i0;
+        const float inv_hd = 1.0f / (float)hd;
+        for (; h < a.n_q; h += step) {
+            const Words x = take(), xo = others(x);
+            float y[EPL], z[EPL];
+#pragma unroll
+            for (int e = 0; e < EPL; e++) y[e] = value_of<T>(x, e), z[e] = value_of<T>(xo, e);
+            if (a.wq) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < EPL; e++) sum += y[e] * y[e];
+                const float mean = group_sum(sum, lp) * inv_hd + a.eps;
+                if (mean > 1e-30f && mean < 1e30f) {
+                    const float r = rsqrtf(mean);
+#pragma unroll
+                    for (int e = 0; e < EPL; e++) y[e] = y[e] * r * wy[e], z[e] = z[e] * r * wz[e];
+                } else {  // the squares leave fp32's range, or are about to
+                    double wide = 0.0;
+#pragma unroll
+                    for (int e = 0; e < EPL; e++) wide += (double)y[e] * y[e];
+                    const double r = 1.0 / sqrt(group_sum(wide, lp) / hd + a.eps);
+#pragma unroll
+                    for (int e = 0; e < EPL; e++) y[e] = (float)(y[e] * r) * wy[e], z[e] = (float)(z[e] * r) * wz[e];
+                }
+            }
+            Pack<T, EPL> out;
+#pragma unroll
+            for (int e = 0; e < EPL; e++) out.v[e] = (T)(i0 + e < a.rot ? fmaf(cf[e], y[e], sf[e] * z[e]) : y[e]);
+            if (on) *reinterpret_cast<Pack<T, EPL>*>(dst + h * hd) = out;
         }
     }
-    const size_t t = t0 + tt;
-    const int nh = a.n_q + c.n_kv + (c.cache ? c.n_kv : 0);
-    for (int h = blockIdx.y * step + group / tb; h < nh; h += gridDim.y * step) {
-        const int kind = h < a.n_q ? 0 : h < a.n_q + c.n_kv ? 1 : 2;  // query, key, value
-        const int head = kind == 0 ? h : kind == 1 ? h - a.n_q : h - a.n_q - c.n_kv;
-        const T* src = kind == 0 ? static_cast<const T*>(a.q) + t * a.ldq
-                     : kind == 1 ? static_cast<const T*>(c.K) + t * c.ldk : static_cast<const T*>(c.V) + t * c.ldv;
-        Pack<T, EPL> x{};
-        if (on) x = *reinterpret_cast<const Pack<T, EPL>*>(src + head * hd + i0);
-        float f[EPL];
-        if (kind == 2) {
+    if (h < a.n_q + c.n_kv) {  // keys, in 64 bits
+        float wy[EPL], wz[EPL];
+        double co[EPL], si[EPL];
+        weights(a.wk, wy, wz);
+        angles(co, si);
+        for (; h < a.n_q + c.n_kv; h += step) {
+            const Words x = take(), xo = others(x);
+            double y[EPL], z[EPL];
 #pragma unroll
-            for (int e = 0; e < EPL; e++) f[e] = to_f32(x.v[e]);
-        } else {
-            double y[EPL], z[EPL];  // the lane's values, and the others of their pairs
-#pragma unroll
-            for (int e = 0; e < EPL; e++) y[e] = to_f32(x.v[e]);
-            const float* wt = kind ? a.wk : a.wq;
-            if (wt) {
+            for (int e = 0; e < EPL; e++) y[e] = value_of<T>(x, e), z[e] = value_of<T>(xo, e);
+            if (a.wk) {
                 double sum = 0.0;
 #pragma unroll
                 for (int e = 0; e < EPL; e++) sum = fma(y[e], y[e], sum);
-                for (int m = 1; m < lp; m <<= 1) sum += __shfl_xor(sum, m);
-                const double r = 1.0 / sqrt(sum / hd + a.eps);
+                const double r = rsqrt_wide(group_sum(sum, lp) / hd + a.eps);
 #pragma unroll
-                for (int e = 0; e < EPL; e++) y[e] = on ? y[e] * r * wt[i0 + e] : 0.0;
+                for (int e = 0; e < EPL; e++) y[e] = y[e] * r * wy[e], z[e] = z[e] * r * wz[e];
             }
-            if constexpr (INTER) {
-#pragma unroll
-                for (int e = 0; e < EPL; e++) z[e] = y[e ^ 1];
-            } else {
-                // four values at a time, whose others are four neighbours too
-#pragma unroll
-                for (int j = 0; j < EPL / 4; j++) {
-                    const int g = ln * (EPL / 4) + j, d = half >> 2;
-                    const int o = g < d ? g + d : g < 2 * d ? g - d : g;
-                    const int from = (threadIdx.x & 63 & ~(lp - 1)) + o / (EPL / 4);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if constexpr (EPL == 4) {
-                            z[e] = __shfl(y[e], from);
-                        } else {
-                            const double lo = __shfl(y[e], from), hi = __shfl(y[4 + e], from);
-                            z[4 * j + e] = o & 1 ? hi : lo;
-                        }
-                    }
-                }
-            }
+            float f[EPL];
             Pack<T, EPL> out;
 #pragma unroll
             for (int e = 0; e < EPL; e++) {
@@ -145,13 +248,18 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int 
                 f[e] = to_odd(v);
                 out.v[e] = round_once<T>(v);
             }
-            T* dst = kind == 0 ? static_cast<T*>(a.q_out) + t * a.ldqo : a.k_out ? static_cast<T*>(a.k_out) + t * a.ldko : nullptr;
-            if (dst && on) *reinterpret_cast<Pack<T, EPL>*>(dst + head * hd + i0) = out;
-            if (kind == 0) continue;
+            if (a.k_out && on) *reinterpret_cast<Pack<T, EPL>*>(static_cast<T*>(a.k_out) + t * a.ldko + (h - a.n_q) * hd + i0) = out;
+            const Kv4Lane q = quantize_lane(f);
+            if (on && where.page >= 0) store_lane<EPL>(c, where, 0, h - a.n_q, ln, q);
         }
-        if (!c.cache) continue;
-        const Kv4Lane z = quantize_lane(f);
-        if (on && w.page >= 0) store_lane<EPL>(c, w, kind - 1, head, ln, z);
+    }
+    for (; h < n_all; h += step) {
+        const Words x = take();
+        float f[EPL];
+#pragma unroll
+        for (int e = 0; e < EPL; e++) f[e] = value_of<T>(x, e);
+        const Kv4Lane q = quantize_lane(f);
+        if (on && where.page >= 0) store_lane<EPL>(c, where, 1, h - a.n_q - c.n_kv, ln, q);
     }
 }
 
@@ -162,10 +270,16 @@ void run_rope_append(RopeAppendArgs a, hipStream_t st) {
     int lp = 1;
     while (lp < lanes) lp <<= 1;
     const int groups = 256 / lp;
-    int tb = c.total < 4096 ? 1 : 16;
-    while (tb > groups || tb * (a.rot / 2) > kTableEntries) tb >>= 1;
+    // As many tokens to a block as bring the blocks down to those that run at once, three to a CU: one token 11 us for 256 tokens (two
+    // 13), 32 for 1536, where two take 25, and 220 for 20500, where 8 take 129 and 16 136 (32 heads of queries, 8 of keys, of 128 values, 16 bits).
+    int tb = 1;
+    while (tb < kMaxTokens && tb * 2 <= groups && tb * a.rot <= kTableEntries && c.total > (int64_t)tb * 3 * kCus) tb <<= 1;
     a.tokens_per_block = tb;
-    const dim3 grid((unsigned)(((int64_t)c.total + tb - 1) / tb), 1);
+    // and more blocks to a token while the card has CUs without any (a token of such heads 5.5 us for 7.7, 64 tokens 7.4 for 10.3)
+    const int n_all = a.n_q + c.n_kv + (c.cache ? c.n_kv : 0), rounds = (n_all * tb + groups - 1) / groups;
+    const int spare = kCus / c.total;
+    const unsigned blocks = (unsigned)(((int64_t)c.total + tb - 1) / tb);
+    const dim3 grid(blocks, rounds < spare ? rounds : spare > 1 ? spare : 1);
     if (a.interleaved) rope_append_kernel<T, true><<<grid, 256, 0, st>>>(a, lp);
     else rope_append_kernel<T, false><<<grid, 256, 0, st>>>(a, lp);
     VLA_LAUNCH_CHECK();
@@ -184,7 +298,7 @@ void check_strided(const void* p, int64_t ld, int heads, const Kv4Args& c, const
 void launch_rope_kv4_append(RopeAppendArgs a, hipStream_t st) {
     const Kv4Args& c = a.kv;
     check_cache(c, "rope_kv4_append");
-    VLA_REQUIRE(c.total < 1 << 26, "rope_kv4_append: fewer than 2^26 rows");  // a launch has less than 2^32 threads
+    VLA_REQUIRE(c.total < (1 << 26) - 3, "rope_kv4_append: fewer than 2^26 - 3 rows");  // 4 or more to a block, a launch has less than 2^32 threads
     VLA_REQUIRE(a.n_q >= 0 && a.n_q <= 65536, "rope_kv4_append: 0 to 65536 query heads");
     VLA_REQUIRE(a.rot >= 0 && a.rot <= c.head_dim && a.rot % 8 == 0, "rope_kv4_append: rot_dim must be a multiple of 8 up to head_dim");
     VLA_REQUIRE(std::isfinite(a.magnitude), "rope_kv4_append: magnitude must be finite");
