@@ -385,9 +385,9 @@ template <class T, int NB>
 struct TreeGeo {
     static constexpr bool KHALF = !__is_same(T, bf16_t);      // keys in fp16 too
     static constexpr int W = 4, HD = 32 * NB;
-    static constexpr int NQ = NB <= 4 ? 2 : 1;                // row tiles of a wave
+    static constexpr int NQ = 2;                              // row tiles of a wave
     static constexpr int PF = KHALF ? 2 : 1;                  // fp16 parts of weights
-    static constexpr int TILES = NB <= 4 ? 2 : 1;             // of a stage
+    static constexpr int TILES = 2;                           // of a stage
     static constexpr int KU = 2 * NB * TILES, VU = NB * TILES;  // units of a stage: a step's 16 keys of 32 dims, a tile's values of 32 dims
     static constexpr int KN = (KU + W - 1) / W, VN = (VU + W - 1) / W;
     static constexpr int KBYTES = KU * 1024, STAGE = KBYTES + VU * 2048;
@@ -515,17 +515,17 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
             }
 #pragma unroll
             for (int i = 0; i < G::KN; i++) {
-                const int t = TILES == 1 ? 0 : k_tile[i];
-                x.kc[i] = *reinterpret_cast<const uint32_t*>((t ? tc[TILES - 1] : tc[0]) + k_at[i]);
-                x.kb[i] = *reinterpret_cast<const uint32_t*>((t ? ts[TILES - 1] : ts[0]) + ks_at[i]);
+                const int t = k_tile[i];
+                x.kc[i] = *reinterpret_cast<const uint32_t*>((t ? tc[1] : tc[0]) + k_at[i]);
+                x.kb[i] = *reinterpret_cast<const uint32_t*>((t ? ts[1] : ts[0]) + ks_at[i]);
             }
 #pragma unroll
             for (int i = 0; i < G::VN; i++) {
-                const int t = TILES == 1 ? 0 : v_tile[i];
-                const auto w = *reinterpret_cast<const Pack<unsigned, 2>*>((t ? ts[TILES - 1] : ts[0]) + ns + vs_at[i]);
+                const int t = v_tile[i];
+                const auto w = *reinterpret_cast<const Pack<unsigned, 2>*>((t ? ts[1] : ts[0]) + ns + vs_at[i]);
                 x.vb[i][0] = w.v[0];
                 x.vb[i][1] = w.v[1];
-                const uint8_t* vp = (t ? tc[TILES - 1] : tc[0]) + nc;
+                const uint8_t* vp = (t ? tc[1] : tc[0]) + nc;
 #pragma unroll
                 for (int k = 0; k < 8; k++) x.vc[i][k] = *reinterpret_cast<const uint32_t*>(vp + (v_at[i] + k * (HD / 2)));
             }
@@ -592,7 +592,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
         auto clean = [&]<bool SLOW>(int stage, Raw& x) {
 #pragma unroll
             for (int i = 0; i < G::VN; i++) {
-                const int t = TILES == 1 ? 0 : v_tile[i], key = k_begin + (stage * TILES + t) * kTile + 8 * g;
+                const int t = v_tile[i], key = k_begin + (stage * TILES + t) * kTile + 8 * g;
                 const bool gone = x.gone >> t & 1u;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
@@ -961,20 +961,21 @@ int64_t row_blocks(int64_t most, int total_q, int n_seqs, int n_q, int n_kv, int
 // them again: two in registers (heads up to 128 in 16-bit types) halve that, from five on four waves share
 // what is converted. Measured, us, 48 sequences mixed up to 8192 keys, 32 heads on 8 of 128, bf16, one in registers | two |
 // shared: 4 new tokens (one row tile) 50 | 67 | 127, 8 (two) 84 | 74 | 131, 16 (four) 118 | 114 | 137, 20 (five) - | 155 | 141, 32 (eight)
-// 200 | 197 | 151; 2 x 131072, 8 new 90 | 80 | 203, 16 new 158 | 132 | 206, 64 new 625 | 507 | 494 (fp16). Heads of
-// 192, 16 new 175 | - | 184; of 256, 32 new 382 | - | 350. (Two waves sharing for four row tiles: 117 and 164 for 114 and 132.)
-constexpr int kSharedTiles = 5;  // row tiles from which on waves share
+// 200 | 197 | 151; 2 x 131072, 8 new 90 | 80 | 203, 16 new 158 | 132 | 206, 64 new 625 | 507 | 494 (fp16). Heads
+// above 128 leave a wave no room for two row tiles, and sharing for four gains nothing: of 256, 16 new 215 | - | 230, 32 new
+// 380 | - | 418, 64 new 706 | - | 1157. (Two waves sharing for four row tiles of 128: 117 and 164 for 114 and 132.)
+constexpr int kSharedTiles = 5, kSharedRows = 8;  // row tiles from which on waves share, and of a block then
 int rows_per_block(int total_q, int max_new, int n_q, int n_kv, int head_dim, bool half) {
-    if (!half) return 1;
+    if (!half || head_dim > 128) return 1;
     const int64_t tiles = row_tiles(max_new < total_q ? max_new : total_q, n_q, n_kv);
-    const int wave = head_dim <= 128 ? 2 : 1;
-    return tiles >= kSharedTiles ? 4 * wave : tiles == 1 ? 1 : wave;
+    return tiles >= kSharedTiles ? kSharedRows : tiles == 1 ? 1 : 2;
 }
 
 // How a call runs, from sizes the host knows: equal runs of tiles (and a second kernel), or a
 // block per sequence and row tiles. In registers as the attention of a causal chunk, by the same measure: a block's steps against the blocks
-// that the card is short of. Shared tiles: runs, each of at least two stages, unless blocks of sequences fill the card twice (us, runs |
-// sequences: 4 x 1000 keys, 32 new 21 | 47, 16 x 3000, 64 new 103 | 126, 48 mixed up to 8192, 32 new 151 | 337, 64 x 4000, 16 new 205 | 195).
+// that the card is short of. Shared tiles: runs, each of at least two stages, unless blocks of sequences fill the card four times (us, runs |
+// sequences: 4 x 1000 keys, 32 new 21 | 47, 16 x 3000, 64 new 103 | 126, 48 mixed up to 8192, 32 new 151 | 337, 100 new 488 | 585, 200
+// new 950 | 898, 64 x 4000, 16 new 205 | 195); no more runs than are under way at once (2 x 131072, 200 new: 9 runs 1690, 10 2590).
 Kv4Run plan(int total_q, int n_seqs, int max_new, int64_t max_len, int n_q, int n_kv, int head_dim, int nq) {
     Kv4Run r{};
     max_new = max_new < total_q ? max_new : total_q;
@@ -983,12 +984,12 @@ Kv4Run plan(int total_q, int n_seqs, int max_new, int64_t max_len, int n_q, int 
     const int64_t most = ((int64_t)1 << 23) / n_kv;  // (a launch has less than 2^32 threads; a block loops over the rest)
     r.tok_tiles = (int)(tiles_of_rows < most ? tiles_of_rows : most);
     const int64_t blocks = row_blocks(r.tok_tiles, total_q, n_seqs, n_q, n_kv, nq);
-    const bool shared = nq >= 4;
+    const bool shared = nq == kSharedRows;
     const int64_t card = shared || attn_waves(head_dim) == 4 ? 512 : 1024;
     const int64_t steps = max_len / (kTile * attn_waves(head_dim));
-    if (shared ? blocks >= 2 * card || max_len <= 8 * kTile : steps <= 64 && steps * (card - blocks) <= 12 * card) return r;
+    if (shared ? blocks >= 4 * card || max_len <= 8 * kTile : steps <= 64 && steps * (card - blocks) <= 12 * card) return r;
     const int64_t tiles = (max_len + kTile - 1) / kTile * n_seqs;
-    int64_t runs = (card * n_seqs + blocks - 1) / blocks;
+    int64_t runs = (card * n_seqs + (shared ? 0 : blocks - 1)) / blocks;
     const int64_t rounds = tiles / (shared ? 4 : 2 * attn_waves(head_dim));
     runs = runs < rounds ? runs : rounds;
     runs = runs < kMaxPieces ? runs : kMaxPieces;
@@ -1008,14 +1009,13 @@ void run_tree_nb(const Kv4TreeArgs& a, const Kv4Run& r, hipStream_t st) {
 
 template <class T, int PQ, int PP, int NB>
 void run_tree_nq(const Kv4TreeArgs& a, const Kv4Run& r, int nq, hipStream_t st) {
-    if constexpr (sizeof(T) == 2) {
-        if (nq >= 4) {
+    if constexpr (sizeof(T) == 2 && NB <= 4) {
+        if (nq == kSharedRows) {
             kv4_tree_shared_kernel<T, NB><<<dim3(a.kv.n_kv * r.tok_tiles, r.runs ? r.runs : a.kv.n_seqs), 256, 0, st>>>(a, r);
             VLA_LAUNCH_CHECK();
             return;
         }
-        if constexpr (NB <= 4)
-            if (nq == 2) return run_tree_nb<T, PQ, PP, NB, 2>(a, r, st);
+        if (nq == 2) return run_tree_nb<T, PQ, PP, NB, 2>(a, r, st);
     }
     run_tree_nb<T, PQ, PP, NB, 1>(a, r, st);
 }
@@ -1089,7 +1089,7 @@ void launch_kv4_tree_attention(const Kv4TreeArgs& ta, hipStream_t st) {
     const int64_t most = grid / ((int64_t)a.n_kv * (r.runs ? r.runs : a.n_seqs));
     if (r.tok_tiles > most) r.tok_tiles = (int)(most < 1 ? 1 : most);
     int log2_n = 0;
-    while (1 << log2_n < a.ld_table * a.page_size) log2_n++;
+    while ((int64_t)1 << log2_n < (int64_t)a.ld_table * a.page_size) log2_n++;
     r.lift = 6.0f + (float)log2_n;
     r.wscale = a.dtype == kF32 ? std::ldexp(1.0f, -6 - log2_n) : 1.0f;
     if (a.dtype == kF32) run_tree<float, 3, 3>(ta, r, nq, st);
