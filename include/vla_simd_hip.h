@@ -600,7 +600,7 @@ VLA_API int32_t vla_verify_drafts_dev(int32_t* path, int32_t* count, int32_t* to
 
 /* Keeps a path of the newest n tokens: the cached token lens[s] - n + path[i] becomes token lens[s] - n + i
  * for i < count[s], in place (path packed as the rows, ascending, path[i] >= i, as vla_verify_drafts_dev gives
- * it), and new_lens[s] (NULL: not wanted; not lens itself) lens[s] - n + count[s]. count is clamped to [0, n]. What
+ * it), and new_lens[s] (NULL: not wanted; not lens or count itself) lens[s] - n + count[s]. count is clamped to [0, n]. What
  * lies behind keeps its bytes. A token without a page is dropped, or moves as NaN. Every layer's cache is kept
  * with the same path. At most 65535 sequences. */
 VLA_API int32_t vla_kv4_keep_dev(void* cache, int32_t n_pages, int32_t page_size, const int32_t* table,

@@ -97,6 +97,11 @@ def test_keep_refusals(vla, kw, msg):
     assert msg in _refused(vla, "vla_kv4_keep_dev", kw)
 
 
+def test_results_over_what_other_blocks_read(vla):
+    assert "parent" in _refused(vla, "vla_draft_tree_dev", dict(pos=P, parent=P))
+    assert "count" in _refused(vla, "vla_kv4_keep_dev", dict(new_lens=P, count=P, lens=P + 64))
+
+
 def test_work_bytes(vla):
     n = vla.kv4_tree_attention_work_bytes
     assert n(64, 2, 32, 131072, 32, 8, 128) > 0

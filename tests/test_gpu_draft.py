@@ -49,6 +49,26 @@ def test_tree(vla, new, wide, extra):
         assert bool((pos[total:] == 77).all()) and bool((see[total:] == 77).all())  # rows behind the sequences
 
 
+@pytest.mark.parametrize("wide,words", [(0, 10), (5, 10), (200, 12), (0, 2), (9, 4), (3, 1)])
+def test_tree_of_many_rows_among_short_ones(vla, wide, words):
+    """Sequences of more than 64 rows where most are short."""
+    r = random.Random(wide)
+    new = [1, 300, 0, 2] + [1] * 40 + [129, 64, 65]
+    parents, lens, start = [_tree(r, n, wide) for n in new], [n + 7 for n in new], _starts(new)
+    if wide == 5:
+        parents[1][100] = parents[1][200] = -1  # further roots
+        parents[1][150] = 150
+    pos = torch.empty(sum(new), dtype=torch.int32, device=DEV)
+    see = torch.empty(sum(new), words, dtype=torch.int32, device=DEV)
+    for _ in range(2):  # whatever the buffers held
+        vla.draft_tree_dev(pos, see, _i32([x for p in parents for x in p]), _i32(lens), _i32(start))
+        for s, n in enumerate(new):
+            bits, depth = dref.tree(parents[s], n)
+            assert pos[start[s]:start[s + 1]].tolist() == [7 + d for d in depth]
+            assert torch.equal(see[start[s]:start[s + 1]].cpu(), dref.words(bits, words)) if n else True
+        pos.fill_(-99), see.fill_(-1)
+
+
 def test_tree_odd_parents_and_few_words(vla):
     """Parents that are not before their node are none; bits past the words are left out."""
     parent = [7, 0, 2, -5, 1, 4, 2 ** 31 - 1, 3] + [i - 1 for i in range(8, 70)]
@@ -699,6 +719,92 @@ def test_keep_a_token_without_a_page(vla):
     k, v = torch.empty(6, 32, device=DEV), torch.empty(6, 32, device=DEV)
     vla.kv4_gather_dev(k, v, cache, n_kv, hd, page, _i32([[0, 1]]), _i32([0, 6]), _i32([28]))
     assert k[:, 0].isnan().tolist() == v[:, 0].isnan().tolist() == [False, True, True, False, False, False]
+
+
+# ------------------------------------------------------ far apart in memory --
+
+def _far_rows(x, ld):
+    """The same rows, `ld` elements apart, the last one 2^31 elements or more behind the first."""
+    assert (x.shape[0] - 1) * ld >= 2 ** 31
+    buf = torch.empty((x.shape[0] - 1) * ld + x.shape[1], dtype=x.dtype, device=DEV)
+    return torch.as_strided(buf, x.shape, (ld, 1)).copy_(x)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_append_far_rows(vla, interleaved):
+    """Rows, and pages of the cache, behind 2^31 elements and bytes."""
+    n_q, n_kv, hd, page, new = 4, 2, 64, 32, [3, 6]
+    q, k, v, lens, table, cache = _append_case(vla, new, 20, n_q, n_kv, hd, page, BF16, 71)
+    rest = (n_q, n_kv, hd, page)
+    args = (_i32(lens), _i32(_starts(new)), dref.freqs(hd).to(DEV))
+    qo, ko = torch.empty_like(q, device=DEV), torch.empty_like(k, device=DEV)
+    vla.rope_kv4_append_dev(qo, cache, q.to(DEV), k.to(DEV), v.to(DEV), *rest, table.to(DEV), *args, interleaved=interleaved, k_out=ko)
+    nb, ld = cache.shape[1], 2 ** 28 + 64
+    far = torch.empty((2 ** 32 + 2 ** 20) // nb, nb, dtype=torch.uint8, device=DEV)
+    off = far.shape[0] - cache.shape[0]
+    far[off:].fill_(0xEE)
+    qf, kf = _far_rows(q, ld), _far_rows(k, ld)
+    vla.rope_kv4_append_dev(qf, far, qf, kf, _far_rows(v, ld), *rest, (table + off).to(DEV), *args, interleaved=interleaved, k_out=kf)
+    assert torch.equal(qf, qo) and torch.equal(kf, ko) and torch.equal(far[off:], cache)
+
+
+@pytest.mark.parametrize("dtype,hd", [(F32, 64), (BF16, 128), (F16, 64), (F16, 256)])
+@pytest.mark.parametrize("m", [2, 9, 33])
+def test_tree_attention_and_keep_far_pages(vla, dtype, hd, m):
+    """Rows and pages behind 2^31 elements and 2^32 bytes give the bits that they give near, in each of the forms."""
+    n_q, n_kv, page, lens, new = 6, 2, 64, [200, 700], [2, m]
+    q, cache, table, _, _ = _decode_case(vla, lens, new, n_q, n_kv, hd, page, dtype, seed=hd + m)
+    _, see = _masks(new, 4, 5)
+    see, total = see.to(DEV), sum(new)
+    need = vla.kv4_tree_attention_work_bytes(total, 2, m, 700, n_q, n_kv, hd)
+    work = torch.empty(max(16, need), dtype=torch.uint8, device=DEV)
+
+    def run(out, q, cache, table):
+        vla.kv4_tree_attention_dev(out, q, cache, n_q, n_kv, hd, page, hd ** -0.5, table, _i32(lens), _i32(_starts(new)), see, m, 700, work)
+        return out
+
+    near = run(torch.empty_like(q, device=DEV), q.to(DEV), cache, table)
+    nb = cache.shape[1]
+    far = torch.empty((2 ** 32 + 2 ** 20) // nb + cache.shape[0], nb, dtype=torch.uint8, device=DEV)
+    off = far.shape[0] - cache.shape[0]
+    far[off:].copy_(cache)
+    there = torch.where(table >= 0, table + off, table)
+    ld = (2 ** 31 // (total - 1) + 64) // 16 * 16
+    out = _far_rows(torch.zeros_like(q), ld)
+    assert torch.equal(run(out, _far_rows(q, ld), far, there), near)
+    path, count = _i32([1, 0] + list(range(m - 1, -1, -1))), _i32([1, 1])
+    for c, t in ((cache, table), (far, there)):
+        vla.kv4_keep_dev(c, n_kv, hd, page, t, _i32(lens), _i32(_starts(new)), path, count)
+    assert torch.equal(far[off:], cache)
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+def test_verify_far_rows(vla, sampled):
+    g, r = _gen(81), random.Random(81)
+    for dtype in (BF16, F32):
+        p, q, tokens, parent, start, u, un = _drafts(g, r, [4, 1, 5], 999, dtype, 2, sampled)
+        want = dref.verify(p, q, tokens, parent, start, u, un)
+        ld = 2 ** 31 // 9 + 5
+        path, count, token = (torch.empty(k, dtype=torch.int32, device=DEV) for k in (10, 3, 3))
+        vla.verify_drafts_dev(path, count, token, _far_rows(p, ld), _i32(tokens), _i32(start), u.to(DEV), un.to(DEV), _i32(parent),
+                              _far_rows(q, ld) if sampled else None)
+        assert (path.tolist(), count.tolist(), token.tolist()) == want
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_verify_many_refused(vla, dtype):
+    """A hundred drafted tokens refused at the root, some of them twice, the last values of the vocabulary among them."""
+    n, V = 101, 1003
+    g = _gen(91)
+    p = torch.softmax(torch.randn(n, V, generator=g), -1).to(dtype)
+    tokens = [0] + [V - 1 - (i % 80) for i in range(n - 1)]
+    parent, u = [-1] + [0] * (n - 1), torch.full((n,), 1.0 - 2.0 ** -20)
+    for un in (0.0, 0.5, 1.0 - 2.0 ** -24):
+        case = (p, None, tokens, parent, [0, n], u, torch.tensor([un]))
+        want = dref.verify(*case)
+        assert want[1] == [1] and want[2][0] not in tokens[1:]
+        assert _verify(vla, *case) == want
+        assert _verify(vla, *case, pad=5, shift=3) == want
 
 
 # ------------------------------------------------------------ as one step --

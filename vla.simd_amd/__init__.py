@@ -1059,7 +1059,7 @@ def verify_drafts_dev(path, count, token, p, tokens, start, u, u_next, parent=No
 
 def kv4_keep_dev(cache, n_kv, head_dim, page_size, table, lens, start, path, count, new_lens=None, stream=None):
     """Keeps the accepted ones of each sequence's newest n tokens in the cache, in place: token lens[s] - n + path[i]
-    becomes token lens[s] - n + i for i < count[s] (verify_drafts_dev's); new_lens (not lens itself) takes the new lengths."""
+    becomes token lens[s] - n + i for i < count[s] (verify_drafts_dev's); new_lens (not lens or count itself) takes the new lengths."""
     pages, n, ld = _cache_shape(cache, n_kv, head_dim, page_size, table)
     total = path.shape[0] if path.dim() == 1 else -1
     for name, t, size in (("lens", lens, n), ("start", start, n + 1), ("path", path, total), ("count", count, n)):

@@ -71,37 +71,44 @@ __global__ __launch_bounds__(256) void draft_tree_rows_kernel(DraftTreeArgs a) {
     });
 }
 
-// A wave for each sequence: up to 64 rows take as many steps as the depth has bits, each joining a row's bits and depth with those of
-// the row that it has got to. (256 trees of 64 rows 2.6 us, by walks 5.4; as many chains 2.8 and 13.7.)
+// A wave for each sequence, 64 rows at a time: they take as many steps as the depth among them has bits, each joining a row's
+// bits and depth with those of the row that it has got to; what is in front of the 64 stands in memory already.
+// (256 trees of 64 rows 2.6 us, by walks 5.4; as many chains 2.8 and 13.7.)
 __global__ __launch_bounds__(64) void draft_tree_wave_kernel(DraftTreeArgs a) {
     const int lane = threadIdx.x;
     for (int s = blockIdx.x; s < a.n_seqs; s += gridDim.x) {
         const Nodes nd = nodes_of(a.start, s, a.total);
-        if (nd.n > 64) {
-            for (int i = lane; i < nd.n; i += 64) walk_up(a, nd, s, i, [&](int at) { return a.parent ? a.parent[nd.first + at] : at - 1; });
-            continue;
-        }
-        int up = lane < nd.n ? a.parent ? a.parent[nd.first + lane] : lane - 1 : -1;
-        up = up >= 0 && up < lane ? up : -1;
-        uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
-        int depth = up >= 0;
-        while (__any(up >= 0)) {
-            const int from = up >= 0 ? up : lane;
-            const uint32_t l = __shfl(lo, from), h = __shfl(hi, from);
-            const int d = __shfl(depth, from), u = __shfl(up, from);
-            if (up >= 0) {
-                lo |= l;
-                hi |= h;
-                depth += d;
-                up = u;
+        const unsigned first_pos = (unsigned)a.lens[s] - (unsigned)nd.n;
+        for (int c0 = 0; c0 < nd.n; c0 += 64) {
+            const int i = c0 + lane;
+            int up = i < nd.n ? a.parent ? a.parent[nd.first + i] : i - 1 : -1;
+            up = up >= 0 && up < i ? up : -1;
+            uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
+            unsigned depth = up >= 0;
+            while (__any(up >= c0)) {
+                const int from = up >= c0 ? up - c0 : lane;
+                const uint32_t l = __shfl(lo, from), h = __shfl(hi, from), d = __shfl(depth, from);
+                const int u = __shfl(up, from);
+                if (up >= c0) {
+                    lo |= l;
+                    hi |= h;
+                    depth += d;
+                    up = u;
+                }
             }
+            if (i < nd.n) {  // (no lane reads what another one writes here: `up` is in front of the 64)
+                uint32_t* see = a.see + (int64_t)(nd.first + i) * a.ld_see;
+                const uint32_t* front = up >= 0 ? a.see + (int64_t)(nd.first + up) * a.ld_see : nullptr;
+                const int w0 = c0 >> 5;
+                for (int w = 0; w < w0 && w < a.ld_see; w++) see[w] = front ? front[w] : 0;
+                if (w0 < a.ld_see) see[w0] = lo;
+                if (w0 + 1 < a.ld_see) see[w0 + 1] = hi;
+                for (int w = w0 + 2; w < a.ld_see; w++) see[w] = 0;
+                if (up >= 0) depth += (unsigned)a.pos[nd.first + up] - first_pos;
+                a.pos[nd.first + i] = (int)(first_pos + depth);
+            }
+            __syncthreads();  // (one wave: its stores before the loads of the next 64)
         }
-        if (lane >= nd.n) continue;
-        uint32_t* see = a.see + (int64_t)(nd.first + lane) * a.ld_see;
-        see[0] = lo;
-        if (a.ld_see > 1) see[1] = hi;
-        for (int w = 2; w < a.ld_see; w++) see[w] = 0;
-        a.pos[nd.first + lane] = (int)((unsigned)a.lens[s] - (unsigned)nd.n + (unsigned)depth);
     }
 }
 
@@ -119,7 +126,7 @@ __global__ __launch_bounds__(64) void draft_tree_wave_kernel(DraftTreeArgs a) {
 // within 2^-50 of a border. A block takes a sequence. Children in front of the first refusal
 // need two probabilities each; every refusal with q, and the draw, go through rows of the vocabulary. What bounds that
 // are the 64-bit instructions, five a value (49280 values of fp32 or of bf16: 3.3 us a time, 120 GB/s of a CU); a chain of four
-// drafted tokens over them takes 14.6 us, 48 trees of 32 take 36, the time of the tree with most refusals.
+// drafted tokens over them takes 14.6 us, 48 trees of 32 take 36 (31 one after the other), the time of the tree with most refusals.
 // (Loading six chunks ahead for four changes nothing; more blocks to a sequence would have to wait for each other.)
 constexpr int kVerifyNodes = 512;   // probabilities held in LDS
 constexpr int kVerifyThreads = 1024;
@@ -391,7 +398,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
 // Token len - n + path[i] of the cache becomes token len - n + i, in place. A block takes one head
 // of a sequence; a thread moves the codes and the scale of a block of 32 values. Rows move
 // forward (path[i] >= i, ascending), so what a pass over some tokens has read before
-// it writes is all that its own writes can reach. Latency bounds it: some hundred bytes a head.
+// it writes is all that its own writes can reach. Latency bounds it, of the offsets, the path, two
+// entries of the table and the codes, one after the other: 8 drafted rows of one sequence, 5 heads of 64, 3.8 us; 64 rows of each of
+// 64 sequences, 8 heads of 128, 17 us, where every 16 bytes are in a line of their own.
 constexpr int kKeepThreads = 128;
 
 struct alignas(16) Codes16 {
@@ -451,6 +460,7 @@ void launch_draft_tree(const DraftTreeArgs& a, hipStream_t st) {
     VLA_REQUIRE(a.ld_see >= 1 && a.ld_see <= 1 << 20, "draft_tree: rows of 1 to 2^20 words");
     if (a.n_seqs == 0 || a.total == 0) return;
     VLA_REQUIRE(a.pos && a.see && a.lens && a.start, "draft_tree: null buffer");
+    VLA_REQUIRE(a.pos != a.parent, "draft_tree: pos must not be parent, which other rows still read");
     // a wave for each sequence where they are small on average
     if (a.total <= (int64_t)64 * a.n_seqs) draft_tree_wave_kernel<<<a.n_seqs < 1 << 20 ? a.n_seqs : 1 << 20, 64, 0, st>>>(a);
     else draft_tree_rows_kernel<<<(a.total + 255) / 256, 256, 0, st>>>(a);
@@ -482,7 +492,7 @@ void launch_kv4_keep(const Kv4KeepArgs& a, hipStream_t st) {
     VLA_REQUIRE(c.n_pages > 0 && c.cache && aligned(c.cache, 16), "kv4_keep: the cache must hold a page and be 16-byte aligned");
     VLA_REQUIRE(c.table && c.ld_table > 0, "kv4_keep: page table missing");
     VLA_REQUIRE(c.lens && c.start && a.count && (a.path || c.total == 0), "kv4_keep: null buffer");
-    VLA_REQUIRE(a.new_lens != c.lens, "kv4_keep: new_lens must not be lens, which other blocks still read");
+    VLA_REQUIRE(!a.new_lens || (a.new_lens != c.lens && a.new_lens != a.count), "kv4_keep: new_lens must not be lens or count, which other blocks still read");
     kv4_keep_kernel<<<dim3(c.n_kv, c.n_seqs), kKeepThreads, 0, st>>>(a);
     VLA_LAUNCH_CHECK();
 }
