@@ -12,11 +12,11 @@
 // are normed and turned in 64 bits and quantized from there: a code then is the nearest of
 // the exact value but where that lies within 2^-40 or so of a border. A result is rounded once.
 //
-// Few rows are bound by latency (the chain from the offsets to the table, the sines, a store: 5.5 us), many by HBM and by the lanes'
-// own work on heads: 16 prompts of 20500 tokens (484 MB with the fp16 rows of the keys) 136 us, 4.4 TB/s of HBM for a copy's 5.1, with pairs as
-// halves 175; 1536 rows with norms 25 us, 1.6 TB/s; fp32, 1000 rows each, 39 us, 6.9 TB/s of caches and HBM. A block takes a few tokens and fills a table of their sines and cosines in
-// LDS, the same for all heads. A group of lanes stays with one token, a lane with 16 bytes of a row
-// at the same place of every head, so that it keeps its sines and cosines in registers. The other
+// Few rows are bound by latency (from the offsets to the table, the sines, a store: 5.5 us), many by HBM and by the lanes'
+// own work on heads: 16 prompts of 20500 tokens (484 MB with the fp16 rows of the keys) 136 us, 3.6 TB/s where a copy has 5.1,
+// with pairs as halves 175; 1536 rows with norms 25 us, 1.3 TB/s, half of it vector instructions; 5005 rows of fp32 39 us.
+// A block takes a few tokens and fills a table of their sines and cosines in LDS, the same for all heads. A group of lanes stays
+// with one token, a lane with 16 bytes of a row at the same place of every head, so that it keeps its sines and cosines in registers. The other
 // value of a pair is another lane's of the group where pairs are halves.
 
 #include "kv4_device.h"
