@@ -399,13 +399,12 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
 // of a sequence; a thread moves the codes and the scale of a block of 32 values. Rows move
 // forward (path[i] >= i, ascending), so what a pass over some tokens has read before
 // it writes is all that its own writes can reach. Latency bounds it, of the offsets, the path, two
-// entries of the table and the codes, one after the other: 8 drafted rows of one sequence, 5 heads of 64, 3.8 us; 64 rows of each of
-// 64 sequences, 8 heads of 128, 17 us, where every 16 bytes are in a line of their own.
+// entries of the table and the codes, one after the other: 8 drafted rows of one sequence, 5 heads of 64, 2.5 us; 64 rows of each of
+// 64 sequences, 8 heads of 128, 3.3 us, an empty launch 2.2.
 constexpr int kKeepThreads = 128;
 
-struct alignas(16) Codes16 {
-    uint32_t u[4];
-};
+// (a vector: an array that lives over the barriers would go to LDS by way of the launch's packet, which is in host memory: 17 us)
+typedef uint32_t Codes16 __attribute__((ext_vector_type(4)));
 
 __global__ __launch_bounds__(kKeepThreads) void kv4_keep_kernel(Kv4KeepArgs k) {
     const Kv4Args& a = k.kv;
@@ -438,7 +437,7 @@ __global__ __launch_bounds__(kKeepThreads) void kv4_keep_kernel(Kv4KeepArgs k) {
         uint8_t *codes = nullptr, *scale = nullptr, *codes_to = nullptr, *scale_to = nullptr;
         const bool to = on && place(base + i, codes_to, scale_to);  // (looked up while the path is on its way)
         const bool moves = to && from != i;
-        Codes16 c{};
+        Codes16 c = {0, 0, 0, 0};
         int byte = kKv4NanByte;  // a token without a page reads as NaN
         if (moves && place(base + from, codes, scale)) {
             c = *reinterpret_cast<const Codes16*>(codes);
