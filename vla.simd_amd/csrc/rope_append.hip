@@ -109,8 +109,8 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int 
     Words x{};  // the first one is on its way while the table is filled
     if (in && h < n_all) x = row(h);
 
-    auto fill = [&] {
-        for (int idx = threadIdx.x; idx < nt * half; idx += 256) {
+    auto fill = [&](int threads) {
+        for (int idx = threadIdx.x; idx < nt * half; idx += threads) {
             const int k = idx / half, i = idx - k * half;
             int p;
             if (a.pos) {
@@ -124,10 +124,24 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int 
             cs[idx] = make_double2(co * a.magnitude, sn * a.magnitude);
         }
     };
-    if (a.pos) fill();
-    locate_rows(c, t0, nt, false, starts, place);
-    if (!a.pos) {
-        fill();
+    if (a.pos) {  // the last wave finds the tokens' places meanwhile
+        if (threadIdx.x < 192) {
+            fill(192);
+        } else {
+            const int i = threadIdx.x - 192;
+            const int32_t* start = c.start;
+            if (c.n_seqs < kStartsInLds) {
+                for (int s = i; s <= c.n_seqs; s += 64) starts[s] = c.start[s];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                start = starts;
+            }
+            if (i < nt) place[i] = locate(c, start, t0 + i, false);
+        }
+        __syncthreads();
+    } else {
+        locate_rows(c, t0, nt, false, starts, place);
+        fill(256);
         __syncthreads();
     }
     const Where where = place[tt < nt ? tt : 0];
