@@ -88,6 +88,7 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int 
     __shared__ double2 cs[kTableEntries];
     __shared__ int32_t starts[kStartsInLds];
     __shared__ Where place[kMaxTokens];
+    __shared__ __attribute__((aligned(16))) float norm[2][256];  // the norms' weights
     const Kv4Args& c = a.kv;
     const int tb = a.tokens_per_block, t0 = blockIdx.x * tb;
     const int nt = c.total - t0 < tb ? c.total - t0 : tb;
@@ -103,11 +104,14 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int 
         const T* src = h < a.n_q ? static_cast<const T*>(a.q) + t * a.ldq + h * hd
                      : h < a.n_q + c.n_kv ? static_cast<const T*>(c.K) + t * c.ldk + (h - a.n_q) * hd
                                           : static_cast<const T*>(c.V) + t * c.ldv + (h - a.n_q - c.n_kv) * hd;
-        return *reinterpret_cast<const Words*>(src + i0);
+        return *reinterpret_cast<const Words*>(src + (i0 < hd ? i0 : 0));
     };
     const int n_all = a.n_q + c.n_kv + (c.cache ? c.n_kv : 0);
-    Words x{};  // the first one is on its way while the table is filled
-    if (in && h < n_all) x = row(h);
+    // A head's load is under way while the one before it is worked on, the first one while the table is filled. All lanes load
+    // in every turn (those without a row another one's, which is not used), so that a wait is for one load and not for a branch's.
+    Words x = row(h < n_all ? h : n_all - 1);
+    if (a.wq && threadIdx.x < hd) norm[0][threadIdx.x] = a.wq[threadIdx.x];
+    if (a.wk && threadIdx.x < hd) norm[1][threadIdx.x] = a.wk[threadIdx.x];
 
     auto fill = [&](int threads) {
         for (int idx = threadIdx.x; idx < nt * half; idx += threads) {
@@ -146,26 +150,31 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int 
     }
     const Where where = place[tt < nt ? tt : 0];
     const bool on = in && where.seq >= 0;  // (rows behind the last sequence are left as they are)
-    // This lane's sines and cosines, 1 and 0 behind the part that turns; the sine's sign is that of the other value's share.
+    // This lane's sines and cosines, by fours; the sine's sign is that of the other value's share. (Behind the part that turns they are not used.)
+    bool turns[EPL / 4];
+#pragma unroll
+    for (int j = 0; j < EPL / 4; j++) turns[j] = on && i0 + 4 * j < a.rot;
     auto angles = [&]<class F>(F (&co)[EPL], F (&si)[EPL]) {
 #pragma unroll
-        for (int e = 0; e < EPL; e++) {
-            const int v = i0 + e;
-            co[e] = 1;
-            si[e] = 0;
-            if (on && v < a.rot) {
-                const int pair = INTER ? v >> 1 : v < half ? v : v - half;
-                const bool second = INTER ? v & 1 : v >= half;
-                const double2 z = cs[tt * half + pair];
-                co[e] = (F)z.x;
-                si[e] = (F)(second ? z.y : -z.y);
+        for (int j = 0; j < EPL / 4; j++) {
+            const int v = i0 + 4 * j;
+            const bool second = !INTER && v >= half;
+            const double2* z = cs + (turns[j] ? tt * half + (INTER ? v >> 1 : second ? v - half : v) : 0);
+            double2 at[INTER ? 2 : 4];
+#pragma unroll
+            for (int e = 0; e < (INTER ? 2 : 4); e++) at[e] = z[e];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double sn = at[INTER ? e >> 1 : e].y;
+                co[4 * j + e] = (F)at[INTER ? e >> 1 : e].x;
+                si[4 * j + e] = (F)((INTER ? e & 1 : second) ? sn : -sn);
             }
         }
     };
     // Where the other values of the lane's pairs are: of halves, four neighbours belong to four neighbours of one lane, in the same
     // half of it or (odd) the other. Behind the part that turns they are not used.
     const int d = half >> 2;  // fours between them
-    const bool odd = EPL == 8 && (d & 1);
+    const unsigned odd = EPL == 8 && (d & 1) ? ~0u : 0u;
     int from[EPL / 4], other[EPL / 4];  // the lane, and the first of the other values, for the weights
 #pragma unroll
     for (int j = 0; j < EPL / 4; j++) {
@@ -182,29 +191,32 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int 
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 if constexpr (EPL == 4) z.w[i] = __shfl(x.w[i], from[0]);
-                else z.w[i] = __shfl(odd ? x.w[i ^ 2] : x.w[i], from[i >> 1]);
+                else z.w[i] = __shfl((x.w[i ^ 2] & odd) | (x.w[i] & ~odd), from[i >> 1]);
             }
         }
         return z;
     };
     // the norm's weights of the lane's values and of the others
-    auto weights = [&](const float* w, float (&mine)[EPL], float (&theirs)[EPL]) {
+    auto weights = [&](const float (&w)[256], float (&mine)[EPL], float (&theirs)[EPL]) {
 #pragma unroll
-        for (int e = 0; e < EPL; e++) {
-            mine[e] = w && on ? w[i0 + e] : 1.0f;
-            theirs[e] = w && on ? w[INTER ? i0 + (e ^ 1) : other[e >> 2] + (e & 3)] : 1.0f;
+        for (int j = 0; j < EPL / 4; j++) {
+            const int at = i0 < hd ? i0 + 4 * j : 0, there = INTER ? at : i0 < hd ? other[j] : 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) mine[4 * j + e] = w[at + e], theirs[4 * j + e] = w[there + (INTER ? e ^ 1 : e)];
         }
     };
 
-    // (a head's load is under way while the one before it is worked on; lanes without a row keep what they have)
+    const unsigned mine = i0 < hd ? ~0u : 0u;
     auto take = [&] {
-        const Words now = x;
-        if (in && h + step < n_all) x = row(h + step);
+        Words now = x;
+        x = row(h + step < n_all ? h + step : n_all - 1);
+#pragma unroll
+        for (int i = 0; i < 4; i++) now.w[i] &= mine;
         return now;
     };
     if (h < a.n_q) {  // queries, in 32 bits
         float cf[EPL], sf[EPL], wy[EPL], wz[EPL];
-        weights(a.wq, wy, wz);
+        if (a.wq) weights(norm[0], wy, wz);
         angles(cf, sf);
         T* dst = static_cast<T*>(a.q_out) + t * a.ldqo + i0;
         const float inv_hd = 1.0f / (float)hd;
@@ -233,14 +245,15 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int 
             }
             Pack<T, EPL> out;
 #pragma unroll
-            for (int e = 0; e < EPL; e++) out.v[e] = (T)(i0 + e < a.rot ? fmaf(cf[e], y[e], sf[e] * z[e]) : y[e]);
+            for (int e = 0; e < EPL; e++) out.v[e] = (T)(turns[e >> 2] ? fmaf(cf[e], y[e], sf[e] * z[e]) : y[e]);
             if (on) *reinterpret_cast<Pack<T, EPL>*>(dst + h * hd) = out;
         }
     }
     if (h < a.n_q + c.n_kv) {  // keys, in 64 bits
         float wy[EPL], wz[EPL];
         double co[EPL], si[EPL];
-        weights(a.wk, wy, wz);
+        const double inv_hd = 1.0 / hd;
+        if (a.wk) weights(norm[1], wy, wz);
         angles(co, si);
         for (; h < a.n_q + c.n_kv; h += step) {
             const Words x = take(), xo = others(x);
@@ -251,7 +264,7 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int 
                 double sum = 0.0;
 #pragma unroll
                 for (int e = 0; e < EPL; e++) sum = fma(y[e], y[e], sum);
-                const double r = rsqrt_wide(group_sum(sum, lp) / hd + a.eps);
+                const double r = rsqrt_wide(fma(group_sum(sum, lp), inv_hd, (double)a.eps));
 #pragma unroll
                 for (int e = 0; e < EPL; e++) y[e] = y[e] * r * wy[e], z[e] = z[e] * r * wz[e];
             }
@@ -259,7 +272,7 @@ __global__ __launch_bounds__(256) void rope_append_kernel(RopeAppendArgs a, int 
             Pack<T, EPL> out;
 #pragma unroll
             for (int e = 0; e < EPL; e++) {
-                const double v = i0 + e < a.rot ? fma(co[e], y[e], si[e] * z[e]) : y[e];
+                const double v = turns[e >> 2] ? fma(co[e], y[e], si[e] * z[e]) : y[e];
                 f[e] = to_odd(v);
                 out.v[e] = round_once<T>(v);
             }
