@@ -12,9 +12,9 @@
 // are normed and turned in 64 bits and quantized from there: a code then is the nearest of
 // the exact value but where that lies within 2^-40 or so of a border. A result is rounded once.
 //
-// Few rows are bound by latency (from the offsets to the table, the sines, a store: 5.5 us), many by HBM and by the lanes'
-// own work on heads: 16 prompts of 20500 tokens (484 MB with the fp16 rows of the keys) 136 us, 3.6 TB/s where a copy has 5.1,
-// with pairs as halves 175; 1536 rows with norms 25 us, 1.3 TB/s, half of it vector instructions; 5005 rows of fp32 39 us.
+// Few rows are bound by latency (from the offsets to the table, the sines, a store: 4 us), many by HBM: 16 prompts of 20500 tokens
+// (484 MB with the fp16 rows of the keys) 104 us, 4.6 TB/s where a copy has 5.1, with pairs as halves 118; 1536 rows with norms
+// 13.8 us, 2.4 TB/s; 5005 rows of fp32 38 us.
 // A block takes a few tokens and fills a table of their sines and cosines in LDS, the same for all heads. A group of lanes stays
 // with one token, a lane with 16 bytes of a row at the same place of every head, so that it keeps its sines and cosines in registers. The other
 // value of a pair is another lane's of the group where pairs are halves.
@@ -298,13 +298,17 @@ void run_rope_append(RopeAppendArgs a, hipStream_t st) {
     int lp = 1;
     while (lp < lanes) lp <<= 1;
     const int groups = 256 / lp;
-    // As many tokens to a block as bring the blocks down to those that run at once, three to a CU: one token 11 us for 256 tokens (two
-    // 13), 32 for 1536, where two take 25, and 220 for 20500, where 8 take 129 and 16 136 (32 heads of queries, 8 of keys, of 128 values, 16 bits).
+    const int n_all = a.n_q + c.n_kv + (c.cache ? c.n_kv : 0);
+    // As many tokens to a block as bring the blocks down to those that run at once, three to a CU, and where that is not to be had eight
+    // turns of a group, over which its table is worth it. One token | 2 | 4 | 8 | 16, 32 heads of queries and 8 of keys of 128, us:
+    // 256 rows with norms 6.6 | 8.4 | 11.4 | 18.2 | 32, 1536 16.4 | 14.0 | 16.0 | 20.4 | 34, 4800 42 | 35 | 30 | 28 | 41; 20500 without 140 | 110 |
+    // 104 | 110 | 134, of heads of 64 with norms 89 | 63 | 52 | 47 | 51, of 12 and 2 heads 77 | 48 | 35 | 31 | 33.
     int tb = 1;
-    while (tb < kMaxTokens && tb * 2 <= groups && tb * a.rot <= kTableEntries && c.total > (int64_t)tb * 3 * kCus) tb <<= 1;
+    while (tb < kMaxTokens && tb * 2 <= groups && tb * a.rot <= kTableEntries && c.total > (int64_t)tb * 3 * kCus &&
+           (n_all * tb < 8 * groups || c.total <= (int64_t)tb * 6 * kCus || c.total > (int64_t)tb << 23)) tb <<= 1;  // (a launch has less than 2^32 threads)
     a.tokens_per_block = tb;
-    // and more blocks to a token while the card has CUs without any (a token of such heads 5.5 us for 7.7, 64 tokens 7.4 for 10.3)
-    const int n_all = a.n_q + c.n_kv + (c.cache ? c.n_kv : 0), rounds = (n_all * tb + groups - 1) / groups;
+    // and more blocks to a token while the card has CUs without any (one such row 3.9 us, 64 4.7)
+    const int rounds = (n_all * tb + groups - 1) / groups;
     const int spare = kCus / c.total;
     const unsigned blocks = (unsigned)(((int64_t)c.total + tb - 1) / tb);
     const dim3 grid(blocks, rounds < spare ? rounds : spare > 1 ? spare : 1);
@@ -326,7 +330,7 @@ void check_strided(const void* p, int64_t ld, int heads, const Kv4Args& c, const
 void launch_rope_kv4_append(RopeAppendArgs a, hipStream_t st) {
     const Kv4Args& c = a.kv;
     check_cache(c, "rope_kv4_append");
-    VLA_REQUIRE(c.total < (1 << 26) - 3, "rope_kv4_append: fewer than 2^26 - 3 rows");  // 4 or more to a block, a launch has less than 2^32 threads
+    VLA_REQUIRE(c.total < (1 << 26) - 3, "rope_kv4_append: fewer than 2^26 - 3 rows");  // (4 or more to a block then)
     VLA_REQUIRE(a.n_q >= 0 && a.n_q <= 65536, "rope_kv4_append: 0 to 65536 query heads");
     VLA_REQUIRE(a.rot >= 0 && a.rot <= c.head_dim && a.rot % 8 == 0, "rope_kv4_append: rot_dim must be a multiple of 8 up to head_dim");
     VLA_REQUIRE(std::isfinite(a.magnitude), "rope_kv4_append: magnitude must be finite");
