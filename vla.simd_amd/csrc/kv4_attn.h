@@ -212,6 +212,11 @@ __global__ __launch_bounds__(N) void kv4_join_kernel(Kv4Args a, Kv4Run run) {
     const size_t stride = (size_t)run.tok_cap * a.n_q;
     const float* pml = run.ml + (in.x * stride + (size_t)in.z * a.n_q + head) * 2;
     const float* po = run.o + (in.x * stride + (size_t)in.z * a.n_q + head) * a.head_dim;
+    const int lanes = a.head_dim / 4, groups = N / lanes;
+    const int gr = tid / lanes, ln = tid - gr * lanes;
+    // (values of two pieces are under way with the maxima; a lane without a piece loads the last one's)
+    auto value = [&](int s) { return *reinterpret_cast<const float4*>(po + (s < pieces ? s : pieces - 1) * stride * a.head_dim + ln * 4); };
+    const float4 first = value(gr), second = value(gr + groups);
     float2 z[kMaxPieces / N];
     float m = -INFINITY;
 #pragma unroll
@@ -241,19 +246,19 @@ __global__ __launch_bounds__(N) void kv4_join_kernel(Kv4Args a, Kv4Run run) {
 #pragma unroll
     for (int w = 1; w < N / 64; w++) sum += red[w][1];
 
-    const int lanes = a.head_dim / 4, groups = N / lanes;
-    const int gr = tid / lanes, ln = tid - gr * lanes;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (gr < groups) {
-#pragma unroll 4
-        for (int s = gr; s < pieces; s += groups) {
-            const float4 v = *reinterpret_cast<const float4*>(po + s * stride * a.head_dim + ln * 4);
+        auto add = [&](int s, const float4& v) {
             const float w = factor[s];
             acc.x += w * v.x;
             acc.y += w * v.y;
             acc.z += w * v.z;
             acc.w += w * v.w;
-        }
+        };
+        if (gr < pieces) add(gr, first);
+        if (gr + groups < pieces) add(gr + groups, second);
+#pragma unroll 4
+        for (int s = gr + 2 * groups; s < pieces; s += groups) add(s, value(s));
     }
     part[tid] = acc;
     __syncthreads();
