@@ -721,6 +721,39 @@ def test_keep_a_token_without_a_page(vla):
     assert k[:, 0].isnan().tolist() == v[:, 0].isnan().tolist() == [False, True, True, False, False, False]
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_q,n_kv,hd", [(0, 3, 64), (0, 1, 96), (5, 5, 32), (0, 2, 256)])
+def test_rope_append_that_turns_nothing(vla, dtype, n_q, n_kv, hd):
+    """Without pairs and norms it is the append, with or without queries; k_out and q_out get the rows as they are."""
+    new, page = [40, 1, 0, 7], 32
+    q, k, v, lens, table, cache = _append_case(vla, new, 9, max(1, n_q), n_kv, hd, page, dtype, 17)
+    other, ko = cache.clone(), torch.empty_like(k, device=DEV)
+    start, none = _i32(_starts(new)), torch.empty(0, dtype=torch.float64, device=DEV)
+    qd = q.to(DEV) if n_q else None
+    qo = torch.empty_like(qd) if n_q else None
+    vla.rope_kv4_append_dev(qo, cache, qd, k.to(DEV), v.to(DEV), n_q, n_kv, hd, page, table.to(DEV), _i32(lens), start, none, k_out=ko)
+    vla.kv4_append_dev(other, k.to(DEV), v.to(DEV), n_kv, hd, page, table.to(DEV), _i32(lens), start)
+    assert torch.equal(cache, other) and torch.equal(ko.cpu(), k)
+    assert not n_q or torch.equal(qo.cpu(), q)
+
+
+@pytest.mark.parametrize("dtype,hd", [(F32, 64), (BF16, 64), (F16, 256)])
+def test_tree_attention_of_more_than_it_was_told(vla, dtype, hd):
+    """max_new and max_len choose the launch only, the workspace of those sizes is all that is used."""
+    n_q, n_kv, page, lens, new = 8, 2, 32, [900, 40, 3000, 64], [33, 5, 90, 1]
+    q, cache, table, ks, vs = _decode_case(vla, lens, new, n_q, n_kv, hd, page, dtype, seed=19)
+    truth, see = _masks(new, 6, 5)
+    want, bound = dref.attend(q, ks, vs, new, truth, n_q, n_kv, hd, 0.1)
+    for max_new, max_len in ((1, 1), (1, 3000), (40, 1), (90, 100), (2 ** 31 - 1, 2 ** 31 - 1)):
+        nb = vla.kv4_tree_attention_work_bytes(sum(new), 4, max_new, max_len, n_q, n_kv, hd)
+        room = torch.full((nb + 4096,), 0xA5, dtype=torch.uint8, device=DEV)
+        out = torch.empty_like(q, device=DEV)
+        vla.kv4_tree_attention_dev(out, q.to(DEV), cache, n_q, n_kv, hd, page, 0.1, table, _i32(lens), _i32(_starts(new)), see.to(DEV), max_new,
+                                   max_len, room[:max(16, nb)])
+        ref.within(out, want, bound, str((max_new, max_len)))
+        assert bool((room[max(16, nb):] == 0xA5).all())
+
+
 # ------------------------------------------------------ far apart in memory --
 
 def _far_rows(x, ld):
