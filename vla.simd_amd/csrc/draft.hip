@@ -185,6 +185,13 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
         phase = (int)(reinterpret_cast<uintptr_t>(pr) / sizeof(T) % VEC);
         wide = !qr || (int)(reinterpret_cast<uintptr_t>(qr) / sizeof(T) % VEC) == phase;
     };
+    auto difference = [&](const Pack<T, VEC>& x, const Pack<T, VEC>& y, bool two, double coef, double (&w)[VEC]) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const double pv = to_f32(x.v[e]);
+            w[e] = above_zero(two ? fma(-coef, (double)to_f32(y.v[e]), pv) : pv);
+        }
+    };
     // the weights of values v .. v + VEC - 1 (v + phase a multiple of VEC), 0 outside the row
     auto weights = [&](int v, double coef, double (&w)[VEC]) {
         const bool two = qr && coef != 0.0;
@@ -200,11 +207,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
                 if (two) y.v[e] = in ? qr[v + e] : (T)0.0f;
             }
         }
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-            const double pv = to_f32(x.v[e]);
-            w[e] = above_zero(two ? fma(-coef, (double)to_f32(y.v[e]), pv) : pv);
-        }
+        difference(x, y, two, coef, w);
     };
     // Tokens refused at the node: in LDS, and past its room at the end of the path, of whose n places
     // those kept and refused never need more.
@@ -233,29 +236,54 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
         for (int i = 0; i < W; i++) all += sums[turn][i];
         return all;
     };
-    auto sum_of = [&](int v0, double coef) {  // of a lane's values of the chunk at v0, which all lanes go through
-        const int v = v0 + lane * VEC;
-        double w[VEC], sum = 0.0;
-        weights(v, coef, w);
+    auto plus = [&](int v, double (&w)[VEC]) {
+        double sum = 0.0;
         if (n_refused) drop(v, w);
 #pragma unroll
         for (int e = 0; e < VEC; e++) sum += w[e];
         return sum;
     };
-    // the sum of what is left (some chunks at a time, so that their loads are under way together)
-    auto total_of = [&](double coef) {
-        constexpr int U = 16 / VEC;
-        const int begin = wave * share - phase, end = begin + share < V ? begin + share : V;
-        double sum = 0.0;
-        int v = begin;
-        for (; v + (U - 1) * chunk < end; v += U * chunk) {
-            double part[U];
+    auto sum_of = [&](int v0, double coef) {  // of a lane's values of the chunk at v0, which all lanes go through
+        const int v = v0 + lane * VEC;
+        double w[VEC];
+        weights(v, coef, w);
+        return plus(v, w);
+    };
+    // the same of U chunks in the row, whose loads are all under way before the first is used; `two`: with q
+    auto sums_of = [&]<int U, bool TWO>(int v0, double coef, double (&part)[U]) {
+        Pack<T, VEC> x[U], y[U];
+        const int v = v0 + lane * VEC;
 #pragma unroll
-            for (int i = 0; i < U; i++) part[i] = sum_of(v + i * chunk, coef);
-#pragma unroll
-            for (int i = 0; i < U; i++) sum += part[i];
+        for (int i = 0; i < U; i++) {
+            x[i] = *reinterpret_cast<const Pack<T, VEC>*>(pr + v + i * chunk);
+            if constexpr (TWO) y[i] = *reinterpret_cast<const Pack<T, VEC>*>(qr + v + i * chunk);
         }
-        for (; v < end; v += chunk) sum += sum_of(v, coef);
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            double w[VEC];
+            difference(x[i], y[i], TWO, coef, w);
+            part[i] = plus(v + i * chunk, w);
+        }
+    };
+    // the sum of what is left
+    auto total_of = [&](double coef) {
+        constexpr int U = 4;
+        const int begin = wave * share - phase, end = begin + share < V ? begin + share : V;
+        const bool two = qr && coef != 0.0;
+        double sum = 0.0;
+        for (int v = begin; v < end;) {
+            if (wide && v >= 0 && v + U * chunk <= V && v + (U - 1) * chunk < end) {
+                double part[U];
+                if (two) sums_of.template operator()<U, true>(v, coef, part);
+                else sums_of.template operator()<U, false>(v, coef, part);
+#pragma unroll
+                for (int i = 0; i < U; i++) sum += part[i];
+                v += U * chunk;
+            } else {
+                sum += sum_of(v, coef);
+                v += chunk;
+            }
+        }
         return all_of(sum);
     };
 
