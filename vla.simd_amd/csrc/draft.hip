@@ -125,9 +125,9 @@ __global__ __launch_bounds__(64) void draft_tree_wave_kernel(DraftTreeArgs a) {
 // Sums are of 64 bits, so that their order moves a result only where a random number lies
 // within 2^-50 of a border. A block takes a sequence. Children in front of the first refusal
 // need two probabilities each; every refusal with q, and the draw, go through rows of the vocabulary. What bounds that
-// are the 64-bit instructions, five a value (49280 values of fp32 or of bf16: 3.3 us a time, 120 GB/s of a CU); a chain of four
-// drafted tokens over them takes 14.6 us, 48 trees of 32 take 36 (31 one after the other), the time of the tree with most refusals.
-// (Loading six chunks ahead for four changes nothing; more blocks to a sequence would have to wait for each other.)
+// is one CU: the loads' latency, four chunks at a time, and 64-bit instructions, five a value (bf16 takes as long as fp32: 29 us, 31).
+// A chain of four drafted tokens over 49280 values takes 12.8 us, over 131072 17.4; 48 trees of 32 take 31, the time of the tree with most
+// refusals, under 3 us each. (More blocks to a sequence would have to wait for each other.)
 constexpr int kVerifyNodes = 512;   // probabilities held in LDS
 constexpr int kVerifyThreads = 1024;
 
