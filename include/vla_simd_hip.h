@@ -561,7 +561,7 @@ VLA_API int32_t vla_rope_kv4_append_dev(void* q_out, int64_t ldqo, void* k_out, 
 /* vla_kv4_attention_dev with a mask among the newest tokens: row i of the n of sequence s sees
  * the keys j < lens[s] - n, and key lens[s] - n + t (t < n) where bit t of its words in see [total_q, ld_see]
  * is set, itself included. Words that a row does not have are 0. A row that sees no key gets
- * zeros. Weights are held to 24 bits for fp32, for fp16 to 2^-15 of themselves, for bf16 to 2^-11 of
+ * zeros. Weights are held to 24 bits for fp32, for the 16-bit types to 2^-15 of
  * themselves or 2^-18 of the largest among 64 neighbouring keys', where that is more. Everything else as
  * there, the workspace by its own function. */
 VLA_API int64_t vla_kv4_tree_attention_work_bytes(int32_t total_q, int32_t n_seqs, int32_t max_new,

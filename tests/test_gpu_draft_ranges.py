@@ -1,0 +1,74 @@
+"""GPU tests of the operators around drafted tokens where values leave the middle of their range: attention's weights
+bit by bit, scores past 2^24 and below -1e30, small weights beside a sink, infinities under a norm; and their forms for
+many rows."""
+
+import math
+import random
+
+import pytest
+import torch
+
+import draft_ref as dref
+import serving_ref as ref
+from test_gpu_draft import _append_case, _attend, _cache_image, _masks
+from test_gpu_serving import BF16, DEV, F16, F32, TYPES, _decode_case, _dev, _gen, _i32, _rows, _starts
+
+pytestmark = pytest.mark.gpu
+
+
+def _put(vla, cache, table, hd, page, t, part, codes=None, byte=None, block=0, head=0, n_kv=1):
+    """Codes (32, each of 4 bits) and scale byte of a cached block, in a host copy of the cache."""
+    row, flat = table.cpu().numpy()[0], cache.view(-1)
+    if codes is not None:
+        at = vla.kv4_offset(row, n_kv, hd, page, cache.shape[0], t, part, head, block)
+        flat[at:at + 16] = torch.tensor([codes[2 * i] | codes[2 * i + 1] << 4 for i in range(16)], dtype=torch.uint8)
+    if byte is not None:
+        flat[vla.kv4_offset(row, n_kv, hd, page, cache.shape[0], t, part + 2, head, block)] = byte
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n_q,n_kv,hd,m", [(4, 1, 64, 3), (4, 1, 64, 40), (32, 8, 128, 32), (8, 1, 32, 60), (6, 2, 96, 50), (2, 1, 256, 40)])
+def test_tree_attention_weights_keep_16_bits(vla, dtype, n_q, n_kv, hd, m):
+    """Rows that see two keys of nearly equal weight and opposite values: what is left shows the weights' bits.
+
+    A weight is off by at most 2^-15 of itself, whatever form takes the call: bf16 in two parts of 8 bits, cut off; fp16 in two
+    parts leaves 2^-22, or where the rest is a subnormal number 2^-25 against 2^9 for the row's largest, 2^-34 of that."""
+    page = 32
+    q, cache, table, ks, vs = _decode_case(vla, [m], [m], n_q, n_kv, hd, page, dtype, seed=m + hd)
+    q = (q.float() / 16).to(dtype)  # scores a few hundredths apart
+    c, v = cache.cpu(), vs[0].clone()
+    for t in range(m):
+        for h in range(n_kv):
+            for b in range(hd // 32):
+                _put(vla, c, table, hd, page, t, 1, [2 if t % 2 else 10] * 32, 127, b, h, n_kv)  # 1 or -1
+        v[t] = 1.0 if t % 2 else -1.0
+    truth, see = [torch.zeros(m, m, dtype=torch.bool)], torch.zeros(m, (m + 31) // 32, dtype=torch.int32)
+    for i in range(m):
+        bits = 1 << i | (1 << i - 1 if i else 0)
+        truth[0][i, max(0, i - 1):i + 1] = True
+        see[i] = dref.words([bits], see.shape[1])[0]
+    G, scale = n_q // n_kv, hd ** -0.5
+    for kw in (dict(), dict(split=False)):
+        got = _attend(vla, q, c.to(DEV), table, [m], [m], see, n_q, n_kv, hd, page, scale, **kw)
+        for h in range(n_q):
+            cols = slice(h * hd, (h + 1) * hd)
+            want, bound = ref.softmax_rows(q[:, cols].double(), ks[0][:, h // G], v[:, h // G], truth[0], scale, 2.0 ** -15 + 2.0 ** -34)
+            ref.within(got[:, cols], want, bound + ref.rounding(want, dtype), f"head {h} {kw}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tree_attention_repeats_itself(vla, dtype):
+    """The same call gives the same bits, with other work between the calls."""
+    n_q, n_kv, hd, page = 32, 8, 128, 64
+    r = random.Random(3)
+    new = [32] * 10 + [0, 1]
+    lens = [n + r.randrange(0, 2500) for n in new]
+    q, cache, table, ks, vs = _decode_case(vla, lens, new, n_q, n_kv, hd, page, dtype, seed=4)
+    truth, see = _masks(new, 8, 9)
+    outs = []
+    for i in range(6):
+        outs.append(_attend(vla, q, cache, table, lens, new, see, n_q, n_kv, hd, page, hd ** -0.5).clone())
+        _attend(vla, q[:sum(new[:3 + i])], cache, table[:3 + i], lens[:3 + i], new[:3 + i], see[:sum(new[:3 + i])], n_q, n_kv, hd, page, 0.3)
+    assert all(torch.equal(outs[0], x) for x in outs[1:])
+
+

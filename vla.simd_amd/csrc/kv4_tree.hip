@@ -340,14 +340,14 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_tree_kernel(Kv4TreeArgs ta, Kv4
 // while a stage is worked on the next one is put into the other buffer and the one behind it is loaded.
 //
 // Values c * 2^e with e in [-23, 8] are exact in fp16, and so a stage of such values meets weights in
-// fp16: one part of 11 bits for bf16 results, two for fp16, where bf16 takes two. (fp16 queries then meet
+// fp16, in two parts as in bf16. (fp16 queries then meet
 // keys in fp16 too, in one part instead of two.) Weights are 2^9 times as large, up to 2^15, and where a
 // row's are all below 2^-16 of its largest they are raised for that stage, the sums with them, so that
-// a weight is off by half a step of its bits or by 2^-18 of the stage's largest, whichever is more. The first
+// a weight is off by 2^-22 of itself or by 2^-18 of the stage's largest, whichever is more. The first
 // stage with other values, with what may not be finite or without a page turns the block to bf16 parts for good.
 //
-// 2 x 131072 keys, 64 new tokens, 32 heads on 8 of 128: 494 us in fp16, 403 in bf16 (682 TFLOP/s of the product's own
-// operations); 48 mixed up to 8192, 32 new, bf16: 151. What bounds it are the vector instructions (191 for 32 rows and keys) and the matrix
+// 2 x 131072 keys, 64 new tokens, 32 heads on 8 of 128: 497 us in fp16, 483 in bf16 (568 TFLOP/s of the product's own
+// operations); 48 mixed up to 8192, 32 new, bf16: 171. What bounds it are the vector instructions (191 for 32 rows and keys) and the matrix
 // instructions (48, in bf16 32) together: a SIMD's two waves hardly overlap them, nor does conversion between
 // the products of a stage, or the exponentials of its second tile between those of the first, gain anything.
 
@@ -386,7 +386,7 @@ struct TreeGeo {
     static constexpr bool KHALF = !__is_same(T, bf16_t);      // keys in fp16 too
     static constexpr int W = 4, HD = 32 * NB;
     static constexpr int NQ = 2;                              // row tiles of a wave
-    static constexpr int PF = KHALF ? 2 : 1;                  // fp16 parts of weights
+    static constexpr int PF = 2;                              // fp16 parts of weights
     static constexpr int TILES = 2;                           // of a stage
     static constexpr int KU = 2 * NB * TILES, VU = NB * TILES;  // units of a stage: a step's 16 keys of 32 dims, a tile's values of 32 dims
     static constexpr int KN = (KU + W - 1) / W, VN = (VU + W - 1) / W;
