@@ -72,3 +72,58 @@ def test_tree_attention_repeats_itself(vla, dtype):
     assert all(torch.equal(outs[0], x) for x in outs[1:])
 
 
+def _large_scores(vla, dtype, hd, m, sign, e, n):
+    """Scores past 2^24, where a step of fp32 is 2 and more. They are whole steps s * 2^e + d with the scale's product with log2 e
+    exactly 1, so that products, sums and differences are exact and weights depend on d alone: a result has no share of the bound
+    for rounded scores."""
+    n_q, n_kv, page = 4, 1, 64
+    q, cache, table, ks, vs = _decode_case(vla, [n], [m], n_q, n_kv, hd, page, dtype, seed=e)
+    scale = float(torch.tensor(math.log(2.0), dtype=torch.float32))  # times log2 e, in fp32: 1
+    step = 2.0 ** max(0, e - 23)
+    c, k, r = cache.cpu(), torch.zeros(n, 1, hd, dtype=torch.float64), random.Random(e)
+    for t in range(n):  # block 0: 32 times the same; block 1: the step in its first column
+        step_code = r.choice([0, 2, 4, 5, 6, 7])
+        for b in range(hd // 32):
+            _put(vla, c, table, hd, page, t, 0, [2] * 32 if b == 0 else [step_code] + [0] * 31 if b == 1 else [0] * 32, 127 + (5 if b == 0 else 0), b)
+        k[t, 0, :32], k[t, 0, 32] = 32.0, ref.GRID[step_code]
+    q = torch.zeros(m, n_q * hd, dtype=torch.float64)
+    for h in range(n_q):
+        q[:, h * hd:h * hd + 32] = sign * 2.0 ** (e - 10)  # 32 columns of 2^5: 2^e (fp16 up to 2^15: 2^25 here, more below)
+        q[:, h * hd + 32] = step
+    if dtype == F16 and e > 25:  # larger keys instead: of blocks that fp16 takes, up to 2^8
+        up = min(e - 25, 3)
+        q[:, [h * hd + i for h in range(n_q) for i in range(32)]] /= 2.0 ** up
+        k[:, :, :32] *= 2.0 ** up
+        for t in range(n):
+            _put(vla, c, table, hd, page, t, 2 - 2, None, 127 + 5 + up, 0)
+        if e > 28:  # and of others
+            q[:, [h * hd + i for h in range(n_q) for i in range(32)]] /= 2.0 ** 4
+            k[:, :, :32] *= 2.0 ** 4
+            for t in range(n):
+                _put(vla, c, table, hd, page, t, 0, None, 127 + 5 + up + 4, 0)
+    q = q.to(dtype)
+    assert bool(torch.isfinite(q.double()).all())
+    truth, see = _masks([m], 3, 7)
+    full = torch.ones(m, n, dtype=torch.bool)
+    full[:, n - m:] = truth[0]
+    for kw in (dict(), dict(max_len=1 << 20), dict(split=False)):
+        got = _attend(vla, q, c.to(DEV), table, [n], [m], see, n_q, n_kv, hd, page, scale, **kw).double().cpu()
+        z = torch.where(full, (q[:, :hd].double() @ k[:, 0].T) * scale, -math.inf)
+        w = torch.softmax(z, 1)
+        want = (w @ vs[0][:, 0]).repeat(1, n_q)
+        # the exponential's last bits, the sums' order, and the weights' own bits, of fp16 also 2^-18 of the largest of 64
+        rel = (n + 24) * ref.U + (0.0 if dtype == F32 else 2.0 ** -15)
+        low = 0.0 if dtype == F32 else 2.0 ** -18 * w.amax(1, keepdim=True) * vs[0][:, 0].abs().sum(0)
+        bound = (w @ vs[0][:, 0].abs() * rel + low).repeat(1, n_q) + ref.rounding(want, dtype)
+        ref.within(got, want, bound, str(kw))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("m", [3, 40])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("e", [22, 24, 25, 26, 27, 28, 30])
+def test_tree_attention_of_large_scores(vla, dtype, hd, m, sign, e):
+    _large_scores(vla, dtype, hd, m, sign, e, 700)
+
+

@@ -346,8 +346,8 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_tree_kernel(Kv4TreeArgs ta, Kv4
 // a weight is off by 2^-22 of itself or by 2^-18 of the stage's largest, whichever is more. The first
 // stage with other values, with what may not be finite or without a page turns the block to bf16 parts for good.
 //
-// 2 x 131072 keys, 64 new tokens, 32 heads on 8 of 128: 497 us in fp16, 483 in bf16 (568 TFLOP/s of the product's own
-// operations); 48 mixed up to 8192, 32 new, bf16: 171. What bounds it are the vector instructions (191 for 32 rows and keys) and the matrix
+// 2 x 131072 keys, 64 new tokens, 32 heads on 8 of 128: 518 us in fp16, 507 in bf16 (542 TFLOP/s of the product's own
+// operations); 48 mixed up to 8192, 32 new, bf16: 176. What bounds it are the vector instructions (191 for 32 rows and keys) and the matrix
 // instructions (48, in bf16 32) together: a SIMD's two waves hardly overlap them, nor does conversion between
 // the products of a stage, or the exponentials of its second tile between those of the first, gain anything.
 
@@ -647,16 +647,17 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
         float m[NQ], l[NQ];  // the reference of the weights, in log2, and their sum
 #pragma unroll
         for (int z = 0; z < NQ; z++) m[z] = kNone, l[z] = 0.0f;
-        // The reference only has to keep the weights in range: it follows the maximum when
-        // a row's has grown by 2^6, so most tiles rescale nothing.
-        auto follow = [&](const float (&top)[NQ]) {
+        // The reference only has to keep the weights in range: it follows when a row's maximum has passed it by `most`, to `lead` below
+        // that, so most tiles rescale nothing. (Past 2^26, where fp32's steps are above 2 `lead`, it takes the maximum itself.)
+        auto follow = [&](const float (&top)[NQ], float lead, float most) {
             bool grown = false;
 #pragma unroll
-            for (int z = 0; z < NQ; z++) grown |= top[z] > m[z] + 6.0f;
+            for (int z = 0; z < NQ; z++) grown |= top[z] - m[z] > most;
             if (__builtin_expect(__any(grown), 0)) {
 #pragma unroll
                 for (int z = 0; z < NQ; z++) {
-                    const float mn = fmaxf(m[z], rows_max(top[z]));
+                    const float mx = rows_max(top[z]), to = mx - lead;
+                    const float mn = fmaxf(m[z], mx - to > most ? mx : to);
                     const float alpha = __builtin_amdgcn_exp2f(m[z] - mn);
                     m[z] = mn;
                     l[z] *= alpha;
@@ -668,8 +669,11 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
             }
         };
 
-        // a wave's tiles of a stage, in fp16
+        // A wave's tiles of a stage, in fp16. Weights come from the rounded scores that their reference was taken from, and it is
+        // subtracted as it is: from unrounded ones, or with the 2^9 added to it first, they would pass fp16's range
+        // where scores pass 2^24 (48 trees of 32 176 us for 171).
         auto fast_step = [&](const unsigned char* buf, int k0) {
+#pragma clang fp contract(off)
             v4f s[NQ][TILES][2] = {};
 #pragma unroll
             for (int ch = 0; ch < TILES; ch++)
@@ -681,6 +685,10 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
 #pragma unroll
                         for (int z = 0; z < NQ; z++) s[z][ch][sub] = G::KHALF ? mfma16h(k, qv[z][b], s[z][ch][sub]) : mfma16(k, qv[z][b], s[z][ch][sub]);
                     }
+#pragma unroll
+            for (int z = 0; z < NQ; z++)
+#pragma unroll
+                for (int i = 0; i < 8 * TILES; i++) s[z][i >> 3][i >> 2 & 1][i & 3] *= c2;
             if (k0 + TILES * kTile > open) {
 #pragma unroll
                 for (int z = 0; z < NQ; z++)
@@ -698,13 +706,13 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
                 float mx = s[z][0][0][0];
 #pragma unroll
                 for (int i = 1; i < 8 * TILES; i++) mx = fmaxf(mx, s[z][i >> 3][i >> 2 & 1][i & 3]);
-                top[z] = mx * c2;
+                top[z] = mx;
             }
-            follow(top);
+            follow(top, 9.0f, 15.0f);
             // Where the weights of a row are all below 2^-16 of its largest, its sums are raised for these tiles.
             bool low = false;
 #pragma unroll
-            for (int z = 0; z < NQ; z++) low |= top[z] < m[z] - 16.0f && top[z] > kNone;
+            for (int z = 0; z < NQ; z++) low |= top[z] - m[z] < -7.0f && top[z] > kNone;
             low = __any(low);
             float up[NQ];
             auto raise = [&](float sign) {
@@ -723,7 +731,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
             if (__builtin_expect(low, 0)) {
 #pragma unroll
                 for (int z = 0; z < NQ; z++) {
-                    const float k = floorf(m[z] - rows_max(top[z]));
+                    const float k = floorf(m[z] - rows_max(top[z]) + 9.0f);
                     up[z] = k > 40.0f ? 40.0f : k > 0.0f ? k : 0.0f;
                 }
                 raise(1.0f);
@@ -733,11 +741,10 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
                 U4 pw[NQ][G::PF];
 #pragma unroll
                 for (int z = 0; z < NQ; z++) {
-                    const float off = 9.0f - m[z] + up[z];
                     float x[8], sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        x[i] = __builtin_amdgcn_exp2f(fmaf(s[z][ch][i >> 2][i & 3], c2, off));
+                        x[i] = __builtin_amdgcn_exp2f(s[z][ch][i >> 2][i & 3] - m[z] + up[z]);
                         sum += x[i];
                     }
                     l[z] += sum;
@@ -767,6 +774,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
         };
         // one tile of any values and masks, in bf16: fp16 queries and all weights in two parts
         auto slow_step = [&](const unsigned char* buf, int tile, int k0, bool there) {
+#pragma clang fp contract(off)
             v4f s[NQ][2] = {};
 #pragma unroll
             for (int sub = 0; sub < 2; sub++)
@@ -805,15 +813,14 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
                 }
                 top[z] = mx;
             }
-            follow(top);
+            follow(top, 0.0f, 6.0f);
             U4 pw[NQ][2];
 #pragma unroll
             for (int z = 0; z < NQ; z++) {
-                const float off = run.lift + m[z];
                 float x[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    x[i] = bits[z] >> i & 1u ? __builtin_amdgcn_exp2f(s[z][i >> 2][i & 3] - off) : 0.0f;
+                    x[i] = bits[z] >> i & 1u ? __builtin_amdgcn_exp2f(s[z][i >> 2][i & 3] - m[z] - run.lift) : 0.0f;
                     l[z] += x[i];
                 }
 #pragma unroll
@@ -854,8 +861,8 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
             if (i >= 0) fast_step(mem + (i & 1) * G::STAGE + lane * 16, k0);
             i = j;
         }
-        // what is left, from stage i on: sums are of weights 2^-lift as large, not 2^9
-        const float to_slow = __builtin_amdgcn_exp2f(-9.0f - run.lift);
+        // what is left, from stage i on: sums are of weights 2^-lift as large
+        const float to_slow = __builtin_amdgcn_exp2f(-run.lift);
         if (i < stages) {
 #pragma unroll
             for (int z = 0; z < NQ; z++) {
