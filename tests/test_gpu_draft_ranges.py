@@ -127,3 +127,13 @@ def test_tree_attention_of_large_scores(vla, dtype, hd, m, sign, e):
     _large_scores(vla, dtype, hd, m, sign, e, 700)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("m", [3, 40])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("e", [24, 25, 27])
+def test_tree_attention_of_large_scores_in_a_longer_table(vla, dtype, hd, m, sign, e):
+    """The weights' scale is an odd power of two there, which a step of 2 does not take."""
+    _large_scores(vla, dtype, hd, m, sign, e, 1300)
+
+

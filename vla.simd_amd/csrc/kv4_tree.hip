@@ -148,6 +148,7 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_tree_kernel(Kv4TreeArgs ta, Kv4
         };
         int cleaned = 0;
         auto step = [&](Kv4Tile<NB>& t, int k0) {
+#pragma clang fp contract(off)
             v4f s[NQ][2] = {};
 #pragma unroll
             for (int sub = 0; sub < 2; sub++)
@@ -208,11 +209,12 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_tree_kernel(Kv4TreeArgs ta, Kv4
                     scale_sums(z, alpha);
                 }
                 // Weights reach 2^6, and no sum over all keys may leave fp32's range: they are 2^-lift as large, in the
-                // product alone where they have 24 bits, as their exponent's rounding to 2^-19 would show.
-                const float mu = (m[z] == -INFINITY ? 0.0f : m[z]) + (PP == 3 ? 0.0f : run.lift);
+                // product alone where they have 24 bits, as their exponent's rounding to 2^-19 would show. (Subtracted behind the
+                // reference: a sum of both is rounded by a power of two where scores pass 2^24, and not the same one for every reference.)
+                const float mu = m[z] == -INFINITY ? 0.0f : m[z];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    x[z][i] = __builtin_amdgcn_exp2f(x[z][i] - mu);
+                    x[z][i] = __builtin_amdgcn_exp2f(PP == 3 ? x[z][i] - mu : x[z][i] - mu - run.lift);
                     l[z] += x[z][i];
                     if (PP == 3) x[z][i] *= run.wscale;
                 }
