@@ -137,3 +137,32 @@ def test_tree_attention_of_large_scores_in_a_longer_table(vla, dtype, hd, m, sig
     _large_scores(vla, dtype, hd, m, sign, e, 1300)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [32, 128, 256])
+@pytest.mark.parametrize("m", [3, 40])
+def test_tree_attention_of_scores_below_all_others(vla, dtype, hd, m):
+    """Every score -2^105 (-4e31) or twice that: the mean over the former."""
+    n_q, n_kv, page, n = 4, 1, 64, 500
+    q, cache, table, ks, vs = _decode_case(vla, [n], [m], n_q, n_kv, hd, page, dtype, seed=11)
+    c, r = cache.cpu(), random.Random(2)
+    k = torch.zeros(n, 1, hd, dtype=torch.float64)
+    up = 15 if dtype == F16 else 60
+    for t in range(n):
+        code = r.choice([2, 4])
+        for b in range(hd // 32):
+            _put(vla, c, table, hd, page, t, 0, [code] + [0] * 31 if b == 0 else [0] * 32, 127 + 105 - up if b == 0 else 127, b)
+        k[t, 0, 0] = ref.GRID[code] * 2.0 ** (105 - up)
+    q = torch.zeros(m, n_q * hd)
+    q[:, ::hd] = -2.0 ** up
+    q = q.to(dtype)
+    truth, see = _masks([m], 3, 7)
+    full = torch.ones(m, n, dtype=torch.bool)
+    full[:, n - m:] = truth[0]
+    w = torch.softmax(torch.where(full, q[:, :hd].double() @ k[:, 0].T, -math.inf), 1)
+    want = (w @ vs[0][:, 0]).repeat(1, n_q)
+    rel = (n + 24) * ref.U + (0.0 if dtype == F32 else 2.0 ** -15)
+    bound = (w @ vs[0][:, 0].abs() * rel).repeat(1, n_q) + ref.rounding(want, dtype)
+    for kw in (dict(), dict(max_len=1 << 20), dict(split=False)):
+        ref.within(_attend(vla, q, c.to(DEV), table, [n], [m], see, n_q, n_kv, hd, page, 1.0, **kw), want, bound, str(kw))
+
+

@@ -399,7 +399,6 @@ template <class T, int NB>
 __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta, Kv4Run run) {
     using G = TreeGeo<T, NB>;
     constexpr int W = G::W, NQ = G::NQ, TILES = G::TILES, HD = G::HD, NT = 2 * NB;
-    constexpr float kNone = -1e30f;  // of a row that has seen no key
     const Kv4Args& a = ta.kv;
     __shared__ __attribute__((aligned(16))) unsigned char mem[2 * G::STAGE];
     __shared__ int slow_at, cleaned;  // the first stage that fp16 does not take; whether values were taken out
@@ -411,7 +410,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
     const int group = a.n_q / a.n_kv;
     const int heads = group < 16 ? group : 16;         // heads of a row tile
     const int toks = group < 16 ? 16 / group : 1;      // tokens of a row tile
-    const float c2 = fmaxf(fabsf(a.scale) * kLog2e, 1e-30f);  // (not 0: scores that are not seen are -infinity)
+    const float c2 = fabsf(a.scale) * kLog2e;
     const unsigned flip = a.scale < 0.0f ? 0x80008000u : 0u;  // of the queries' signs
     const size_t nc = kv4_code_bytes(a.n_kv, HD, a.page_size), ns = kv4_scale_bytes(a.n_kv, HD, a.page_size), pb = 2 * (nc + ns);
     const uint8_t* codes = a.cache + (size_t)kvh * a.page_size * (HD / 2);
@@ -648,19 +647,19 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
         v4f o[NQ][NT] = {};
         float m[NQ], l[NQ];  // the reference of the weights, in log2, and their sum
 #pragma unroll
-        for (int z = 0; z < NQ; z++) m[z] = kNone, l[z] = 0.0f;
+        for (int z = 0; z < NQ; z++) m[z] = -INFINITY, l[z] = 0.0f;
         // The reference only has to keep the weights in range: it follows when a row's maximum has passed it by `most`, to `lead` below
         // that, so most tiles rescale nothing. (Past 2^26, where fp32's steps are above 2 `lead`, it takes the maximum itself.)
         auto follow = [&](const float (&top)[NQ], float lead, float most) {
             bool grown = false;
 #pragma unroll
-            for (int z = 0; z < NQ; z++) grown |= top[z] - m[z] > most;
+            for (int z = 0; z < NQ; z++) grown |= top[z] - m[z] > most;  // (not where a row has seen nothing)
             if (__builtin_expect(__any(grown), 0)) {
 #pragma unroll
                 for (int z = 0; z < NQ; z++) {
                     const float mx = rows_max(top[z]), to = mx - lead;
                     const float mn = fmaxf(m[z], mx - to > most ? mx : to);
-                    const float alpha = __builtin_amdgcn_exp2f(m[z] - mn);
+                    const float alpha = __builtin_amdgcn_exp2f(m[z] - (mn == -INFINITY ? 0.0f : mn));
                     m[z] = mn;
                     l[z] *= alpha;
 #pragma unroll
@@ -714,7 +713,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
             // Where the weights of a row are all below 2^-16 of its largest, its sums are raised for these tiles.
             bool low = false;
 #pragma unroll
-            for (int z = 0; z < NQ; z++) low |= top[z] - m[z] < -7.0f && top[z] > kNone;
+            for (int z = 0; z < NQ; z++) low |= top[z] - m[z] < -7.0f && top[z] > -INFINITY;
             low = __any(low);
             float up[NQ];
             auto raise = [&](float sign) {
@@ -743,10 +742,11 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
                 U4 pw[NQ][G::PF];
 #pragma unroll
                 for (int z = 0; z < NQ; z++) {
+                    const float mu = m[z] == -INFINITY ? 0.0f : m[z];
                     float x[8], sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        x[i] = __builtin_amdgcn_exp2f(s[z][ch][i >> 2][i & 3] - m[z] + up[z]);
+                        x[i] = __builtin_amdgcn_exp2f(s[z][ch][i >> 2][i & 3] - mu + up[z]);
                         sum += x[i];
                     }
                     l[z] += sum;
@@ -819,10 +819,11 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
             U4 pw[NQ][2];
 #pragma unroll
             for (int z = 0; z < NQ; z++) {
+                const float mu = m[z] == -INFINITY ? 0.0f : m[z];
                 float x[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    x[i] = bits[z] >> i & 1u ? __builtin_amdgcn_exp2f(s[z][i >> 2][i & 3] - m[z] - run.lift) : 0.0f;
+                    x[i] = bits[z] >> i & 1u ? __builtin_amdgcn_exp2f(s[z][i >> 2][i & 3] - mu - run.lift) : 0.0f;
                     l[z] += x[i];
                 }
 #pragma unroll
