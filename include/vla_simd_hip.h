@@ -562,8 +562,8 @@ VLA_API int32_t vla_rope_kv4_append_dev(void* q_out, int64_t ldqo, void* k_out, 
  * the keys j < lens[s] - n, and key lens[s] - n + t (t < n) where bit t of its words in see [total_q, ld_see]
  * is set, itself included. Words that a row does not have are 0. A row that sees no key gets
  * zeros. Weights are held to 24 bits for fp32, for the 16-bit types to 2^-15 of
- * themselves or 2^-18 of the largest among 64 neighbouring keys', where that is more. Everything else as
- * there, the workspace by its own function. */
+ * themselves or 2^-18 of the largest among 64 neighbouring keys', where that is more, down to 2^-80 of
+ * the row's largest. Everything else as there, the workspace by its own function. */
 VLA_API int64_t vla_kv4_tree_attention_work_bytes(int32_t total_q, int32_t n_seqs, int32_t max_new,
                                                   int32_t max_len, int32_t n_q, int32_t n_kv,
                                                   int32_t head_dim);

@@ -166,3 +166,72 @@ def test_tree_attention_of_scores_below_all_others(vla, dtype, hd, m):
         ref.within(_attend(vla, q, c.to(DEV), table, [n], [m], see, n_q, n_kv, hd, page, 1.0, **kw), want, bound, str(kw))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("below", [38, 45, 52, 60])
+@pytest.mark.parametrize("m", [3, 40])
+def test_tree_attention_far_below_a_sink(vla, dtype, hd, below, m):
+    """One key takes the weight of every row and has the value zero; the others' weights, down to e^-60, are what the result is made of."""
+    n_q, n_kv, page, n = 4, 1, 64, 2000
+    q, cache, table, ks, vs = _decode_case(vla, [n], [m], n_q, n_kv, hd, page, dtype, seed=below)
+    c, k, v = cache.cpu(), ks[0].clone(), vs[0].clone()
+    q = torch.zeros_like(q)
+    q[:, ::hd] = 1.0  # a row's score is its key's first value
+    scale = below / 4.0
+    for t in range(n):
+        _put(vla, c, table, hd, page, t, 0, [6 if t == 0 else 0] + [0] * 31, 127)  # 4, the others 0
+        k[t, 0, :32] = 0.0
+    k[0, 0, 0], v[0] = 4.0, 0.0
+    for b in range(hd // 32):
+        _put(vla, c, table, hd, page, 0, 1, [0] * 32, None, b)
+    truth, see = _masks([m], 3, 7)
+    full = torch.ones(m, n, dtype=torch.bool)
+    full[:, n - m:] = truth[0]
+    w = torch.softmax(torch.where(full, q[:, :hd].double() @ k[:, 0].T * scale, -math.inf), 1)
+    want = (w @ v[:, 0]).repeat(1, n_q)
+    # The scores are exact but for the scale's three roundings: 2 * 3 u of `below`. Weights: 2^-15 of themselves, or 2^-18 of the
+    # largest among the 64 neighbours, as all of them are. Of those beside the sink that leaves nothing.
+    rel = (n + 24) * ref.U + 6 * ref.U * below + (0.0 if dtype == F32 else 2.0 ** -15 + 2.0 ** -18)
+    near = w.clone()
+    near[:, 64:] = 0.0
+    bound = (w @ v[:, 0].abs() * rel + (0.0 if dtype == F32 else near @ v[:, 0].abs())).repeat(1, n_q) + ref.rounding(want, dtype)
+    for kw in (dict(), dict(max_len=1 << 20), dict(split=False)):
+        ref.within(_attend(vla, q, c.to(DEV), table, [n], [m], see, n_q, n_kv, hd, page, scale, **kw), want, bound, str(kw))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("below", [30, 45, 60])
+@pytest.mark.parametrize("late", [777, 1470, 1499])
+def test_tree_attention_far_below_sinks_of_some_rows(vla, dtype, below, late):
+    """Sinks for some rows at the first key, for others at a later one, for the rest none: what one wave of a block leaves to the
+    other form the others have done."""
+    n_q, n_kv, hd, page, n, m = 4, 1, 64, 64, 1500, 40
+    q, cache, table, ks, vs = _decode_case(vla, [n], [m], n_q, n_kv, hd, page, dtype, seed=below)
+    c, k, v = cache.cpu(), torch.zeros(n, 1, hd, dtype=torch.float64), vs[0].clone()
+    q = torch.zeros_like(q)
+    q[:16, ::hd], q[16:32, 1::hd] = 1.0, 1.0
+    scale = below / 4.0
+    for t in range(n):
+        for b in range(2):
+            _put(vla, c, table, hd, page, t, 0, [6 if t == 0 and b == 0 else 0, 6 if t == late and b == 0 else 0] + [0] * 30, 127, b)
+    k[0, 0, 0] = k[late, 0, 1] = 4.0
+    for t in (0, late):
+        v[t] = 0.0
+        for b in range(2):
+            _put(vla, c, table, hd, page, t, 1, [0] * 32, None, b)
+    truth, see = torch.ones(m, m, dtype=torch.bool), torch.full((m, 2), -1, dtype=torch.int32)
+    truth[5, 3:], see[5] = False, torch.tensor([7, 0])
+    full = torch.ones(m, n, dtype=torch.bool)
+    full[:, n - m:] = truth
+    w = torch.softmax(torch.where(full, q[:, :hd].double() @ k[:, 0].T * scale, -math.inf), 1)
+    want = (w @ v[:, 0]).repeat(1, n_q)
+    # as above; the largest of 64 neighbours lies in the tile of 32 or one beside it
+    tiles = torch.nn.functional.pad(w, (0, -n % 32)).unflatten(1, (-1, 32)).amax(-1)
+    near = torch.stack([torch.nn.functional.pad(tiles, (1, 1))[:, i:i + tiles.shape[1]] for i in range(3)]).amax(0).repeat_interleave(32, 1)[:, :n]
+    rel = (n + 24) * ref.U + 6 * ref.U * below + (0.0 if dtype == F32 else 2.0 ** -15)
+    lost = 0.0 if dtype == F32 else torch.minimum(w, 2.0 ** -18 * near) @ v[:, 0].abs()
+    bound = (w @ v[:, 0].abs() * rel + lost).repeat(1, n_q) + ref.rounding(want, dtype)
+    for kw in (dict(), dict(max_len=1 << 20), dict(split=False)):
+        ref.within(_attend(vla, q, c.to(DEV), table, [n], [m], see, n_q, n_kv, hd, page, scale, **kw), want, bound, str(kw))
+
+

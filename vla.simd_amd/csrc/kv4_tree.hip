@@ -346,10 +346,12 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_tree_kernel(Kv4TreeArgs ta, Kv4
 // keys in fp16 too, in one part instead of two.) Weights are 2^9 times as large, up to 2^15, and where a
 // row's are all below 2^-16 of its largest they are raised for that stage, the sums with them, so that
 // a weight is off by 2^-22 of itself or by 2^-18 of the stage's largest, whichever is more. The first
-// stage with other values, with what may not be finite or without a page turns the block to bf16 parts for good.
+// stage with other values, with what may not be finite, without a page or with a row that is further down than
+// sums can be raised turns the block to bf16 parts for good. (Scores of a deviation of 4, or a key 20 above all others, raise sums in
+// most stages: 2 x 131072 in bf16 588 and 579 us for 497; 80 above, in bf16 parts 725.)
 //
-// 2 x 131072 keys, 64 new tokens, 32 heads on 8 of 128: 518 us in fp16, 507 in bf16 (542 TFLOP/s of the product's own
-// operations); 48 mixed up to 8192, 32 new, bf16: 176. What bounds it are the vector instructions (191 for 32 rows and keys) and the matrix
+// 2 x 131072 keys, 64 new tokens, 32 heads on 8 of 128: 513 us in fp16, 497 in bf16 (552 TFLOP/s of the product's own
+// operations); 48 mixed up to 8192, 32 new, bf16: 175. What bounds it are the vector instructions (191 for 32 rows and keys) and the matrix
 // instructions (48, in bf16 32) together: a SIMD's two waves hardly overlap them, nor does conversion between
 // the products of a stage, or the exponentials of its second tile between those of the first, gain anything.
 
@@ -388,7 +390,6 @@ struct TreeGeo {
     static constexpr bool KHALF = !__is_same(T, bf16_t);      // keys in fp16 too
     static constexpr int W = 4, HD = 32 * NB;
     static constexpr int NQ = 2;                              // row tiles of a wave
-    static constexpr int PF = 2;                              // fp16 parts of weights
     static constexpr int TILES = 2;                           // of a stage
     static constexpr int KU = 2 * NB * TILES, VU = NB * TILES;  // units of a stage: a step's 16 keys of 32 dims, a tile's values of 32 dims
     static constexpr int KN = (KU + W - 1) / W, VN = (VU + W - 1) / W;
@@ -401,7 +402,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
     constexpr int W = G::W, NQ = G::NQ, TILES = G::TILES, HD = G::HD, NT = 2 * NB;
     const Kv4Args& a = ta.kv;
     __shared__ __attribute__((aligned(16))) unsigned char mem[2 * G::STAGE];
-    __shared__ int slow_at, cleaned;  // the first stage that fp16 does not take; whether values were taken out
+    __shared__ int slow_at, redo, cleaned;  // the first stage that fp16 does not take; the first that some wave has left; whether values were taken out
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g = lane >> 4;
@@ -609,7 +610,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
         };
 
         if (threadIdx.x == 0) {
-            slow_at = 0x7fffffff;
+            slow_at = redo = 0x7fffffff;
             cleaned = 0;
         }
         Raw now;
@@ -649,7 +650,8 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
 #pragma unroll
         for (int z = 0; z < NQ; z++) m[z] = -INFINITY, l[z] = 0.0f;
         // The reference only has to keep the weights in range: it follows when a row's maximum has passed it by `most`, to `lead` below
-        // that, so most tiles rescale nothing. (Past 2^26, where fp32's steps are above 2 `lead`, it takes the maximum itself.)
+        // that, so most tiles rescale nothing. It is a whole number, to which others are added without rounding up to 2^24. (Past 2^26,
+        // where fp32's steps are above 2 `lead`, it takes the maximum itself.)
         auto follow = [&](const float (&top)[NQ], float lead, float most) {
             bool grown = false;
 #pragma unroll
@@ -657,7 +659,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
             if (__builtin_expect(__any(grown), 0)) {
 #pragma unroll
                 for (int z = 0; z < NQ; z++) {
-                    const float mx = rows_max(top[z]), to = mx - lead;
+                    const float mx = rows_max(top[z]), to = floorf(mx - lead);
                     const float mn = fmaxf(m[z], mx - to > most ? mx : to);
                     const float alpha = __builtin_amdgcn_exp2f(m[z] - (mn == -INFINITY ? 0.0f : mn));
                     m[z] = mn;
@@ -673,8 +675,11 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
         // A wave's tiles of a stage, in fp16. Weights come from the rounded scores that their reference was taken from, and it is
         // subtracted as it is: from unrounded ones, or with the 2^9 added to it first, they would pass fp16's range
         // where scores pass 2^24 (48 trees of 32 176 us for 171).
-        auto fast_step = [&](const unsigned char* buf, int k0) {
+        int next = 0x7fffffff;  // the stage from which on this wave leaves all of them to the parts in bf16
+        auto fast_step = [&](int stage) {
 #pragma clang fp contract(off)
+            const unsigned char* buf = mem + (stage & 1) * G::STAGE + lane * 16;
+            const int k0 = k_begin + stage * TILES * kTile;
             v4f s[NQ][TILES][2] = {};
 #pragma unroll
             for (int ch = 0; ch < TILES; ch++)
@@ -710,16 +715,20 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
                 top[z] = mx;
             }
             follow(top, 9.0f, 15.0f);
-            // Where the weights of a row are all below 2^-16 of its largest, its sums are raised for these tiles.
+            // Where the weights of a row are all below 2^-16 of its largest, its sums are raised by what is missing for this stage, as
+            // far as fp32's range goes (sums are below 2^26 times the number of keys). What lies further down is left to the parts in bf16.
+            float mu[NQ], up[NQ];
             bool low = false;
 #pragma unroll
-            for (int z = 0; z < NQ; z++) low |= top[z] - m[z] < -7.0f && top[z] > -INFINITY;
+            for (int z = 0; z < NQ; z++) {
+                mu[z] = m[z] == -INFINITY ? 0.0f : m[z];
+                low |= top[z] - m[z] < -7.0f && top[z] > -INFINITY;
+            }
             low = __any(low);
-            float up[NQ];
-            auto raise = [&](float sign) {
+            auto raise = [&](int sign) {
 #pragma unroll
                 for (int z = 0; z < NQ; z++) {
-                    const float f = __builtin_amdgcn_exp2f(sign * up[z]);
+                    const float f = __builtin_ldexpf(1.0f, sign * (int)up[z]);
                     l[z] *= f;
 #pragma unroll
                     for (int t = 0; t < NT; t++)
@@ -727,40 +736,44 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
                         for (int r = 0; r < 4; r++) o[z][t][r] *= f;
                 }
             };
-#pragma unroll
-            for (int z = 0; z < NQ; z++) up[z] = 0.0f;
             if (__builtin_expect(low, 0)) {
+                const float up_most = 106.0f - run.lift;  // 100 less log2 of the keys
+                bool far = false;
 #pragma unroll
                 for (int z = 0; z < NQ; z++) {
-                    const float k = floorf(m[z] - rows_max(top[z]) + 9.0f);
-                    up[z] = k > 40.0f ? 40.0f : k > 0.0f ? k : 0.0f;
+                    const float mx = rows_max(top[z]), k = mx > -INFINITY ? floorf(m[z] - mx + 9.0f) : 0.0f, base = mu[z];
+                    mu[z] -= fminf(fmaxf(k, 0.0f), up_most);
+                    up[z] = base - mu[z];
+                    far |= k > up_most + 16.0f || mx - mu[z] > 15.0f;  // (the latter where the reference had to be rounded)
                 }
-                raise(1.0f);
+                if (__any(far)) {
+                    next = stage;
+                    if (lane == 0) {
+                        atomicMin(&slow_at, stage + 2);  // (which the others find out behind the next barrier)
+                        atomicMin(&redo, stage);
+                    }
+                    return;
+                }
+                raise(1);
             }
 #pragma unroll
             for (int ch = 0; ch < TILES; ch++) {
-                U4 pw[NQ][G::PF];
+                U4 pw[NQ][2];
 #pragma unroll
                 for (int z = 0; z < NQ; z++) {
-                    const float mu = m[z] == -INFINITY ? 0.0f : m[z];
                     float x[8], sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        x[i] = __builtin_amdgcn_exp2f(s[z][ch][i >> 2][i & 3] - mu + up[z]);
+                        x[i] = __builtin_amdgcn_exp2f(s[z][ch][i >> 2][i & 3] - mu[z]);
                         sum += x[i];
                     }
                     l[z] += sum;
 #pragma unroll
-                    for (int q = 0; q < G::PF; q++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            pw[z][q].u[j] = pack_half(x[2 * j], x[2 * j + 1]);
-                            if (q + 1 < G::PF) {
-                                const v2h h = __builtin_bit_cast(v2h, pw[z][q].u[j]);
-                                x[2 * j] -= (float)h[0];
-                                x[2 * j + 1] -= (float)h[1];
-                            }
-                        }
+                    for (int j = 0; j < 4; j++) {
+                        pw[z][0].u[j] = pack_half(x[2 * j], x[2 * j + 1]);
+                        const v2h h = __builtin_bit_cast(v2h, pw[z][0].u[j]);
+                        pw[z][1].u[j] = pack_half(x[2 * j] - (float)h[0], x[2 * j + 1] - (float)h[1]);
+                    }
                 }
                 const unsigned char* vbuf = buf + G::KBYTES + ch * NB * 2048;
 #pragma unroll
@@ -769,10 +782,10 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
 #pragma unroll
                     for (int z = 0; z < NQ; z++)
 #pragma unroll
-                        for (int q = G::PF - 1; q >= 0; q--) o[z][d] = mfma16h(v, pw[z][q], o[z][d]);
+                        for (int q = 1; q >= 0; q--) o[z][d] = mfma16h(v, pw[z][q], o[z][d]);
                 }
             }
-            if (__builtin_expect(low, 0)) raise(-1.0f);
+            if (__builtin_expect(low, 0)) raise(-1);
         };
         // one tile of any values and masks, in bf16: fp16 queries and all weights in two parts
         auto slow_step = [&](const unsigned char* buf, int tile, int k0, bool there) {
@@ -860,11 +873,13 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
                 load(j + 1, pages, now);
                 pages = pages_of(j + 2);
             }
-            const int k0 = k_begin + i * TILES * kTile;
-            if (i >= 0) fast_step(mem + (i & 1) * G::STAGE + lane * 16, k0);
+            if (i >= 0 && i < next) fast_step(i);
             i = j;
         }
-        // what is left, from stage i on: sums are of weights 2^-lift as large
+        __syncthreads();
+        next = next < i ? next : i;
+        i = __builtin_amdgcn_readfirstlane(redo) < i ? __builtin_amdgcn_readfirstlane(redo) : i;
+        // what is left, from stage i on, for a wave from `next` on: sums are of weights 2^-lift as large
         const float to_slow = __builtin_amdgcn_exp2f(-run.lift);
         if (i < stages) {
 #pragma unroll
@@ -885,7 +900,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
 #pragma unroll 1
                 for (int ch = 0; ch < TILES; ch++) {
                     const int k0 = k_begin + (i * TILES + ch) * kTile;
-                    if (k0 < k_end) slow_step(mem + (i & 1) * G::STAGE + lane * 16, ch, k0, !(gone >> ch & 1u));
+                    if (i >= next && k0 < k_end) slow_step(mem + (i & 1) * G::STAGE + lane * 16, ch, k0, !(gone >> ch & 1u));
                 }
                 if (++i >= stages) break;
             }
