@@ -235,3 +235,30 @@ def test_tree_attention_far_below_sinks_of_some_rows(vla, dtype, below, late):
         ref.within(_attend(vla, q, c.to(DEV), table, [n], [m], see, n_q, n_kv, hd, page, scale, **kw), want, bound, str(kw))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,inter", [(64, False), (128, True), (192, False)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_rope_append_infinities_under_a_norm(vla, dtype, hd, inter, bad):
+    """A row with an infinity has an infinite norm: its finite values become zeros, the infinite one and the other of its pair NaN, in
+    queries and in keys; a NaN makes the whole head NaN."""
+    new, n_q, n_kv, page, rot = [6], 2, 2, 32, 32
+    q, k, v, lens, table, cache = _append_case(vla, new, 0, n_q, n_kv, hd, page, dtype, 8)
+    w = torch.full((hd,), 1.5)
+    q[1, 3], k[2, hd + 5], k[4, 0] = bad, bad, bad
+    pos = torch.tensor([3, 7, 11, 0, 2, 900], dtype=torch.int32)
+    f = dref.freqs(rot)
+    qo, ko = torch.empty_like(q, device=DEV), torch.empty_like(k, device=DEV)
+    vla.rope_kv4_append_dev(qo, cache, q.to(DEV), k.to(DEV), v.to(DEV), n_q, n_kv, hd, page, table.to(DEV), _i32(lens), _i32([0, 6]), f.to(DEV),
+                            pos=pos.to(DEV), interleaved=inter, q_weight=w.to(DEV), k_weight=w.to(DEV), k_out=ko)
+    for name, x, got, heads in (("q", q, qo, n_q), ("k", k, ko, n_kv)):
+        want, mag = dref.rotated(x, heads, hd, pos, f, 1.0, inter, w, 1e-6)
+        assert int(want.isnan().sum()) > 0
+        mag = torch.where(torch.isfinite(mag), mag, torch.zeros_like(mag))
+        bound = ref.rounding(torch.where(want.isnan(), torch.zeros_like(want), want), dtype) + 28 * ref.U * mag
+        ref.within(got, want.flatten(1), bound.flatten(1), name)
+    kr, _ = dref.rotated(k, n_kv, hd, pos, f, 1.0, inter, w, 1e-6)
+    kb, vb = (torch.empty(6, n_kv * hd, dtype=F32, device=DEV) for _ in range(2))
+    vla.kv4_gather_dev(kb, vb, cache, n_kv, hd, page, table.to(DEV), _i32([0, 6]))
+    ref.within(kb, ref.values(*ref.quantize(kr)).flatten(1), torch.zeros(6, n_kv * hd, dtype=torch.float64), "cached")
+
+

@@ -58,11 +58,12 @@ __device__ __forceinline__ float value_of(const Words& x, int e) {
     else return to_f32(__builtin_bit_cast(T, (unsigned short)(x.w[e >> 1] >> (16 * (e & 1)))));
 }
 
-// 1 / sqrt(x) to the last bits of a double: the hardware's number and two steps of Newton's
+// 1 / sqrt(x) to the last bits of a double: the hardware's number and two steps of Newton's. (Their factor is about 1; where
+// x is infinite it is NaN, and the maximum leaves the 0 as it is. A choice of results would take registers that the fourth wave needs.)
 __device__ __forceinline__ double rsqrt_wide(double x) {
     double y = __builtin_amdgcn_rsq(x);
 #pragma unroll
-    for (int i = 0; i < 2; i++) y = y * fma(-0.5 * x * y, y, 1.5);
+    for (int i = 0; i < 2; i++) y = y * fmax(fma(-0.5 * x * y, y, 1.5), 0.5);
     return y;
 }
 
