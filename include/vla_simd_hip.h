@@ -546,7 +546,7 @@ VLA_API int32_t vla_rope_freqs(double* freqs, double* magnitude, int32_t rot_dim
  * the head stay. Queries go to q_out (n_q may be 0), keys to k_out unless it is NULL, keys and V into the
  * cache as vla_kv4_append_dev writes rows, but from the rotated keys in 64 bits, before they are rounded to their
  * type (a value past fp32's range counts as infinite). cache NULL: nothing is stored, V, table and the page
- * sizes are not used. q_out may be q, k_out may be K. head_dim as for the cache; fewer than 2^26 - 3
+ * sizes are not used. q_out may be q, k_out may be K (at the same stride). head_dim as for the cache; fewer than 2^26 - 3
  * rows. */
 VLA_API int32_t vla_rope_kv4_append_dev(void* q_out, int64_t ldqo, void* k_out, int64_t ldko, void* cache,
                                         int32_t n_pages, int32_t page_size, const void* q, int64_t ldq,

@@ -343,8 +343,12 @@ void launch_rope_kv4_append(RopeAppendArgs a, hipStream_t st) {
     if (a.n_q) {
         check_strided(a.q, a.ldq, a.n_q, c, "queries");
         check_strided(a.q_out, a.ldqo, a.n_q, c, "q_out");
+        VLA_REQUIRE(a.q_out != a.q || a.ldqo == a.ldq || c.total == 1, "rope_kv4_append: q_out over q needs the same stride");
     }
-    if (a.k_out) check_strided(a.k_out, a.ldko, c.n_kv, c, "k_out");
+    if (a.k_out) {
+        check_strided(a.k_out, a.ldko, c.n_kv, c, "k_out");
+        VLA_REQUIRE(a.k_out != c.K || a.ldko == c.ldk || c.total == 1, "rope_kv4_append: k_out over the keys needs the same stride");
+    }
     if (c.cache) {
         VLA_REQUIRE(c.n_pages > 0 && aligned(c.cache, 16), "rope_kv4_append: the cache must hold a page and be 16-byte aligned");
         VLA_REQUIRE(c.table && c.ld_table > 0, "rope_kv4_append: page table missing");
