@@ -10,7 +10,7 @@ import torch
 
 import draft_ref as dref
 import serving_ref as ref
-from test_gpu_draft import _append_case, _attend, _cache_image, _masks
+from test_gpu_draft import _append_case, _attend, _masks
 from test_gpu_serving import BF16, DEV, F16, F32, TYPES, _decode_case, _dev, _gen, _i32, _rows, _starts
 
 pytestmark = pytest.mark.gpu
@@ -260,5 +260,64 @@ def test_rope_append_infinities_under_a_norm(vla, dtype, hd, inter, bad):
     kb, vb = (torch.empty(6, n_kv * hd, dtype=F32, device=DEV) for _ in range(2))
     vla.kv4_gather_dev(kb, vb, cache, n_kv, hd, page, table.to(DEV), _i32([0, 6]))
     ref.within(kb, ref.values(*ref.quantize(kr)).flatten(1), torch.zeros(6, n_kv * hd, dtype=torch.float64), "cached")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_q,n_kv,hd,rot,inter,norm,rows", [
+    (4, 2, 64, 64, False, True, 5000), (2, 1, 96, 48, True, True, 3000), (3, 1, 192, 176, False, True, 2600), (1, 1, 128, 128, True, False, 7000),
+    (2, 2, 32, 24, False, True, 14000), (1, 1, 32, 16, True, True, 14000), (2, 1, 256, 64, False, False, 2000), (6, 2, 96, 96, False, False, 2500),
+])
+def test_rope_append_forms_of_many_rows(vla, dtype, n_q, n_kv, hd, rot, inter, norm, rows):
+    """Two to sixteen tokens a block, in every form: norms, neighbours, part of a head, heads whose lanes a group does not fill,
+    keys as rows, in place; positions given and of the sequences themselves."""
+    r = random.Random(hd + rot)
+    page, past, new = 64, 5, []
+    while sum(new) < rows:
+        new.append(r.choice([0, 1, 2, 17, 130, 900]))
+    q, k, v, lens, table, cache = _append_case(vla, new, past, n_q, n_kv, hd, page, dtype, 5)
+    total, g = sum(new), _gen(rot)
+    wq, wk = (1 + 0.2 * torch.randn(hd, generator=g) if norm else None for _ in range(2))
+    pos = torch.cat([torch.arange(past, past + n) for n in new]).to(torch.int32)
+    f, mag = dref.freqs(rot), 1.25
+    kr, kmag = dref.rotated(k, n_kv, hd, pos, f, mag, inter, wk, float(torch.tensor(1e-5)))
+    qr, qmag = dref.rotated(q, n_q, hd, pos, f, mag, inter, wq, float(torch.tensor(1e-5)))
+    start, codes = _starts(new), ref.values(*ref.quantize(kr)).flatten(1)
+    vals = ref.values(*ref.quantize(v.reshape(total, n_kv, hd))).flatten(1)
+    for given in (pos.to(DEV), None):
+        cache.fill_(0xEE)
+        dq, dk, qo, ko = q.to(DEV), k.to(DEV), torch.full_like(q, 5.0, device=DEV), torch.full_like(k, 5.0, device=DEV)
+        args = (v.to(DEV), n_q, n_kv, hd, page, table.to(DEV), _i32(lens), _i32(start), f.to(DEV), given, mag, inter, _dev(wq), _dev(wk), 1e-5)
+        vla.rope_kv4_append_dev(qo, cache, dq, dk, *args, k_out=ko)
+        ref.within(ko, kr.flatten(1), (ref.rounding(kr, dtype) + 2.0 ** -30 * kmag).flatten(1), "k")
+        ref.within(qo, qr.flatten(1), (ref.rounding(qr, dtype) + 28 * ref.U * qmag).flatten(1), "q")
+        kb, vb = (torch.empty(total, n_kv * hd, dtype=F32, device=DEV) for _ in range(2))
+        vla.kv4_gather_dev(kb, vb, cache, n_kv, hd, page, table.to(DEV), _i32(start), _i32([past] * len(new)))
+        assert torch.equal(kb.cpu().double(), codes) and torch.equal(vb.cpu().double(), vals)
+        again = torch.full_like(cache, 0xEE)
+        vla.rope_kv4_append_dev(dq, again, dq, dk, *args, k_out=dk)
+        assert torch.equal(dq, qo) and torch.equal(dk, ko) and torch.equal(again, cache)
+
+
+@pytest.mark.parametrize("n_seqs", [1023, 1024, 3000])
+def test_rope_append_many_sequences(vla, n_seqs):
+    """Offsets that LDS has room for, and more, searched where they are."""
+    r = random.Random(n_seqs)
+    n_q, n_kv, hd, page, past, dtype = 2, 1, 32, 32, 3, BF16
+    new = [r.choice([0, 1, 1, 2, 5]) for _ in range(n_seqs)]
+    q, k, v, lens, table, cache = _append_case(vla, new, past, n_q, n_kv, hd, page, dtype, 6)
+    total, start = sum(new), _starts(new)
+    pos = torch.cat([torch.arange(past, past + n) for n in new]).to(torch.int32)
+    f = dref.freqs(hd)
+    kr, _ = dref.rotated(k, n_kv, hd, pos, f, 1.0, False, None, 0.0)
+    qr, qmag = dref.rotated(q, n_q, hd, pos, f, 1.0, False, None, 0.0)
+    for given in (pos.to(DEV), None):
+        cache.fill_(0xEE)
+        qo = torch.empty_like(q, device=DEV)
+        vla.rope_kv4_append_dev(qo, cache, q.to(DEV), k.to(DEV), v.to(DEV), n_q, n_kv, hd, page, table.to(DEV), _i32(lens), _i32(start), f.to(DEV), pos=given)
+        ref.within(qo, qr.flatten(1), (ref.rounding(qr, dtype) + 28 * ref.U * qmag).flatten(1), "q")
+        kb, vb = (torch.empty(total, n_kv * hd, dtype=F32, device=DEV) for _ in range(2))
+        vla.kv4_gather_dev(kb, vb, cache, n_kv, hd, page, table.to(DEV), _i32(start), _i32([past] * n_seqs))
+        assert torch.equal(kb.cpu().double(), ref.values(*ref.quantize(kr)).flatten(1))
+        assert torch.equal(vb.cpu().double(), ref.values(*ref.quantize(v.reshape(total, n_kv, hd))).flatten(1))
 
 
