@@ -321,3 +321,26 @@ def test_rope_append_many_sequences(vla, n_seqs):
         assert torch.equal(vb.cpu().double(), ref.values(*ref.quantize(v.reshape(total, n_kv, hd))).flatten(1))
 
 
+@pytest.mark.parametrize("new", [[700, 513], [64, 512, 3, 1469], [512], [513], [1024, 0, 1]])
+@pytest.mark.parametrize("words", [1, 17, 46, 50])
+def test_tree_of_long_sequences(vla, new, words):
+    """Averages on both sides of 512 rows: parents of all kinds, further roots, too few and too many words."""
+    r = random.Random(sum(new))
+    parents = []
+    for n in new:
+        p = [-1 if i == 0 else r.choice([i - 1, i - 1, i - 1, max(0, i - 70), r.randrange(i)]) for i in range(n)]
+        for i, x in ((n // 3, -1), (n // 2, n // 2), (2 * n // 3, 2 ** 31 - 1), (n - 1, -(2 ** 31))) if n > 9 else ():
+            p[i] = x
+        parents.append(p)
+    lens, start, total = [n + 11 for n in new], _starts(new), sum(new)
+    for parent in (parents, None):
+        pos = torch.full((total + 2,), 77, dtype=torch.int32, device=DEV)
+        see = torch.full((total + 2, words), 77, dtype=torch.int32, device=DEV)
+        vla.draft_tree_dev(pos, see, _i32([x for p in parents for x in p] + [0, 0]) if parent else None, _i32(lens), _i32(start))
+        for s, n in enumerate(new):
+            bits, depth = dref.tree(parents[s] if parent else None, n)
+            assert pos[start[s]:start[s + 1]].tolist() == [11 + d for d in depth]
+            assert torch.equal(see[start[s]:start[s + 1]].cpu(), dref.words(bits, words)) or n == 0
+        assert bool((pos[total:] == 77).all()) and bool((see[total:] == 77).all())
+
+
