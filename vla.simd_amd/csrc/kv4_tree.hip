@@ -378,6 +378,16 @@ __device__ __forceinline__ unsigned pack_half(float a, float b) {
     return __builtin_bit_cast(unsigned, __builtin_convertvector(x, v2h));
 }
 
+// x less the lower or upper half of two fp16 numbers, exact for what was rounded from it: one instruction, where the compiler
+// takes a conversion and a subtraction (48 trees of 32 175 us, now 172; 2 x 131072 in fp16 515, now 501)
+template <int UPPER>
+__device__ __forceinline__ float less_half(float x, unsigned h) {
+    float d;
+    if constexpr (UPPER) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(x));
+    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(x));
+    return d;
+}
+
 // a barrier for what is in LDS: __syncthreads would wait for the loads of later stages too
 __device__ __forceinline__ void lds_barrier() {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -771,8 +781,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         pw[z][0].u[j] = pack_half(x[2 * j], x[2 * j + 1]);
-                        const v2h h = __builtin_bit_cast(v2h, pw[z][0].u[j]);
-                        pw[z][1].u[j] = pack_half(x[2 * j] - (float)h[0], x[2 * j + 1] - (float)h[1]);
+                        pw[z][1].u[j] = pack_half(less_half<0>(x[2 * j], pw[z][0].u[j]), less_half<1>(x[2 * j + 1], pw[z][0].u[j]));
                     }
                 }
                 const unsigned char* vbuf = buf + G::KBYTES + ch * NB * 2048;
