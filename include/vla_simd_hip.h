@@ -533,7 +533,9 @@ VLA_API int32_t vla_draft_tree_dev(int32_t* pos, uint32_t* see, int32_t ld_see, 
  *   LINEAR  all divided by factor (position interpolation);
  *   BASE    of the base times factor^(rot_dim / (rot_dim - 2));
  *   PARTS   a pair that makes `turns` turns over `trained` positions is divided by factor where turns <= low,
- *           left where turns >= high, and mixed in between by (turns - low) / (high - low).
+ *           left where turns >= high, and mixed in between by (turns - low) / (high - low). (Mixing over
+ *           the pairs' numbers, between borders rounded to whole pairs, gives other angles: a model
+ *           trained with those needs them, and the calls below take any.)
  * magnitude (may be NULL): 1, for PARTS 0.1 ln(factor) + 1, to scale the rotated values by. */
 typedef enum { VLA_ROPE_PLAIN = 0, VLA_ROPE_LINEAR = 1, VLA_ROPE_BASE = 2, VLA_ROPE_PARTS = 3 } vla_rope_scaling;
 VLA_API int32_t vla_rope_freqs(double* freqs, double* magnitude, int32_t rot_dim, double base,

@@ -975,7 +975,7 @@ def rope_kv4_append_dev(q_out, cache, q, k, v, n_q, n_kv, head_dim, page_size, t
     and values into the cache as the newest tokens of their sequences, in one pass. freqs: a float64 tensor
     [rot_dim / 2] on the GPU (rope_freqs); pairs are (i, i + rot_dim / 2), or neighbours where interleaved. pos [total]
     int32 (None: a token's number in its sequence). k_out takes the rotated keys as rows too. cache, v and table None:
-    only rotated; q and q_out None with n_q 0. q_out may be q, k_out may be k."""
+    only rotated; q and q_out None with n_q 0. q_out may be q, k_out may be k, at the same stride."""
     dt, dtype, total, n = _type_id(k), k.dtype, k.shape[0], _seqs_of("start", start)
     ldk = _row_ld("k", k, total, n_kv * head_dim, dtype)
     ldq = ldqo = ldv = ldko = pages = ld = 0

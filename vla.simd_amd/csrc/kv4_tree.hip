@@ -348,11 +348,11 @@ __global__ __launch_bounds__(W * 64, 2) void kv4_tree_kernel(Kv4TreeArgs ta, Kv4
 // a weight is off by 2^-22 of itself or by 2^-18 of the stage's largest, whichever is more. The first
 // stage with other values, with what may not be finite, without a page or with a row that is further down than
 // sums can be raised turns the block to bf16 parts for good. (Scores of a deviation of 4, or a key 20 above all others, raise sums in
-// most stages: 2 x 131072 in bf16 588 and 579 us for 497; 80 above, in bf16 parts 725.)
+// most stages: 2 x 131072 in bf16 579 and 569 us for 488; 80 above, in bf16 parts 731.)
 //
-// 2 x 131072 keys, 64 new tokens, 32 heads on 8 of 128: 513 us in fp16, 497 in bf16 (552 TFLOP/s of the product's own
-// operations); 48 mixed up to 8192, 32 new, bf16: 175. What bounds it are the vector instructions (191 for 32 rows and keys) and the matrix
-// instructions (48, in bf16 32) together: a SIMD's two waves hardly overlap them, nor does conversion between
+// 2 x 131072 keys, 64 new tokens, 32 heads on 8 of 128: 501 us in fp16, 488 in bf16 (563 TFLOP/s of the product's own
+// operations); 48 mixed up to 8192, 32 new, bf16: 172. What bounds it are the vector instructions (257 for 32 rows and keys) and the matrix
+// instructions (48) together: a SIMD's two waves hardly overlap them, nor does conversion between
 // the products of a stage, or the exponentials of its second tile between those of the first, gain anything.
 
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
@@ -684,7 +684,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tree_shared_kernel(Kv4TreeArgs ta,
 
         // A wave's tiles of a stage, in fp16. Weights come from the rounded scores that their reference was taken from, and it is
         // subtracted as it is: from unrounded ones, or with the 2^9 added to it first, they would pass fp16's range
-        // where scores pass 2^24 (48 trees of 32 176 us for 171).
+        // where scores pass 2^24 (48 trees of 32 took 171 us without this, 176 with it).
         int next = 0x7fffffff;  // the stage from which on this wave leaves all of them to the parts in bf16
         auto fast_step = [&](int stage) {
 #pragma clang fp contract(off)
@@ -993,11 +993,12 @@ int64_t row_blocks(int64_t most, int total_q, int n_seqs, int n_q, int n_kv, int
 
 // Which kernel takes a call, and the row tiles of one of its blocks. Every row tile that has keys to itself reads and converts
 // them again: two in registers (heads up to 128 in 16-bit types) halve that, from five on four waves share
-// what is converted. Measured, us, 48 sequences mixed up to 8192 keys, 32 heads on 8 of 128, bf16, one in registers | two |
-// shared: 4 new tokens (one row tile) 50 | 67 | 127, 8 (two) 84 | 74 | 131, 16 (four) 118 | 114 | 137, 20 (five) - | 155 | 141, 32 (eight)
-// 200 | 197 | 151; 2 x 131072, 8 new 90 | 80 | 203, 16 new 158 | 132 | 206, 64 new 625 | 507 | 494 (fp16). Heads
+// what is converted. Measured, us, 48 sequences mixed up to 8192 keys, 32 heads on 8, bf16, one in registers | two |
+// shared: heads of 128, 4 new tokens (one row tile) 49 | 67 | 150, 8 (two) 86 | 74 | 154, 16 (four) 118 | 116 | 160, 20 (five) 146 | 158 | 163, 24 176 |
+// 162 | 165, 32 (eight) 204 | 201 | 172; of 96, 16 137 | 112 | 141, 20 159 | 159 | 143; of 64, 16 83 | 98 | 110, 20 107 | 120 | 113, 32 152 | 139 | 121; of
+// 32, 16 84 | 81 | 92, 20 97 | 107 | 94; 2 x 131072, heads of 128, 16 new 167 | 144 | 251, 20 258 | 262 | 252, of 64 125 | 101 | 164, 195 | 184 | 165; fp16 alike. Heads
 // above 128 leave a wave no room for two row tiles, and sharing for four gains nothing: of 256, 16 new 215 | - | 230, 32 new
-// 380 | - | 418, 64 new 706 | - | 1157. (Two waves sharing for four row tiles of 128: 117 and 164 for 114 and 132.)
+// 385 | - | 418, 64 new 706 | - | 1157. (Two waves sharing for four row tiles of 128: 117 and 164 for 114 and 132.)
 constexpr int kSharedTiles = 5, kSharedRows = 8;  // row tiles from which on waves share, and of a block then
 int rows_per_block(int total_q, int max_new, int n_q, int n_kv, int head_dim, bool half) {
     if (!half || head_dim > 128) return 1;
@@ -1008,8 +1009,9 @@ int rows_per_block(int total_q, int max_new, int n_q, int n_kv, int head_dim, bo
 // How a call runs, from sizes the host knows: equal runs of tiles (and a second kernel), or a
 // block per sequence and row tiles. In registers as the attention of a causal chunk, by the same measure: a block's steps against the blocks
 // that the card is short of. Shared tiles: runs, each of at least two stages, unless blocks of sequences fill the card four times (us, runs |
-// sequences: 4 x 1000 keys, 32 new 21 | 47, 16 x 3000, 64 new 103 | 126, 48 mixed up to 8192, 32 new 151 | 337, 100 new 488 | 585, 200
-// new 950 | 898, 64 x 4000, 16 new 205 | 195); no more runs than are under way at once (2 x 131072, 200 new: 9 runs 1690, 10 2590).
+// sequences, heads of 128: 4 x 1000 keys, 32 new 30 | 54, 16 x 3000, 64 new 127 | 149, 48 mixed up to 8192, 32 new 180 | 407, 100 new 581 | 703, 200
+// new 1023 | 1077, 64 x 4000, 64 new 507 | 475, 120 new 999 | 927, 200 x 800, 40 new 419 | 359; of 64 21 | 37, 90 | 97, 128 | 270, 402 | 492, 708 | 711, 341 |
+// 309, 674 | 603, 301 | 237); no more runs than are under way at once (2 x 131072, 200 new: 9 runs 1692, 10 2614).
 Kv4Run plan(int total_q, int n_seqs, int max_new, int64_t max_len, int n_q, int n_kv, int head_dim, int nq) {
     Kv4Run r{};
     max_new = max_new < total_q ? max_new : total_q;

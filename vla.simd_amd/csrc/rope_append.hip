@@ -29,7 +29,7 @@ namespace hip {
 namespace {
 
 constexpr int kMaxTokens = 16;   // of a block
-constexpr int kTableEntries = 1024;
+constexpr int kTableEntries = 1024;  // sines and cosines of a block: half of the values that turn for each token (16 tokens of 128 fill it)
 constexpr int kCus = 256;
 
 // d for a later rounding to fewer bits than an fp32 has: cut off, the last bit set where anything
