@@ -322,7 +322,7 @@ def test_rope_append_many_sequences(vla, n_seqs):
 
 
 @pytest.mark.parametrize("new", [[700, 513], [64, 512, 3, 1469], [512], [513], [1024, 0, 1]])
-@pytest.mark.parametrize("words", [1, 17, 46, 50])
+@pytest.mark.parametrize("words", [1, 16, 17, 46, 50])
 def test_tree_of_long_sequences(vla, new, words):
     """Averages on both sides of 512 rows: parents of all kinds, further roots, too few and too many words."""
     r = random.Random(sum(new))

@@ -488,10 +488,13 @@ void launch_draft_tree(const DraftTreeArgs& a, hipStream_t st) {
     if (a.n_seqs == 0 || a.total == 0) return;
     VLA_REQUIRE(a.pos && a.see && a.lens && a.start, "draft_tree: null buffer");
     VLA_REQUIRE(a.pos != a.parent, "draft_tree: pos must not be parent, which other rows still read");
-    // A wave for each sequence up to 512 rows on average, by the depth a thread for each row beyond. Wave | threads, us, 64 sequences:
+    // A wave for each sequence where they are short on average, or up to 512 rows with words for no more: a long one among short
+    // ones keeps one wave busy with its words (48 sequences, one a chain of 8192: 3295 us, by threads 1548). Otherwise, by the depth, a thread for each
+    // row. Wave | threads, us, 64 sequences:
     // chains of 65 rows 3.9 | 15, 256 7.9 | 50, 512 21 | 101, 1024 67 | 203, 4096 925 | 1095; parents among the 8 before of 256 7.4 | 15,
     // 512 21 | 29, 1024 66 | 57, 4096 939 | 349; among all before of 256 6.7 | 6.1, 512 19 | 9.7, 1024 67 | 17. One sequence: the same less a tenth.
-    if (a.total <= (int64_t)512 * a.n_seqs) draft_tree_wave_kernel<<<a.n_seqs < 1 << 20 ? a.n_seqs : 1 << 20, 64, 0, st>>>(a);
+    if (a.total <= (int64_t)64 * a.n_seqs || (a.ld_see <= 16 && a.total <= (int64_t)512 * a.n_seqs))
+        draft_tree_wave_kernel<<<a.n_seqs < 1 << 20 ? a.n_seqs : 1 << 20, 64, 0, st>>>(a);
     else draft_tree_rows_kernel<<<(a.total + 255) / 256, 256, 0, st>>>(a);
     VLA_LAUNCH_CHECK();
 }
